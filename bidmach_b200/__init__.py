@@ -7,10 +7,14 @@ negative-sampling minibatch path behind the reference's CUMACH interface.
                evalbatch) above the C-ABI library
 ``Learner`` / ``ParLearner``  the minibatch schedule that drives it
 ``MatSource`` / ``FileSource``  minibatches from memory or from corpus files
+``EmbedRows``  rows of a matrix by ids, and their gradient
+``AdamW``      one AdamW step over many tensors, moments in 32 or 8 bits
 ``matio`` / ``modelio``  BIDMat matrix files, checkpoints, Google word2vec files
 """
 from .cumach import CUMACH, CUMACHSlice, cuda_error_string  # noqa: F401
 from .word2vec import Word2Vec  # noqa: F401
 from .learner import Learner, ParLearner, MatSource  # noqa: F401
 from .filesource import FileSource, FileSourceOpts  # noqa: F401
+from .embed import EmbedRows  # noqa: F401
+from .adamw import AdamW  # noqa: F401
 from . import matio, modelio  # noqa: F401

@@ -42,6 +42,17 @@ class W2VTiming(C.Structure):
                 ("groups", C.c_int64), ("eval_pairs", C.c_int64), ("eval_groups", C.c_int64)]
 
 
+class W2VAdamwTensor(C.Structure):
+    """``w2v_adamw_tensor``."""
+    _fields_ = [("p", _P), ("m", _P), ("v", _P), ("mscale", _P), ("vscale", _P), ("n", C.c_int64), ("ptype", _I)]
+
+
+class W2VAdamwOpts(C.Structure):
+    """``w2v_adamw_opts``."""
+    _fields_ = [("lrate", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double),
+                ("wdecay", C.c_double)]
+
+
 # name -> (restype, argtypes); every symbol include/bidmach_b200.h declares
 SIGNATURES = {
     "word2vecPos": (_I, [_I, _I, _I, _P, _P, _P, _P, _P, _F, _F]),
@@ -107,6 +118,13 @@ SIGNATURES = {
     "w2v_set_timing": (_I, [_P, _I]),
     "w2v_get_timing": (_I, [_P, C.POINTER(W2VTiming)]),
     "w2v_launch_count": (C.c_longlong, []),
+    "w2v_embed_rows": (_I, [_P, C.c_int64, _P, C.c_int64, C.c_int64, _I, _I, _P, C.c_int64, _P]),
+    "w2v_embed_grad_workspace": (C.c_int64, [C.c_int64, C.c_int64, _I, _I]),
+    "w2v_embed_grad": (_I, [_P, C.c_int64, _P, C.c_int64, C.c_int64, _I, _I, _P, C.c_int64, _P, C.c_int64, _P]),
+    "w2v_adamw_clock": (_I, [_P, C.c_double, C.c_double, C.c_int64, _P]),
+    "w2v_adamw_step": (_I, [C.POINTER(W2VAdamwTensor), C.POINTER(_P), C.POINTER(_I), _I, _I,
+                            C.POINTER(W2VAdamwOpts), _P, _P, _P]),
+    "w2v_adamw_moments": (_I, [C.POINTER(W2VAdamwTensor), C.POINTER(_P), C.POINTER(_P), _I, _P]),
 }
 
 _lib = None

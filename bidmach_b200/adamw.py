@@ -1,0 +1,190 @@
+"""AdamW over many tensors at once, the updater of the full-vocabulary training path.
+
+The moments are held in fp32 or in 8 bits (codes of one byte, one scale for 256 elements); one
+kernel launch reads and writes every tensor once.  PyTorch supplies memory and streams only.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import dataclasses
+
+import torch
+
+from . import _lib
+from .cumach import cuda_error_string
+
+TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def check(err: int, what: str):
+    if err:
+        raise RuntimeError(f"{what} error " + ("1: arguments refused" if err == 1 else cuda_error_string(err)))
+
+
+class on_device:
+    """Makes ``device`` current, at no cost where it is already."""
+
+    def __init__(self, device: torch.device):
+        self._guard = None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self._guard is not None:
+            self._guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self._guard is not None:
+            self._guard.__exit__(*exc)
+
+
+def stream_of(device: torch.device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+@dataclasses.dataclass
+class Opts:
+    """``lrate`` and the usual constants; ``bits``: 32 or 8 for the moments."""
+    lrate: float = 1e-3
+    beta1: float = 0.9
+    beta2: float = 0.999
+    eps: float = 1e-8
+    wdecay: float = 0.01
+    bits: int = 32
+
+
+class AdamW:
+    """``step(grads)`` applies, to every tensor of ``params`` in place,
+
+        m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,
+        p = p (1 - lrate wdecay) - lrate m / (1 - beta1^t) / (sqrt(v / (1 - beta2^t)) + eps)
+
+    ``params``: contiguous CUDA tensors of one device, fp32, bf16 or fp16, none overlapping another.
+    ``state``, when given, is the state to go on from (its tensors are used in place): ``t`` steps
+    done, and lists ``m`` and ``v`` like the parameters: fp32, or for 8 bits uint8 of as many
+    elements, with lists ``mscale`` and ``vscale`` of fp32, one for every 256 elements.  Without it
+    the moments start at zero.  The arithmetic is fp32; a 16-bit parameter is rounded to nearest
+    once a step, so a step smaller than half of its last place leaves it as it is.
+
+    The step count lives on the device: a captured step counts its replays."""
+
+    Opts = Opts
+
+    def __init__(self, params, opts: Opts | None = None, state: dict | None = None):
+        self.params = list(params)
+        self.opts = opts or Opts()
+        o = self.opts
+        if o.bits not in (8, 32):
+            raise ValueError("bits must be 32 or 8")
+        if not (0 <= o.beta1 < 1 and 0 <= o.beta2 < 1 and o.eps > 0 and o.wdecay >= 0):
+            raise ValueError("need 0 <= beta1, beta2 < 1, eps > 0, wdecay >= 0")
+        if not self.params:
+            raise ValueError("AdamW needs at least one tensor")
+        for p in self.params:
+            if not isinstance(p, torch.Tensor) or p.dtype not in TYPES:
+                raise ValueError("parameters are fp32, bf16 or fp16 tensors")
+            if not p.is_contiguous():
+                raise ValueError("parameters have to be contiguous")
+        spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in self.params if p.numel())
+        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise ValueError("two parameters overlap")
+        if any(not p.is_cuda for p in self.params):
+            raise ValueError("AdamW expects CUDA tensors")
+        self.device = self.params[0].device
+        if any(p.device != self.device for p in self.params):
+            raise ValueError("parameters on more than one device")
+        self.m, self.v, self.mscale, self.vscale, t = self._state(state)
+        n = len(self.params)
+        self._sizes = [p.numel() for p in self.params]
+        self._types = [p.dtype for p in self.params]
+        self._table = (_lib.W2VAdamwTensor * n)()
+        for i, p in enumerate(self.params):
+            self._table[i] = _lib.W2VAdamwTensor(
+                p.data_ptr(), self.m[i].data_ptr(), self.v[i].data_ptr(),
+                self.mscale[i].data_ptr() if self.mscale else 0, self.vscale[i].data_ptr() if self.vscale else 0,
+                p.numel(), TYPES[p.dtype])
+        self._clock = torch.zeros(4, dtype=torch.float64, device=self.device)
+        with on_device(self.device):
+            check(_lib.load().w2v_adamw_clock(self._clock.data_ptr(), o.beta1, o.beta2, t, stream_of(self.device)),
+                  "w2v_adamw_clock")
+
+    def _state(self, state):
+        bits = self.opts.bits
+        dtype = torch.float32 if bits == 32 else torch.uint8
+        blocks = [(p.numel() + 255) // 256 for p in self.params]
+
+        def fresh(sizes, dt):
+            return [torch.zeros(n, dtype=dt, device=self.device) for n in sizes]
+
+        sizes = [p.numel() for p in self.params]
+        if state is None:
+            scales = (fresh(blocks, torch.float32), fresh(blocks, torch.float32)) if bits == 8 else (None, None)
+            return fresh(sizes, dtype), fresh(sizes, dtype), *scales, 0
+
+        def given(name, want, dt):
+            got = list(state[name])
+            if len(got) != len(want):
+                raise ValueError(f"state[{name!r}] has {len(got)} tensors for {len(want)} parameters")
+            for x, n in zip(got, want):
+                if x.dtype != dt or x.numel() != n or x.device != self.device or not x.is_contiguous():
+                    raise ValueError(f"state[{name!r}] wants contiguous {dt} tensors of {self.device}, "
+                                     "as many elements as it describes")
+            return got
+
+        if int(state["t"]) < 0:
+            raise ValueError("state['t'] is negative")
+        scales = (given("mscale", blocks, torch.float32), given("vscale", blocks, torch.float32)) if bits == 8 \
+            else (None, None)
+        return given("m", sizes, dtype), given("v", sizes, dtype), *scales, int(state["t"])
+
+    def step(self, grads, lrate: "float | torch.Tensor | None" = None):
+        """One step.  ``grads``: a tensor for each parameter, same number of elements, contiguous, fp32
+        or the parameter's type.  ``lrate`` replaces the option's: a number, or a one-element fp32
+        tensor of the device, read when the step runs."""
+        n = len(self._sizes)
+        if len(grads) != n:
+            raise ValueError(f"{len(grads)} gradients for {n} parameters")
+        dev, types = self.device, self._types
+        kinds = []
+        for g, size, t in zip(grads, self._sizes, types):
+            d = g.dtype
+            if d is not t and d is not torch.float32:
+                raise ValueError("a gradient is fp32 or of its parameter's type")
+            if g.numel() != size or g.device != dev or not g.is_contiguous():
+                raise ValueError("a gradient has its parameter's device and size and is contiguous")
+            kinds.append(TYPES[d])
+        o = self.opts
+        rate, rate_ptr = o.lrate, None
+        if isinstance(lrate, torch.Tensor):
+            if lrate.dtype != torch.float32 or lrate.numel() != 1 or lrate.device != dev:
+                raise ValueError("lrate: a number or a one-element fp32 tensor of the parameters' device")
+            rate_ptr = lrate.data_ptr()
+        elif lrate is not None:
+            rate = float(lrate)
+        opts = _lib.W2VAdamwOpts(rate, o.beta1, o.beta2, o.eps, o.wdecay)
+        with on_device(dev):
+            check(_lib.load().w2v_adamw_step(self._table, (C.c_void_p * n)(*[g.data_ptr() for g in grads]),
+                                             (C.c_int * n)(*kinds), n, o.bits, C.byref(opts), rate_ptr,
+                                             self._clock.data_ptr(), stream_of(dev)), "w2v_adamw_step")
+
+    def moments(self, mout=None, vout=None):
+        """Both moments as fp32 values: lists (m, v).  With 32 bits these are the state itself; with 8
+        the codes are decoded into new tensors or into the lists ``mout`` and ``vout``."""
+        if self.opts.bits == 32:
+            if mout is not None or vout is not None:
+                raise ValueError("32-bit moments are not copied: mout and vout are for 8 bits")
+            return self.m, self.v
+        n = len(self._sizes)
+        if mout is None:
+            mout = [torch.empty(k, dtype=torch.float32, device=self.device) for k in self._sizes]
+        if vout is None:
+            vout = [torch.empty(k, dtype=torch.float32, device=self.device) for k in self._sizes]
+        if len(mout) != n or len(vout) != n:
+            raise ValueError("mout and vout have a tensor for each parameter")
+        dev = self.device
+        for x, k in zip([*mout, *vout], self._sizes * 2):
+            if x.dtype != torch.float32 or x.numel() != k or x.device != dev or not x.is_contiguous():
+                raise ValueError("mout and vout: contiguous fp32 tensors of the parameters' device and sizes")
+        with on_device(dev):
+            check(_lib.load().w2v_adamw_moments(self._table, (C.c_void_p * n)(*[x.data_ptr() for x in mout]),
+                                                (C.c_void_p * n)(*[x.data_ptr() for x in vout]), n,
+                                                stream_of(dev)), "w2v_adamw_moments")
+        return mout, vout

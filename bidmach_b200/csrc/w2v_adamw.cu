@@ -1,0 +1,437 @@
+// AdamW over many tensors in one launch, moments in 32 or in 8 bits.
+//
+//   m = b1 m + (1 - b1) g          v = b2 v + (1 - b2) g^2
+//   p = p (1 - lr wd) - (lr / c1) m / (sqrt(v) / sqrt(c2) + eps),   c = 1 - b^t
+//
+// Every element is read and written once and nothing else moves: 28 bytes an element with fp32
+// moments, 16 with 8-bit ones (fp32 parameters and gradients), so the bound is the memory.  The
+// work is cut into units of 256 elements, a warp each, 8 consecutive elements a lane (32 bytes of
+// fp32: one 256-bit access).  The tensors' addresses travel as kernel arguments, not through a
+// table in device memory: nothing has to be uploaded before a step, and a captured step holds
+// its own.
+//
+// Each operation is rounded on its own (no contraction to fused multiply-adds), so the result does
+// not depend on how a compiler groups them: next to the border of two 8-bit codes that would
+// change a stored moment by a whole step.
+//
+// 8-bit moments.  A unit is also the block that shares a scale, the largest magnitude in it.  A
+// code is the leading bits of the fp32 number y = x / scale (0 < |y| <= 1), rounded to nearest
+// even: for m a sign and 7 bits (3 of mantissa), for sqrt(v) 8 bits (4 of mantissa), the topmost
+// code meaning 1.  Both span about 16 octaves; what is below rounds to zero for m and to the
+// smallest code for sqrt(v), so that no step divides by eps alone.  The root of v is stored, not v:
+// it needs half the octaves.  The step itself uses the moments before they are rounded.
+#include <math.h>
+
+#include <algorithm>
+
+#include "../../include/bidmach_b200.h"
+#include "w2v_device.cuh"
+#include "w2v_internal.h"
+#include "w2v_types.cuh"
+
+namespace {
+
+using w2v::from_float;
+using w2v::kFullMask;
+using w2v::load8;
+using w2v::load_some;
+using w2v::store8;
+using w2v::store_some;
+using w2v::to_float;
+
+constexpr int kUnit = 256;
+constexpr int kThreads = 256;
+
+// Running products b1^t and b2^t and the blocks that have finished the step.
+struct Clock {
+  double b1t, b2t;
+  unsigned arrived, pad;
+};
+
+template <int CAP>
+struct Table {
+  void *p[CAP];
+  const void *g[CAP];
+  void *m[CAP];
+  void *v[CAP];
+  float *ms[CAP];
+  float *vs[CAP];
+  int64_t n[CAP];
+  int64_t first[CAP + 1];   // unit at which the tensor starts
+  unsigned char wide[CAP];  // all addresses allow the 8-element accesses
+  int count;
+};
+
+struct Rates {
+  double lrate, beta1, beta2, eps, wdecay;
+  const float *lrate_dev;
+  Clock *clock;
+  int advance;
+};
+
+// What a step computes once, each rounded to fp32 from its value in 64 bits.
+struct Consts {
+  float b1, ob1, b2, ob2, lrc1, rc2, eps, keep;
+};
+
+__device__ __forceinline__ Consts constants(const Rates &r) {
+  const double c1 = 1.0 - r.clock->b1t * r.beta1, c2 = 1.0 - r.clock->b2t * r.beta2;
+  const double lr = r.lrate_dev ? (double)*r.lrate_dev : r.lrate;
+  return Consts{(float)r.beta1, (float)(1.0 - r.beta1), (float)r.beta2, (float)(1.0 - r.beta2),
+                (float)(lr / c1), (float)(1.0 / sqrt(c2)), (float)r.eps, (float)(1.0 - lr * r.wdecay)};
+}
+
+__device__ __forceinline__ void step8(float (&p)[8], const float (&g)[8], float (&m)[8], float (&v)[8],
+                                      float (&root)[8], const Consts &c) {
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    m[i] = __fadd_rn(__fmul_rn(m[i], c.b1), __fmul_rn(g[i], c.ob1));
+    v[i] = __fadd_rn(__fmul_rn(v[i], c.b2), __fmul_rn(__fmul_rn(g[i], g[i]), c.ob2));
+    root[i] = __fsqrt_rn(v[i]);
+    const float d = __fadd_rn(__fmul_rn(root[i], c.rc2), c.eps);
+    p[i] = __fsub_rn(__fmul_rn(p[i], c.keep), __fdiv_rn(__fmul_rn(m[i], c.lrc1), d));
+  }
+}
+
+constexpr int kOne = 0x3F800000;
+constexpr float kSmallestScale = 1.17549435e-38f;   // 2^-126: its reciprocal is still finite
+
+// Scale of a unit, the largest of |x|; bits of non-negative floats order as unsigned numbers, NaN last.
+__device__ __forceinline__ float unit_scale(const float (&x)[8]) {
+  unsigned top = 0;
+#pragma unroll
+  for (int i = 0; i < 8; i++) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+  top = __reduce_max_sync(kFullMask, top);
+  if (top >= 0x7f800000u) return __uint_as_float(0x7fffffffu);   // infinity or NaN: the unit reads as NaN
+  const float s = __uint_as_float(top);
+  return s >= kSmallestScale ? s : 0.f;
+}
+
+template <bool SIGNED>
+__device__ __forceinline__ void encode8(const float (&x)[8], float scale, unsigned (&code)[2]) {
+  constexpr int shift = SIGNED ? 20 : 19, top = SIGNED ? 127 : 255, offset = (kOne >> shift) - top;
+  const float r = scale > 0.f ? __fdiv_rn(1.f, scale) : 0.f;   // false for a NaN scale
+  code[0] = code[1] = 0;
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    const float y = __fmul_rn(x[i], r);
+    const int bits = __float_as_int(y) & 0x7fffffff;
+    int c = ((bits + ((1 << (shift - 1)) - 1) + ((bits >> shift) & 1)) >> shift) - offset;
+    c = min(max(c, SIGNED ? 0 : 1), top);
+    if (bits == 0 || !(scale > 0.f)) c = 0;
+    if (SIGNED && y < 0.f && c > 0) c |= 128;
+    code[i >> 2] |= (unsigned)c << (8 * (i & 3));
+  }
+}
+
+template <bool SIGNED>
+__device__ __forceinline__ void decode8(const unsigned (&code)[2], float scale, float (&x)[8]) {
+  constexpr int shift = SIGNED ? 20 : 19, top = SIGNED ? 127 : 255, offset = (kOne >> shift) - top;
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    const int c = (code[i >> 2] >> (8 * (i & 3))) & 255;
+    const int low = SIGNED ? c & 127 : c;
+    float y = low > 0 ? __int_as_float((low + offset) << shift) : 0.f;
+    if (SIGNED && (c & 128)) y = -y;
+    x[i] = __fmul_rn(y, scale);
+  }
+}
+
+__device__ __forceinline__ void load_codes(const unsigned char *a, bool wide, int n, unsigned (&c)[2]) {
+  if (wide && n >= 8) {
+    const uint2 r = *reinterpret_cast<const uint2 *>(a);
+    c[0] = r.x;
+    c[1] = r.y;
+    return;
+  }
+  c[0] = c[1] = 0;
+#pragma unroll
+  for (int i = 0; i < 8; i++)
+    if (i < n) c[i >> 2] |= (unsigned)a[i] << (8 * (i & 3));
+}
+__device__ __forceinline__ void store_codes(unsigned char *a, bool wide, int n, const unsigned (&c)[2]) {
+  if (wide && n >= 8) {
+    *reinterpret_cast<uint2 *>(a) = make_uint2(c[0], c[1]);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; i++)
+    if (i < n) a[i] = (unsigned char)(c[i >> 2] >> (8 * (i & 3)));
+}
+
+template <typename T>
+__device__ __forceinline__ void fetch8(const T *a, bool wide, int n, float (&x)[8]) {
+  if (wide && n >= 8) load8(a, x);
+  else load_some(a, n, x);
+}
+template <typename T>
+__device__ __forceinline__ void put8(T *a, bool wide, int n, const float (&x)[8]) {
+  if (wide && n >= 8) store8(a, x);
+  else store_some(a, n, x);
+}
+
+// The tensor that unit `u` belongs to.
+template <int CAP>
+__device__ __forceinline__ int tensor_of(const Table<CAP> &t, int64_t u) {
+  int lo = 0, hi = t.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (t.first[mid] <= u) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+template <typename PT, typename GT, int BITS, int CAP>
+__global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__ Table<CAP> t,
+                                                         const __grid_constant__ Rates rates) {
+  __shared__ Consts shared_consts;
+  if (threadIdx.x == 0) shared_consts = constants(rates);
+  __syncthreads();
+  const Consts c = shared_consts;
+  const int lane = threadIdx.x & 31;
+  const int64_t units = t.first[t.count];
+  const int64_t stride = (int64_t)gridDim.x * (kThreads / 32);
+  for (int64_t u = (int64_t)blockIdx.x * (kThreads / 32) + threadIdx.x / 32; u < units; u += stride) {
+    const int k = tensor_of(t, u);
+    const int64_t block = u - t.first[k];
+    const int64_t at = block * kUnit + lane * 8;
+    const int n = (int)min((int64_t)8, max((int64_t)0, t.n[k] - at));
+    const bool wide = t.wide[k];
+    PT *pp = static_cast<PT *>(t.p[k]) + at;
+    const GT *gp = static_cast<const GT *>(t.g[k]) + at;
+    float p[8], g[8], m[8], v[8], root[8];
+    if (BITS == 32) {
+      float *mp = static_cast<float *>(t.m[k]) + at, *vp = static_cast<float *>(t.v[k]) + at;
+      fetch8(pp, wide, n, p);
+      fetch8(gp, wide, n, g);
+      fetch8(mp, wide, n, m);
+      fetch8(vp, wide, n, v);
+      step8(p, g, m, v, root, c);
+      put8(pp, wide, n, p);
+      put8(mp, wide, n, m);
+      put8(vp, wide, n, v);
+    } else {
+      unsigned char *mp = static_cast<unsigned char *>(t.m[k]) + at, *vp = static_cast<unsigned char *>(t.v[k]) + at;
+      unsigned mc[2], vc[2];
+      fetch8(pp, wide, n, p);
+      fetch8(gp, wide, n, g);
+      load_codes(mp, wide, n, mc);
+      load_codes(vp, wide, n, vc);
+      decode8<true>(mc, t.ms[k][block], m);
+      decode8<false>(vc, t.vs[k][block], v);
+#pragma unroll
+      for (int i = 0; i < 8; i++) v[i] = __fmul_rn(v[i], v[i]);
+      step8(p, g, m, v, root, c);
+      const float ms = unit_scale(m), vs = unit_scale(root);
+      encode8<true>(m, ms, mc);
+      encode8<false>(root, vs, vc);
+      put8(pp, wide, n, p);
+      store_codes(mp, wide, n, mc);
+      store_codes(vp, wide, n, vc);
+      if (lane == 0) {
+        t.ms[k][block] = ms;
+        t.vs[k][block] = vs;
+      }
+    }
+  }
+  // The block that finishes last moves the clock on: every block has read it by then.
+  if (rates.advance) {
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      __threadfence();
+      if (atomicAdd(&rates.clock->arrived, 1u) == gridDim.x - 1) {
+        rates.clock->b1t *= rates.beta1;
+        rates.clock->b2t *= rates.beta2;
+        rates.clock->arrived = 0;
+      }
+    }
+  }
+}
+
+// 8-bit moments as the values they stand for: p and g of the table are the two fp32 outputs.
+template <int CAP>
+__global__ void __launch_bounds__(kThreads) moments_kernel(const __grid_constant__ Table<CAP> t) {
+  const int lane = threadIdx.x & 31;
+  const int64_t units = t.first[t.count];
+  const int64_t stride = (int64_t)gridDim.x * (kThreads / 32);
+  for (int64_t u = (int64_t)blockIdx.x * (kThreads / 32) + threadIdx.x / 32; u < units; u += stride) {
+    const int k = tensor_of(t, u);
+    const int64_t block = u - t.first[k];
+    const int64_t at = block * kUnit + lane * 8;
+    const int n = (int)min((int64_t)8, max((int64_t)0, t.n[k] - at));
+    const bool wide = t.wide[k];
+    unsigned mc[2], vc[2];
+    float m[8], v[8];
+    load_codes(static_cast<const unsigned char *>(t.m[k]) + at, wide, n, mc);
+    load_codes(static_cast<const unsigned char *>(t.v[k]) + at, wide, n, vc);
+    decode8<true>(mc, t.ms[k][block], m);
+    decode8<false>(vc, t.vs[k][block], v);
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = __fmul_rn(v[i], v[i]);
+    put8(static_cast<float *>(t.p[k]) + at, wide, n, m);
+    put8(static_cast<float *>(const_cast<void *>(t.g[k])) + at, wide, n, v);
+  }
+}
+
+__global__ void clock_kernel(Clock *c, double b1t, double b2t) { *c = Clock{b1t, b2t, 0, 0}; }
+
+bool aligned(const void *a, size_t to) { return reinterpret_cast<uintptr_t>(a) % to == 0; }
+size_t type_size(int type) { return type == W2V_F32 ? 4 : 2; }
+
+int grid_for(int64_t units) {
+  // four blocks of eight warps an SM keep 32 KB in flight there with fp32 moments
+  const int64_t need = (units + kThreads / 32 - 1) / (kThreads / 32);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(need, (int64_t)w2v::device_sm_count() * 8));
+}
+
+template <typename PT, typename GT, int CAP>
+int launch_typed(const Table<CAP> &t, const Rates &r, int bits, cudaStream_t s) {
+  const int grid = grid_for(t.first[t.count]);
+  if (bits == 32) adamw_kernel<PT, GT, 32, CAP><<<grid, kThreads, 0, s>>>(t, r);
+  else adamw_kernel<PT, GT, 8, CAP><<<grid, kThreads, 0, s>>>(t, r);
+  w2v::count_launch(1);
+  return (int)cudaGetLastError();
+}
+
+template <int CAP>
+int launch(const Table<CAP> &t, const Rates &r, int ptype, int gtype, int bits, cudaStream_t s) {
+  if (ptype == W2V_F32) return launch_typed<float, float>(t, r, bits, s);
+  if (ptype == W2V_BF16)
+    return gtype == W2V_F32 ? launch_typed<__nv_bfloat16, float>(t, r, bits, s)
+                            : launch_typed<__nv_bfloat16, __nv_bfloat16>(t, r, bits, s);
+  return gtype == W2V_F32 ? launch_typed<__half, float>(t, r, bits, s)
+                          : launch_typed<__half, __half>(t, r, bits, s);
+}
+
+template <int CAP>
+void add(Table<CAP> &t, const w2v_adamw_tensor &x, const void *g, size_t psize, size_t gsize, int bits) {
+  const int k = t.count++;
+  if (k == 0) t.first[0] = 0;
+  t.p[k] = x.p;
+  t.g[k] = g;
+  t.m[k] = x.m;
+  t.v[k] = x.v;
+  t.ms[k] = x.mscale;
+  t.vs[k] = x.vscale;
+  t.n[k] = x.n;
+  t.first[k + 1] = t.first[k] + (x.n + kUnit - 1) / kUnit;
+  const size_t state = bits == 32 ? 32 : 8;
+  t.wide[k] = aligned(x.p, 8 * psize) && aligned(g, 8 * gsize) && aligned(x.m, state) && aligned(x.v, state);
+}
+
+constexpr int kFew = 16, kMany = 256;
+
+// Calls `go` with tables of at most `kMany` of the `n` chosen tensors (small tables for few: the
+// arguments of a launch are copied to the device with it).
+template <typename ADD, typename GO>
+int in_tables(int n, ADD put, GO go) {
+  if (n <= kFew) {
+    Table<kFew> t;
+    t.count = 0;
+    t.first[0] = 0;
+    for (int i = 0; i < n; i++) put(t, i);
+    return go(t, true);
+  }
+  for (int a = 0; a < n; a += kMany) {
+    Table<kMany> t;
+    t.count = 0;
+    t.first[0] = 0;
+    const int b = std::min(n, a + kMany);
+    for (int i = a; i < b; i++) put(t, i);
+    const int err = go(t, b == n);
+    if (err) return err;
+  }
+  return 0;
+}
+
+bool good_state(const w2v_adamw_tensor &x, int bits) {
+  if (x.n < 0 || x.n > ((int64_t)1 << 42)) return false;
+  if (x.n == 0) return true;
+  if (!x.m || !x.v) return false;
+  return bits == 32 || (x.mscale && x.vscale);
+}
+
+}  // namespace
+
+extern "C" int w2v_adamw_clock(void *clock, double beta1, double beta2, int64_t t, void *stream) {
+  if (!clock || !aligned(clock, 8) || t < 0 || !(beta1 >= 0 && beta1 < 1) || !(beta2 >= 0 && beta2 < 1)) return 1;
+  clock_kernel<<<1, 1, 0, static_cast<cudaStream_t>(stream)>>>(static_cast<Clock *>(clock), pow(beta1, (double)t),
+                                                               pow(beta2, (double)t));
+  w2v::count_launch(1);
+  return (int)cudaGetLastError();
+}
+
+extern "C" int w2v_adamw_step(const w2v_adamw_tensor *tensors, const void *const *grads, const int *gtypes,
+                              int ntensors, int bits, const w2v_adamw_opts *o, const float *lrate_dev, void *clock,
+                              void *stream) {
+  if (ntensors < 0 || (ntensors > 0 && (!tensors || !grads || !gtypes)) || !o || !clock || !aligned(clock, 8) ||
+      (bits != 32 && bits != 8))
+    return 1;
+  if (!(o->beta1 >= 0 && o->beta1 < 1) || !(o->beta2 >= 0 && o->beta2 < 1) || !(o->eps > 0)) return 1;
+  // the tensors of each pair of types go together; the last launch of all moves the clock on
+  constexpr int kPairs = 5;
+  const int pairs[kPairs][2] = {{W2V_F32, W2V_F32}, {W2V_BF16, W2V_F32}, {W2V_BF16, W2V_BF16},
+                                {W2V_F16, W2V_F32}, {W2V_F16, W2V_F16}};
+  int counts[kPairs] = {0, 0, 0, 0, 0};
+  auto pair_of = [&](int i) {
+    for (int q = 0; q < kPairs; q++)
+      if (tensors[i].ptype == pairs[q][0] && gtypes[i] == pairs[q][1]) return q;
+    return -1;
+  };
+  for (int i = 0; i < ntensors; i++) {
+    const int q = pair_of(i);
+    if (q < 0 || !good_state(tensors[i], bits)) return 1;
+    if (tensors[i].n > 0 && (!tensors[i].p || !grads[i])) return 1;
+    if (tensors[i].n > 0) counts[q]++;
+  }
+  int last = 0;
+  for (int q = 0; q < kPairs; q++)
+    if (counts[q]) last = q;
+  const auto s = static_cast<cudaStream_t>(stream);
+  Rates r{o->lrate, o->beta1, o->beta2, o->eps, o->wdecay, lrate_dev, static_cast<Clock *>(clock), 0};
+  for (int q = 0; q <= last; q++) {
+    if (!counts[q] && q != last) continue;
+    int next = 0;   // walks the tensors of this pair in order
+    const int err = in_tables(
+        counts[q],
+        [&](auto &t, int) {
+          while (tensors[next].n == 0 || pair_of(next) != q) next++;
+          add(t, tensors[next], grads[next], type_size(pairs[q][0]), type_size(pairs[q][1]), bits);
+          next++;
+        },
+        [&](const auto &t, bool end) {
+          r.advance = end && q == last;
+          return launch(t, r, pairs[q][0], pairs[q][1], bits, s);
+        });
+    if (err) return err;
+  }
+  return 0;
+}
+
+extern "C" int w2v_adamw_moments(const w2v_adamw_tensor *tensors, float *const *mout, float *const *vout, int ntensors,
+                                 void *stream) {
+  if (ntensors < 0 || (ntensors > 0 && (!tensors || !mout || !vout))) return 1;
+  int count = 0;
+  for (int i = 0; i < ntensors; i++) {
+    if (!good_state(tensors[i], 8) || (tensors[i].n > 0 && (!mout[i] || !vout[i]))) return 1;
+    count += tensors[i].n > 0;
+  }
+  if (!count) return 0;
+  const auto s = static_cast<cudaStream_t>(stream);
+  int next = 0;
+  return in_tables(
+      count,
+      [&](auto &t, int) {
+        while (tensors[next].n == 0) next++;
+        w2v_adamw_tensor x = tensors[next];
+        x.p = mout[next];
+        add(t, x, vout[next], 4, 4, 8);
+        next++;
+      },
+      [&](const auto &t, bool) {
+        moments_kernel<<<grid_for(t.first[t.count]), kThreads, 0, s>>>(t);
+        w2v::count_launch(1);
+        return (int)cudaGetLastError();
+      });
+}

@@ -1,0 +1,85 @@
+"""Rows of a matrix picked by word ids, and the gradient of that."""
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+from .adamw import TYPES, check, on_device, stream_of
+
+
+def check_matrix(x, name: str, device=None, dtype=None):
+    """A CUDA matrix whose rows are contiguous; returns its leading dimension."""
+    if not isinstance(x, torch.Tensor) or x.dim() != 2 or x.dtype not in TYPES:
+        raise ValueError(f"{name} is a matrix of fp32, bf16 or fp16")
+    if dtype is not None and x.dtype != dtype:
+        raise ValueError(f"{name} has type {x.dtype}, expected {dtype}")
+    if not x.is_cuda:
+        raise ValueError(f"{name} is not on a CUDA device")
+    if device is not None and x.device != device:
+        raise ValueError(f"{name} is on {x.device}, expected {device}")
+    if x.shape[1] < 1:
+        raise ValueError(f"{name} has no columns")
+    ld = x.stride(0) if x.shape[0] > 1 else x.shape[1]
+    if (x.stride(1) != 1 and x.shape[1] > 1) or ld < x.shape[1]:
+        raise ValueError(f"{name}: rows have to be contiguous and must not overlap")
+    return ld
+
+
+def check_ids(x, name: str, dim: int):
+    if not isinstance(x, torch.Tensor) or x.dim() != dim or x.dtype != torch.int32:
+        raise ValueError(f"{name} is int32 with {dim} dimension" + ("s" if dim > 1 else ""))
+    if not x.is_cuda:
+        raise ValueError(f"{name} is not on a CUDA device")
+    if not x.is_contiguous():
+        raise ValueError(f"{name} is not contiguous")
+
+
+class EmbedRows:
+    """Static methods only.  ``ids``: int32, one for each row; an id outside the matrix (-1 marks a
+    dropped word) gives a row of zeros and takes no part in the gradient."""
+
+    @staticmethod
+    def forward(ids, matrix, out=None):
+        """``out[i] = matrix[ids[i]]``."""
+        check_ids(ids, "ids", 1)
+        ldm = check_matrix(matrix, "matrix", ids.device)
+        n, (vocab, dim) = ids.numel(), matrix.shape
+        if vocab < 1:
+            raise ValueError("matrix has no rows")
+        if out is None:
+            out = torch.empty(n, dim, dtype=matrix.dtype, device=ids.device)
+        ldo = check_matrix(out, "out", ids.device, matrix.dtype)
+        if tuple(out.shape) != (n, dim):
+            raise ValueError(f"out has shape {tuple(out.shape)}, expected {(n, dim)}")
+        with on_device(ids.device):
+            check(_lib.load().w2v_embed_rows(ids.data_ptr(), n, matrix.data_ptr(), ldm, vocab, dim,
+                                             TYPES[matrix.dtype], out.data_ptr(), ldo, stream_of(ids.device)),
+                  "w2v_embed_rows")
+        return out
+
+    @staticmethod
+    def backward(ids, grad, nrows: int, out=None):
+        """Gradient of the matrix, ``[nrows, dim]``: row ``v`` is the sum of the rows of ``grad`` whose
+        id is ``v``, added in fp32 and in an order that the ids fix (equal calls give equal bits), zero
+        where there is none."""
+        check_ids(ids, "ids", 1)
+        ldg = check_matrix(grad, "grad", ids.device)
+        n, dim, nrows = ids.numel(), grad.shape[1], int(nrows)
+        if grad.shape[0] != n:
+            raise ValueError(f"grad has {grad.shape[0]} rows for {n} ids")
+        if not 1 <= nrows < 2 ** 31 - 1 or n >= 2 ** 30 or dim > 65536:
+            raise ValueError("need 1 <= nrows < 2^31 - 1, fewer than 2^30 ids, at most 65536 columns")
+        if out is None:
+            out = torch.empty(nrows, dim, dtype=grad.dtype, device=ids.device)
+        ldo = check_matrix(out, "out", ids.device, grad.dtype)
+        if tuple(out.shape) != (nrows, dim):
+            raise ValueError(f"out has shape {tuple(out.shape)}, expected {(nrows, dim)}")
+        lib, t = _lib.load(), TYPES[grad.dtype]
+        with on_device(ids.device):
+            size = lib.w2v_embed_grad_workspace(n, nrows, dim, t)
+            if size < 0:
+                raise RuntimeError("w2v_embed_grad_workspace refused the sizes")
+            work = torch.empty(size, dtype=torch.uint8, device=ids.device)
+            check(lib.w2v_embed_grad(ids.data_ptr(), n, grad.data_ptr(), ldg, nrows, dim, t, out.data_ptr(), ldo,
+                                     work.data_ptr(), size, stream_of(ids.device)), "w2v_embed_grad")
+        return out

@@ -416,6 +416,70 @@ int64_t bidmach_lz4_compress_bound(int64_t n);
 int64_t bidmach_lz4_compress(const void *src, int64_t n, void *dst, int64_t cap);
 int64_t bidmach_lz4_decompress(const void *src, int64_t n, void *dst, int64_t cap);
 
+/* -------------------------------------------------------------------------
+ * Part 5 -- training operators over whole matrices (no counterpart among the
+ * reference's native functions): rows by ids with their gradient, and AdamW.
+ *
+ * Common to all of them: device pointers; work is enqueued on `stream` and
+ * nothing waits for it; the calls can be captured into a CUDA graph; scratch
+ * memory is the caller's (a *_workspace function gives its size in bytes, the
+ * address must be a multiple of 256) and may be reused once the call's work
+ * has finished, so calls that can run at the same time need workspaces of
+ * their own.  Matrices are rows of contiguous elements, `ld` elements apart
+ * (ld >= dim); any alignment works, multiples of 32 bytes are fastest.
+ * Return value: 0, 1 for arguments that are refused, or a cudaError_t.
+ * ---------------------------------------------------------------------- */
+enum { W2V_F32 = 0, W2V_BF16 = 1, W2V_F16 = 2 };   /* element types */
+
+/* out[i] = matrix[ids[i]] for i < n; an id outside [0, vocab) (a dropped word) gives a row of
+ * zeros.  matrix is vocab x dim, out n x dim, both of `type`. */
+int w2v_embed_rows(const int *ids, int64_t n, const void *matrix, int64_t ldm, int64_t vocab, int dim,
+                   int type, void *out, int64_t ldo, void *stream);
+/* Gradient of w2v_embed_rows: out[v] = sum of grad[i] over the i with ids[i] == v, zero where
+ * there is none; summed in fp32 in an order that the ids alone fix, so equal calls give equal
+ * bits.  grad is n x dim, out vocab x dim, both of `type`.  n < 2^30. */
+int64_t w2v_embed_grad_workspace(int64_t n, int64_t vocab, int dim, int type);   /* -1: refused */
+int w2v_embed_grad(const int *ids, int64_t n, const void *grad, int64_t ldg, int64_t vocab, int dim,
+                   int type, void *out, int64_t ldo, void *workspace, int64_t workspace_bytes,
+                   void *stream);
+
+/* One tensor of an AdamW step: `n` contiguous elements of `ptype`.  With 32-bit moments m and v are
+ * fp32[n] and the scales null.  With 8-bit ones m and v are uint8[n] and every 256 elements share a
+ * scale, fp32[(n + 255) / 256] each:
+ *   m      = +-f(code & 127, 3 bits) * mscale   (code 128 and above: negative)
+ *   v      = (f(code, 4 bits) * vscale)^2
+ *   f(0) = 0, else f is the fp32 number whose bits are (code + 0x3F8 - 127) << 20 for m and
+ *   (code + 0x7F0 - 255) << 19 for v; the scale is the largest magnitude of the 256 (of |m|, of
+ *   sqrt(v)), zero below 2^-126, NaN where one of them is not finite.
+ * Zeros are a valid initial state in both forms. */
+typedef struct w2v_adamw_tensor {
+  void *p;
+  void *m;
+  void *v;
+  float *mscale;
+  float *vscale;
+  int64_t n;
+  int ptype;
+} w2v_adamw_tensor;
+typedef struct w2v_adamw_opts {
+  double lrate, beta1, beta2, eps, wdecay;
+} w2v_adamw_opts;
+
+/* Sets the step counter of an updater, 32 bytes of device memory (8-byte aligned): t steps done. */
+int w2v_adamw_clock(void *clock, double beta1, double beta2, int64_t t, void *stream);
+/* One step for all `ntensors` tensors and the counter:
+ *   m = b1 m + (1-b1) g;  v = b2 v + (1-b2) g^2;
+ *   p = p (1 - lrate wdecay) - (lrate / (1-b1^t)) m / (sqrt(v) / sqrt(1-b2^t) + eps)
+ * grads[i] holds n elements of gtypes[i]: fp32, or the type of the tensor.  `tensors`, `grads` and
+ * `gtypes` are host arrays that may be freed on return.  lrate_dev, when not null, is a device float
+ * that replaces opts->lrate (so a replayed graph can follow a schedule).  Tensors must not overlap. */
+int w2v_adamw_step(const w2v_adamw_tensor *tensors, const void *const *grads, const int *gtypes,
+                   int ntensors, int bits, const w2v_adamw_opts *opts, const float *lrate_dev,
+                   void *clock, void *stream);
+/* 8-bit moments as the fp32 values they stand for: mout[i], vout[i] are fp32[n]. */
+int w2v_adamw_moments(const w2v_adamw_tensor *tensors, float *const *mout, float *const *vout,
+                      int ntensors, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,227 @@
+"""AdamW against a restatement in numpy: bit for bit in fp32 (every operation is rounded on its own), and
+against 64 bits with a tolerance counted in roundings."""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+F = np.float32
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+LR, B1, B2, EPS, WD = 3e-3, 0.9, 0.999, 1e-8, 0.02
+
+
+def encode(x, signed):
+    """Codes and scales of a vector, blocks of 256."""
+    shift, top = (20, 127) if signed else (19, 255)
+    n = len(x)
+    x = np.concatenate([x, np.zeros(-n % 256, F)]).reshape(-1, 256)
+    scale = np.abs(x).max(1)
+    fine = scale >= F(2.0 ** -126)
+    with np.errstate(divide="ignore"):
+        r = np.where(fine, F(1) / scale, F(0)).astype(F)
+    y = (x * r[:, None]).astype(F)
+    bits = np.abs(y).view(np.int32)
+    code = ((bits + ((1 << (shift - 1)) - 1) + ((bits >> shift) & 1)) >> shift) - ((0x3F800000 >> shift) - top)
+    code = np.where(bits == 0, 0, np.clip(code, 0 if signed else 1, top))
+    code = np.where(fine[:, None], code, 0)
+    if signed:
+        code = code + 128 * ((y < 0) & (code > 0))
+    return code.reshape(-1)[:n].astype(np.uint8), np.where(fine, scale, F(0)).astype(F)
+
+
+def decode(codes, scale, signed):
+    shift, top = (20, 127) if signed else (19, 255)
+    low = codes.astype(np.int32)
+    sign = low >= 128 if signed else np.zeros(len(low), bool)
+    low = low & 127 if signed else low
+    y = np.where(low > 0, ((low + ((0x3F800000 >> shift) - top)) << shift).astype(np.int32).view(F), F(0))
+    y = np.where(sign, -y, y)
+    return (y * np.repeat(scale, 256)[:len(codes)]).astype(F)
+
+
+def step_f32(p, g, m, v, t, lr=LR):
+    """One step in fp32, one rounding an operation: (p, m, v, root of v)."""
+    c1, c2 = 1.0 - B1 ** t, 1.0 - B2 ** t
+    m = m * F(B1) + g * F(1.0 - B1)
+    v = v * F(B2) + (g * g) * F(1.0 - B2)
+    root = np.sqrt(v)
+    return p * F(1.0 - lr * WD) - (m * F(lr / c1)) / (root * F(1.0 / np.sqrt(c2)) + F(EPS)), m, v, root
+
+
+def make(sizes, ptype, gtype, seed):
+    gen = torch.Generator().manual_seed(seed)
+    ps = [(torch.randn(n, generator=gen) * 0.4).to(TYPES[ptype]) for n in sizes]
+    gs = [(torch.randn(n, generator=gen) * torch.exp(-8 * torch.rand(n, generator=gen))).to(TYPES[gtype])
+          for n in sizes]
+    return ps, gs
+
+
+def f32(x):
+    return x.detach().float().cpu().numpy().reshape(-1)
+
+
+SIZES = [[1], [255, 256, 257], [0, 5, 1000], [70001], [7 + 13 * i for i in range(40)], [3] * 300]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("ptype,gtype", [("f32", "f32"), ("bf16", "bf16"), ("bf16", "f32"), ("f16", "f16"),
+                                         ("f16", "f32")])
+@pytest.mark.parametrize("sizes", SIZES, ids=lambda s: f"{len(s)}x{s[0]}")
+def test_steps_match_the_restatement(bits, ptype, gtype, sizes):
+    from bidmach_b200 import AdamW
+    ps, _ = make(sizes, ptype, gtype, 1)
+    dev = [p.cuda() for p in ps]
+    opt = AdamW(dev, AdamW.Opts(lrate=LR, beta1=B1, beta2=B2, eps=EPS, wdecay=WD, bits=bits))
+    p = [f32(x) for x in ps]
+    m, v = [np.zeros(n, F) for n in sizes], [np.zeros(n, F) for n in sizes]
+    for t in (1, 2, 3):
+        gs = make(sizes, ptype, gtype, 10 + t)[1]
+        opt.step([g.cuda() for g in gs])
+        for i, g in enumerate(gs):
+            new, m[i], v[i], root = step_f32(p[i], f32(g), m[i], v[i], t)
+            p[i] = f32(torch.from_numpy(new).to(TYPES[ptype]))
+            if bits == 8:
+                mc, ms = encode(m[i], True)
+                vc, vs = encode(root, False)
+                np.testing.assert_array_equal(opt.m[i].cpu().numpy(), mc)
+                np.testing.assert_array_equal(opt.v[i].cpu().numpy(), vc)
+                np.testing.assert_array_equal(opt.mscale[i].cpu().numpy(), ms[:(sizes[i] + 255) // 256])
+                m[i], v[i] = decode(mc, ms, True), decode(vc, vs, False) ** 2
+            np.testing.assert_array_equal(f32(dev[i]), p[i])
+        got = opt.moments()
+        for i in range(len(sizes)):
+            np.testing.assert_array_equal(f32(got[0][i]), m[i])
+            np.testing.assert_array_equal(f32(got[1][i]), v[i])
+
+
+@pytest.mark.parametrize("ptype", list(TYPES))
+def test_step_against_64_bits(ptype):
+    """m is two products and a sum of rounded constants: 4 roundings of its terms.  The step has 10
+    (m 4, root 4 / 2 + 1, product, sum, product, quotient, ...); p is off by 2 roundings of its own
+    terms, 12 of the step's and the rounding to its type."""
+    from bidmach_b200 import AdamW
+    u = 2.0 ** -24
+    (p,), (g,) = make([10007], ptype, "f32", 5)
+    rng = np.random.default_rng(2)
+    m0 = rng.standard_normal(10007).astype(F)
+    v0 = np.square(rng.standard_normal(10007)).astype(F)
+    dp, dm, dv = p.cuda(), torch.from_numpy(m0).cuda(), torch.from_numpy(v0).cuda()
+    opt = AdamW([dp], AdamW.Opts(lrate=LR, beta1=B1, beta2=B2, eps=EPS, wdecay=WD),
+                state={"t": 6, "m": [dm], "v": [dv]})
+    opt.step([g.cuda()])
+    g, p = g.double().numpy(), p.double().numpy()
+    m = B1 * m0.astype(np.float64) + (1 - B1) * g
+    v = B2 * v0.astype(np.float64) + (1 - B2) * g ** 2
+    step = LR / (1 - B1 ** 7) * m / (np.sqrt(v / (1 - B2 ** 7)) + EPS)
+    terms = np.abs(B1 * m0) + np.abs((1 - B1) * g)
+    want = p * (1 - LR * WD) - step
+    assert np.all(np.abs(dm.cpu().numpy() - m) <= 4 * u * terms)
+    assert np.all(np.abs(dv.cpu().numpy() - v) <= 5 * u * v)
+    size = LR / (1 - B1 ** 7) * terms / np.sqrt(v / (1 - B2 ** 7))
+    half = torch.finfo(TYPES[ptype]).eps / 2
+    assert np.all(np.abs(dp.double().cpu().numpy() - want) <= 3 * u * np.abs(p) + 12 * u * size +
+                  (half + u) * (np.abs(want) + size) + (2.0 ** -25 if ptype == "f16" else 0))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_any_alignment(bits):
+    """Views at odd offsets of one buffer: the same bits as separate tensors."""
+    from bidmach_b200 import AdamW
+    o = AdamW.Opts(bits=bits)
+    for off, n in [(1, 777), (3, 256), (2, 513)]:
+        (p,), (g,) = make([n], "f32", "f32", off)
+        flat, gflat = torch.zeros(2000, device="cuda"), torch.zeros(2000, device="cuda")
+        flat[off:off + n] = p.cuda()
+        gflat[off:off + n] = g.cuda()
+        flat[off + n] = 7.0
+        q = p.cuda()
+        a, b = AdamW([flat[off:off + n]], o), AdamW([q], o)
+        for _ in range(2):
+            a.step([gflat[off:off + n]])
+            b.step([g.cuda()])
+        assert torch.equal(flat[off:off + n], q)
+        assert torch.equal(a.m[0], b.m[0]) and torch.equal(a.v[0], b.v[0])
+        assert flat[off + n] == 7.0 and flat[:off].abs().sum() == 0
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_not_finite_gradients(bits):
+    """A NaN or an infinity spoils its element (with 8 bits the moments of its 256), nothing else."""
+    from bidmach_b200 import AdamW
+    p = torch.ones(1024, device="cuda")
+    opt = AdamW([p], AdamW.Opts(bits=bits))
+    g = torch.full((1024,), 0.5, device="cuda")
+    g[300], g[900] = float("nan"), float("inf")
+    opt.step([g])
+    bad = torch.zeros(1024, dtype=torch.bool, device="cuda")
+    bad[300] = bad[900] = True
+    assert torch.isnan(p[bad]).all() and torch.isfinite(p[~bad]).all()
+    m, v = opt.moments()
+    if bits == 8:
+        bad[256:512] = True
+        bad[768:] = True
+        assert torch.isnan(m[0][bad]).all()
+    assert torch.isfinite(m[0][~bad]).all() and torch.isfinite(v[0][~bad]).all()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_tiny_and_zero_gradients(bits):
+    """No step is larger than lrate / (1 - beta1) whatever the gradients' size; zeros move nothing."""
+    from bidmach_b200 import AdamW
+    for size in (0.0, 1e-30, 1e-38, 1e-42, 1e30 ** 0.5):
+        p = torch.zeros(600, device="cuda")
+        g = torch.linspace(-1, 1, 600, device="cuda") * size
+        opt = AdamW([p], AdamW.Opts(lrate=0.1, bits=bits))
+        for _ in range(4):
+            opt.step([g])
+        assert torch.isfinite(p).all() and float(p.abs().max()) <= 4 * 1.0
+        if size == 0.0:
+            assert float(p.abs().max()) == 0
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_captured_steps_count(bits):
+    """A captured step, replayed, does what as many calls do, with a rate read from the device."""
+    from bidmach_b200 import AdamW
+    (p,), (g,) = make([5000], "f32", "f32", 3)
+    a, b, g = p.cuda(), p.cuda(), g.cuda()
+    rate = torch.tensor([0.01], device="cuda")
+    oa, ob = AdamW([a], AdamW.Opts(bits=bits)), AdamW([b], AdamW.Opts(bits=bits))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        ob.step([g], rate)
+    torch.cuda.current_stream().wait_stream(side)
+    with torch.cuda.graph(graph):
+        ob.step([g], rate)
+    oa.step([g], 0.01)
+    for r in (0.01, 0.02, 0.005):
+        rate.fill_(r)
+        graph.replay()
+        oa.step([g], float(torch.tensor(r)))
+    torch.cuda.synchronize()
+    assert torch.equal(a, b) and torch.equal(oa.m[0], ob.m[0]) and torch.equal(oa.v[0], ob.v[0])
+
+
+def test_refusals_on_the_device():
+    from bidmach_b200 import AdamW
+    p = torch.zeros(512, device="cuda")
+    with pytest.raises(ValueError, match="overlap"):
+        AdamW([p[:300], p[200:]])
+    with pytest.raises(ValueError, match="contiguous"):
+        AdamW([p.view(2, 256).t()])
+    opt = AdamW([p])
+    for g in (torch.zeros(511, device="cuda"), torch.zeros(512), torch.zeros(512, device="cuda", dtype=torch.float16),
+              torch.zeros(1024, device="cuda")[::2]):
+        with pytest.raises(ValueError):
+            opt.step([g])
+    with pytest.raises(ValueError):
+        opt.step([])
+    with pytest.raises(ValueError):
+        opt.step([p], torch.zeros(1))
+    with pytest.raises(ValueError, match="state"):
+        AdamW([p], state={"t": 0, "m": [torch.zeros(511, device="cuda")], "v": [p.clone()]})
+    with pytest.raises(ValueError):
+        opt.moments(mout=[p.clone()])

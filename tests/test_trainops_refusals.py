@@ -1,0 +1,46 @@
+"""What the training operators refuse before they touch a GPU."""
+import ctypes as C
+
+import pytest
+import torch
+
+from bidmach_b200 import AdamW, EmbedRows, _lib
+
+
+def test_adamw_options_and_tensors():
+    p = torch.zeros(8)
+    for o in (dict(bits=16), dict(beta1=1.0), dict(beta2=-0.1), dict(eps=0.0), dict(wdecay=-1.0)):
+        with pytest.raises(ValueError):
+            AdamW([p], AdamW.Opts(**o))
+    for params in ([], [p], [torch.zeros(3, dtype=torch.int32)], [torch.zeros(3, dtype=torch.float64)]):
+        with pytest.raises(ValueError):
+            AdamW(params)
+
+
+def test_embed_wants_device_tensors():
+    with pytest.raises(ValueError, match="CUDA"):
+        EmbedRows.forward(torch.zeros(3, dtype=torch.int32), torch.zeros(4, 4))
+    with pytest.raises(ValueError, match="int32"):
+        EmbedRows.backward(torch.zeros(3, dtype=torch.int64), torch.zeros(3, 4), 5)
+
+
+def test_c_entries_refuse_without_a_launch():
+    lib = _lib.load()
+    before = lib.w2v_launch_count()
+    t = (_lib.W2VAdamwTensor * 1)(_lib.W2VAdamwTensor(64, 64, 64, 0, 0, 4, 0))
+    g, k = (C.c_void_p * 1)(64), (C.c_int * 1)(0)
+    o = _lib.W2VAdamwOpts(1e-3, 0.9, 0.999, 1e-8, 0.0)
+    bad = [dict(bits=16), dict(clock=0), dict(clock=4), dict(k=(C.c_int * 1)(2)), dict(bits=8), dict(n=-1),
+           dict(g=(C.c_void_p * 1)(0)), dict(o=_lib.W2VAdamwOpts(1e-3, 1.0, 0.999, 1e-8, 0.0))]
+    for b in bad:
+        assert lib.w2v_adamw_step(t, b.get("g", g), b.get("k", k), b.get("n", 1), b.get("bits", 32),
+                                  C.byref(b.get("o", o)), None, b.get("clock", 64), None) == 1
+    assert lib.w2v_adamw_clock(0, 0.9, 0.999, 0, None) == 1
+    assert lib.w2v_adamw_clock(64, 0.9, 0.999, -1, None) == 1
+    assert lib.w2v_adamw_moments(t, None, None, 1, None) == 1
+    for n, vocab, dim, kind in [(-1, 5, 4, 0), (1 << 30, 5, 4, 0), (3, 0, 4, 0), (3, 5, 0, 0), (3, 5, 4, 3)]:
+        assert lib.w2v_embed_grad_workspace(n, vocab, dim, kind) == -1
+        assert lib.w2v_embed_rows(64, n, 64, dim, vocab, dim, kind, 64, dim, None) == 1
+    assert lib.w2v_embed_rows(64, 3, 64, 3, 5, 4, 0, 64, 4, None) == 1       # rows overlap
+    assert lib.w2v_embed_grad(64, 3, 64, 4, 5, 4, 0, 64, 4, 0, 0, None) == 1   # no workspace
+    assert lib.w2v_launch_count() == before
