@@ -1,0 +1,94 @@
+"""Softmax cross entropy over a whole vocabulary, with its gradients, without keeping the logits."""
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+from .adamw import TYPES, check, on_device, stream_of
+from .embed import check_ids, check_matrix
+
+
+def _vector(x, name: str, n: int, device):
+    if not isinstance(x, torch.Tensor) or x.dtype != torch.float32 or tuple(x.shape) != (n,) or x.device != device \
+            or not x.is_contiguous():
+        raise ValueError(f"{name}: contiguous fp32 [{n}] on {device}")
+
+
+class Softmax:
+    """Static methods only.  With the logits ``l = hidden @ weight.T``:
+
+        lse[i]  = log sum_v exp l[i, v]
+        loss[i] = sum over the targets y of row i of (lse[i] - l[i, y])
+
+    ``hidden`` is ``[n, dim]``, ``weight`` ``[vocab, dim]``, both fp32, bf16 or fp16, ``dim`` up to 4096;
+    ``targets`` int32 ``[n]`` or ``[n, labels]``.  A target outside ``[0, vocab)`` (-1 by convention) stands
+    for none; a row may have none (its loss and gradient are zero) or the same word more than once.
+    fp32 operands are multiplied to 22 bits and accumulated in fp32; 16-bit ones are multiplied exactly.
+    Every row takes part in the products, so ``hidden`` has to be finite in rows without targets too."""
+
+    @staticmethod
+    def _operands(hidden, weight, targets):
+        ldh = check_matrix(hidden, "hidden")
+        ldw = check_matrix(weight, "weight", hidden.device, hidden.dtype)
+        if not isinstance(targets, torch.Tensor) or targets.dim() not in (1, 2):
+            raise ValueError("targets is int32 [n] or [n, labels]")
+        check_ids(targets, "targets", targets.dim())
+        n, dim = hidden.shape
+        labels = 1 if targets.dim() == 1 else targets.shape[1]
+        if targets.shape[0] != n or targets.device != hidden.device:
+            raise ValueError(f"targets has {targets.shape[0]} rows on {targets.device}, hidden {n} on {hidden.device}")
+        if weight.shape[1] != dim:
+            raise ValueError(f"weight has {weight.shape[1]} columns, hidden {dim}")
+        if dim > 4096 or not 1 <= labels <= 1024 or weight.shape[0] < 1:
+            raise ValueError("need dim <= 4096, 1 <= labels <= 1024 and at least one word")
+        return ldh, ldw, n, weight.shape[0], dim, labels
+
+    @staticmethod
+    def _workspace(n, vocab, dim, labels, kind, grad, device):
+        size = _lib.load().w2v_softmax_workspace(n, vocab, dim, labels, kind, int(grad))
+        if size < 0:
+            raise ValueError("w2v_softmax_workspace refused the sizes")
+        return torch.empty(size, dtype=torch.uint8, device=device), size
+
+    @staticmethod
+    def loss(hidden, weight, targets, loss=None, lse=None):
+        """Returns ``(loss, lse)``, fp32 ``[n]`` each, new or in the given tensors."""
+        ldh, ldw, n, vocab, dim, labels = Softmax._operands(hidden, weight, targets)
+        dev, kind = hidden.device, TYPES[hidden.dtype]
+        loss = torch.empty(n, dtype=torch.float32, device=dev) if loss is None else loss
+        lse = torch.empty(n, dtype=torch.float32, device=dev) if lse is None else lse
+        _vector(loss, "loss", n, dev)
+        _vector(lse, "lse", n, dev)
+        with on_device(dev):
+            work, size = Softmax._workspace(n, vocab, dim, labels, kind, False, dev)
+            check(_lib.load().w2v_softmax_loss(hidden.data_ptr(), ldh, weight.data_ptr(), ldw, targets.data_ptr(), n,
+                                               vocab, dim, labels, kind, loss.data_ptr(), lse.data_ptr(),
+                                               work.data_ptr(), size, stream_of(dev)), "w2v_softmax_loss")
+        return loss, lse
+
+    @staticmethod
+    def grad(hidden, weight, targets, lse, gloss, dhidden=None, dweight=None):
+        """Gradients of ``sum_i gloss[i] loss[i]`` for ``hidden`` and ``weight``, of their type:
+        ``(dhidden, dweight)``, new or in the given tensors.  ``lse`` is what ``loss`` returned; ``gloss``
+        fp32 ``[n]``, or one element for all rows."""
+        ldh, ldw, n, vocab, dim, labels = Softmax._operands(hidden, weight, targets)
+        dev, kind = hidden.device, TYPES[hidden.dtype]
+        _vector(lse, "lse", n, dev)
+        if not isinstance(gloss, torch.Tensor) or gloss.dtype != torch.float32 or gloss.device != dev:
+            raise ValueError(f"gloss is an fp32 tensor on {dev}")
+        one = gloss.numel() == 1
+        if not one:
+            _vector(gloss, "gloss", n, dev)
+        dhidden = torch.empty(n, dim, dtype=hidden.dtype, device=dev) if dhidden is None else dhidden
+        dweight = torch.empty(vocab, dim, dtype=hidden.dtype, device=dev) if dweight is None else dweight
+        lddh = check_matrix(dhidden, "dhidden", dev, hidden.dtype)
+        lddw = check_matrix(dweight, "dweight", dev, hidden.dtype)
+        if tuple(dhidden.shape) != (n, dim) or tuple(dweight.shape) != (vocab, dim):
+            raise ValueError(f"dhidden is {(n, dim)} and dweight {(vocab, dim)}")
+        with on_device(dev):
+            work, size = Softmax._workspace(n, vocab, dim, labels, kind, True, dev)
+            check(_lib.load().w2v_softmax_grad(hidden.data_ptr(), ldh, weight.data_ptr(), ldw, targets.data_ptr(), n,
+                                               vocab, dim, labels, kind, lse.data_ptr(), gloss.data_ptr(),
+                                               0 if one else 1, dhidden.data_ptr(), lddh, dweight.data_ptr(), lddw,
+                                               work.data_ptr(), size, stream_of(dev)), "w2v_softmax_grad")
+        return dhidden, dweight

@@ -418,7 +418,8 @@ int64_t bidmach_lz4_decompress(const void *src, int64_t n, void *dst, int64_t ca
 
 /* -------------------------------------------------------------------------
  * Part 5 -- training operators over whole matrices (no counterpart among the
- * reference's native functions): rows by ids with their gradient, and AdamW.
+ * reference's native functions): softmax cross entropy over the vocabulary with
+ * its gradients, rows by ids with their gradient, and AdamW.
  *
  * Common to all of them: device pointers; work is enqueued on `stream` and
  * nothing waits for it; the calls can be captured into a CUDA graph; scratch
@@ -442,6 +443,28 @@ int64_t w2v_embed_grad_workspace(int64_t n, int64_t vocab, int dim, int type);  
 int w2v_embed_grad(const int *ids, int64_t n, const void *grad, int64_t ldg, int64_t vocab, int dim,
                    int type, void *out, int64_t ldo, void *workspace, int64_t workspace_bytes,
                    void *stream);
+
+/* Softmax cross entropy of n rows of hidden vectors against all words, in pieces of the vocabulary
+ * (no logits are kept).  With l = hidden weight^T, `labels` targets a row (targets is n x labels; one
+ * outside [0, vocab) stands for none, a row may have none or the same word twice):
+ *   lse[i]  = log sum_v exp l[i][v]
+ *   loss[i] = sum over the targets y of row i of (lse[i] - l[i][y])        (0 without any)
+ * hidden is n x dim, weight vocab x dim, both of `type`; loss and lse are fp32[n].  dim <= 4096,
+ * labels <= 1024.  A row of hidden with an infinity or a NaN gives a NaN in lse. */
+int64_t w2v_softmax_workspace(int64_t n, int64_t vocab, int dim, int labels, int type, int grad);   /* -1: refused */
+int w2v_softmax_loss(const void *hidden, int64_t ldh, const void *weight, int64_t ldw,
+                     const int *targets, int64_t n, int64_t vocab, int dim, int labels, int type,
+                     float *loss, float *lse, void *workspace, int64_t workspace_bytes, void *stream);
+/* Gradients of sum_i gloss[i * ldg] loss[i] (ldg 1, or 0 for one value for all rows), from the lse
+ * that w2v_softmax_loss gave: with k_i targets in row i
+ *   d[i][v] = gloss_i (k_i exp(l[i][v] - lse[i]) - targets of row i that are v)
+ *   dhidden = d weight,  dweight = d^T hidden
+ * both written whole, of `type`.  Equal calls give equal bits. */
+int w2v_softmax_grad(const void *hidden, int64_t ldh, const void *weight, int64_t ldw,
+                     const int *targets, int64_t n, int64_t vocab, int dim, int labels, int type,
+                     const float *lse, const float *gloss, int64_t ldg, void *dhidden, int64_t lddh,
+                     void *dweight, int64_t lddw, void *workspace, int64_t workspace_bytes,
+                     void *stream);
 
 /* One tensor of an AdamW step: `n` contiguous elements of `ptype`.  With 32-bit moments m and v are
  * fp32[n] and the scales null.  With 8-bit ones m and v are uint8[n] and every 256 elements share a

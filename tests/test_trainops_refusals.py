@@ -44,3 +44,26 @@ def test_c_entries_refuse_without_a_launch():
     assert lib.w2v_embed_rows(64, 3, 64, 3, 5, 4, 0, 64, 4, None) == 1       # rows overlap
     assert lib.w2v_embed_grad(64, 3, 64, 4, 5, 4, 0, 64, 4, 0, 0, None) == 1   # no workspace
     assert lib.w2v_launch_count() == before
+
+
+def test_softmax_refuses():
+    from bidmach_b200 import Softmax
+    lib = _lib.load()
+    before = lib.w2v_launch_count()
+    for n, vocab, dim, labels, kind in [(-1, 5, 4, 1, 0), (3, 0, 4, 1, 0), (3, 5, 0, 1, 0), (3, 5, 4097, 1, 0),
+                                        (3, 5, 4, 0, 0), (3, 5, 4, 1025, 0), (3, 5, 4, 1, 3), (3, 1 << 31, 4, 1, 0),
+                                        (1 << 31, 5, 4, 1, 0)]:
+        assert lib.w2v_softmax_workspace(n, vocab, dim, labels, kind, 1) == -1
+        assert lib.w2v_softmax_loss(64, dim, 64, dim, 64, n, vocab, dim, labels, kind, 64, 64, 256, 1 << 40, None) == 1
+    ok = (64, 4, 64, 4, 64, 20, 50, 4, 1, 0)
+    for ws, size in [(0, 1 << 40), (64, 1 << 40), (256, 0)]:     # none, not aligned, too small
+        assert lib.w2v_softmax_loss(*ok, 64, 64, ws, size, None) == 1
+        assert lib.w2v_softmax_grad(*ok, 64, 64, 1, 64, 4, 64, 4, ws, size, None) == 1
+    assert lib.w2v_softmax_grad(*ok, 64, 64, 2, 64, 4, 64, 4, 256, 1 << 40, None) == 1     # stride of gloss
+    assert lib.w2v_softmax_grad(*ok, 64, 64, 1, 64, 3, 64, 4, 256, 1 << 40, None) == 1     # rows overlap
+    assert lib.w2v_softmax_loss(64, 4, 64, 3, *ok[4:], 64, 64, 256, 1 << 40, None) == 1
+    assert lib.w2v_launch_count() == before
+    with pytest.raises(ValueError, match="CUDA"):
+        Softmax.loss(torch.zeros(3, 4), torch.zeros(5, 4), torch.zeros(3, dtype=torch.int32))
+    with pytest.raises(ValueError):
+        Softmax.loss(torch.zeros(3, 4, dtype=torch.float64), torch.zeros(5, 4), torch.zeros(3, dtype=torch.int32))
