@@ -276,20 +276,55 @@ __global__ void __launch_bounds__(kFewThreads) few_dh_kernel(const T *w, int64_t
   }
 }
 
-// out[r][c] = scale * sum over slabs, in their order.
+// What a gradient's sums have to be multiplied with: the powers of two that d and the other operand
+// were scaled by, and the one factor for all rows where there is one.
+struct Rescale {
+  const Scalars *sc;   // null: 1
+  const float *gloss;  // null: 1
+  int operand;         // 0: none scaled, 1: W, 2: H
+};
+__device__ __forceinline__ float rescale_of(const Rescale &r) {
+  float x = r.gloss ? *r.gloss : 1.f;
+  if (r.sc) {
+    x *= pow2(-scale_exp(r.sc->g, kProbTop));
+    if (r.operand) x *= pow2(-scale_exp(r.operand == 1 ? r.sc->w : r.sc->h, kOperandTop));
+  }
+  return x;
+}
+
+// out[r][c] = factor * sum over slabs, in their order; a warp a row.
 template <typename T>
 __global__ void __launch_bounds__(256) slabs_kernel(const float *slabs, int count, int64_t slab, int64_t lds, int64_t rows,
-                                                    int dim, T *out, int64_t ldo, const Scalars *sc, int which) {
-  float scale = 1.f;
-  if (sc) scale = pow2(-scale_exp(sc->g, kProbTop)) * (which == 0 ? 1.f : pow2(-scale_exp(which == 1 ? sc->w : sc->h, kOperandTop)));
-  const int64_t total = rows * dim, stride = (int64_t)gridDim.x * 256;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += stride) {
-    const int64_t r = i / dim;
-    const int c = (int)(i % dim);
+                                                    int dim, T *out, int64_t ldo, bool wide, const Rescale rescale) {
+  const float f = rescale_of(rescale);
+  const int lane = threadIdx.x & 31;
+  const int cols = (dim + 255) / 256;
+  const int64_t stride = (int64_t)gridDim.x * 8;
+  for (int64_t i = (int64_t)blockIdx.x * 8 + threadIdx.x / 32; i < rows * cols; i += stride) {
+    const int64_t r = cols == 1 ? i : i / cols;
+    const int c = (int)(i - r * cols) * 256 + lane * 8, have = min(8, dim - c);
+    if (have <= 0) continue;
     const float *p = slabs + r * lds + c;
-    float x = p[0];
-    for (int k = 1; k < count; k++) x += p[k * slab];
-    out[r * ldo + c] = from_float<T>(x * scale);
+    float x[8];
+    if (wide) load8(p, x);
+    else load_some(p, have, x);
+    for (int k = 1; k < count; k += 4) {
+      float y[4][8];
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        if (wide && k + j < count) load8(p + (k + j) * slab, y[j]);
+        else load_some(p + (k + j) * slab, k + j < count ? have : 0, y[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] += y[j][e];
+    }
+#pragma unroll
+    for (int e = 0; e < 8; e++) x[e] *= f;
+    T *to = out + r * ldo + c;
+    if (have == 8 && reinterpret_cast<uintptr_t>(to) % (8 * sizeof(T)) == 0) store8(to, x);
+    else store_some(to, have, x);
   }
 }
 
@@ -297,59 +332,75 @@ __global__ void __launch_bounds__(256) slabs_kernel(const float *slabs, int coun
 // Joining the parts of a row and the targets' logits
 // ---------------------------------------------------------------------------------------------
 constexpr int kJoinThreads = 256;
-constexpr int kJoinRows = 32;
+constexpr int kJoinRows = 8;
 
-// parts[k][row], row < ldp.  A lane is a row while the parts are read (they lie row by row); the
-// targets' dot products go to a warp each.
+// parts[k][row], row < ldp.  While the parts are read a warp is eight rows times four parts (the rows
+// of a part lie side by side); then a warp is a row, two targets' dot products at a time.
 template <typename T>
 __global__ void __launch_bounds__(kJoinThreads) loss_join_kernel(const Part *parts, int count, int64_t ldp, int rows,
                                                                  const T *h, int64_t ldh, const T *w, int64_t ldw,
-                                                                 int64_t vocab, int dim, const int *targets, int labels,
-                                                                 float *loss, float *lse) {
+                                                                 int64_t vocab, int dim, bool wide, const int *targets,
+                                                                 int labels, float *loss, float *lse) {
   __shared__ Part sums[kJoinThreads / 32][kJoinRows];
-  __shared__ float lse_s[kJoinRows];
   const int lane = threadIdx.x & 31, warp = threadIdx.x / 32, warps = kJoinThreads / 32;
   const int r0 = blockIdx.x * kJoinRows, here = min(kJoinRows, rows - r0);
   Part p{-INFINITY, 0.f};
-  if (here > 8) {
-    if (lane < here) {
-      for (int k = warp; k < count; k += warps * 4) {
-        Part x[4];
+  const int row = lane % kJoinRows;
+  constexpr int step = kJoinThreads / kJoinRows;
+  if (row < here)
+    for (int k = threadIdx.x / kJoinRows; k < count; k += step * 4) {
+      Part x[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-          x[j] = k + j * warps < count ? parts[(int64_t)(k + j * warps) * ldp + r0 + lane] : Part{-INFINITY, 0.f};
+      for (int j = 0; j < 4; j++)
+        x[j] = k + j * step < count ? parts[(int64_t)(k + j * step) * ldp + r0 + row] : Part{-INFINITY, 0.f};
 #pragma unroll
-        for (int j = 0; j < 4; j++) p = join(p, x[j]);
+      for (int j = 0; j < 4; j++) p = join(p, x[j]);
+    }
+#pragma unroll
+  for (int s = 16; s >= kJoinRows; s >>= 1)
+    p = join(p, Part{__shfl_xor_sync(kFullMask, p.m, s), __shfl_xor_sync(kFullMask, p.s, s)});
+  if (lane < kJoinRows) sums[warp][lane] = p;
+  __syncthreads();
+  if (warp >= here) return;
+  p = sums[0][warp];
+#pragma unroll
+  for (int k = 1; k < warps; k++) p = join(p, sums[k][warp]);
+  const float z = (p.m + log2f(p.s)) / kLog2e;
+  const int64_t n = r0 + warp;
+  const int *y = targets + n * labels;
+  const T *hr = h + n * ldh;
+  float sum = 0.f;
+  for (int j = 0; j < labels; j += 2) {
+    int at[2];
+    float x[2] = {0.f, 0.f};
+#pragma unroll
+    for (int q = 0; q < 2; q++) at[q] = j + q < labels ? y[j + q] : -1;
+    for (int c = lane * 8; c < dim; c += 256) {
+      const int have = min(8, dim - c);
+      float a[8], b[2][8];
+      if (wide && have == 8) load8(hr + c, a);
+      else load_some(hr + c, have, a);
+#pragma unroll
+      for (int q = 0; q < 2; q++) {
+        const bool there = at[q] >= 0 && at[q] < vocab;
+        const T *wr = w + (there ? (int64_t)at[q] : 0) * ldw + c;
+        if (wide && there && have == 8) load8(wr, b[q]);
+        else load_some(wr, there ? have : 0, b[q]);
       }
-    }
-    sums[warp][lane] = p;
-    __syncthreads();
-    if (warp == 0) {
-      for (int k = 1; k < warps; k++) p = join(p, sums[k][lane]);
-      lse_s[lane] = (p.m + log2f(p.s)) / kLog2e;
-    }
-  } else {
-    if (warp < here) {   // a warp a row, its lanes share the parts
-      for (int k = lane; k < count; k += 32) p = join(p, parts[(int64_t)k * ldp + r0 + warp]);
 #pragma unroll
-      for (int s = 16; s > 0; s >>= 1)
-        p = join(p, Part{__shfl_xor_sync(kFullMask, p.m, s), __shfl_xor_sync(kFullMask, p.s, s)});
-      if (lane == 0) lse_s[warp] = (p.m + log2f(p.s)) / kLog2e;
+      for (int q = 0; q < 2; q++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[q] = fmaf(a[e], b[q][e], x[q]);
+    }
+#pragma unroll
+    for (int q = 0; q < 2; q++) {
+      const float l = warp_sum(x[q]);
+      if (at[q] >= 0 && at[q] < vocab) sum += z - l;
     }
   }
-  __syncthreads();
-  if (threadIdx.x < here) lse[r0 + threadIdx.x] = lse_s[threadIdx.x];
-  for (int r = warp; r < here; r += warps) {
-    const int64_t n = r0 + r;
-    float sum = 0.f;
-    for (int j = 0; j < labels; j++) {
-      const int y = targets[n * labels + j];
-      if (y < 0 || y >= vocab) continue;
-      float x = 0.f;
-      for (int c = lane; c < dim; c += 32) x = fmaf(to_float(h[n * ldh + c]), to_float(w[(int64_t)y * ldw + c]), x);
-      sum += lse_s[r] - warp_sum(x);
-    }
-    if (lane == 0) loss[n] = sum;
+  if (lane == 0) {
+    lse[n] = z;
+    loss[n] = sum;
   }
 }
 
@@ -387,7 +438,7 @@ __global__ void __launch_bounds__(256) amax_kernel(Source h, Source w, int dim, 
   } else if (gloss) {
     for (int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x; n < h.rows; n += (int64_t)gridDim.x * 256) {
       const int k = valid_targets(targets + n * labels, labels, vocab);
-      if (k) top = max(top, __float_as_uint(gloss[n * ldg] * (float)k) & 0x7fffffffu);
+      if (k) top = max(top, __float_as_uint((ldg ? gloss[n] : 1.f) * (float)k) & 0x7fffffffu);
     }
     block_max(top, &sc->g);
   }
@@ -444,7 +495,8 @@ __global__ void __launch_bounds__(256) row_coef_kernel(const float *lse, const f
                                                        const Scalars *sc, RowCoef *out) {
   const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (n >= rows) return;
-  const float g = gloss[n * ldg] * pow2(scale_exp(sc->g, kProbTop));
+  // one factor for all rows is left to the end: the targets' -1 then has no rounding in d
+  const float g = (ldg ? gloss[n] : 1.f) * pow2(scale_exp(sc->g, kProbTop));
   const int k = valid_targets(targets + n * labels, labels, vocab);
   // lse log2e to twice the precision: what the rounded exponent lacks goes into the factor
   const float hi = lse[n] * kLog2e, lo = fmaf(lse[n], kLog2e, -hi);
@@ -460,13 +512,15 @@ constexpr int kBytesA = kM * kK * 2, kBytesB = kN * kK * 2;
 constexpr int kMmaThreads = 384;   // producer, issuer, two idle warps, eight that read the tiles
 constexpr int kSmem = kStages * (kBytesA + kBytesB) + 1024;
 
-enum Use { kLogits, kProbs, kGrad };
+enum Use { kLogits, kProbs, kGrad, kGradSegments };
+__host__ __device__ constexpr bool is_grad(Use u) { return u == kGrad || u == kGradSegments; }
 
 struct Product {
   CUtensorMap a, b;
   int mt, nt, ntile;      // tiles, columns a tile (a multiple of 16)
   int splits, kblocks;    // of 64, over all splits, for one pair of parts
-  int pairs, pa[3], pb[3];// offsets of the parts that are multiplied
+  int pairs, pa[3], pb[3];// offsets of the parts that are multiplied, the smaller products first
+  int k16;                // steps of 16 in the last block of K
   int a_mn, b_mn;         // operands whose rows run along K
   int a_y, b_y;           // first row of each in its matrix
   int bf16;
@@ -481,14 +535,19 @@ struct Product {
   const RowCoef *coef;
   const int *targets;
   int labels;
-  uint16_t *probs;
-  int64_t ldprobs;
-  int prob_lo;            // offset of the second part, 0 for none
+  uint16_t *probs;        // d in strips of 64 columns: [part][strip][row][64]
+  int strip;              // rows of a strip
+  int64_t prob_lo;        // offset of the second part, 0 for none
   // gradients
+  int segment;            // blocks of K that are accumulated in tensor memory at a time
+  float *scratch;         // kM x kN for each block
   float *acc;             // [splits][acc_rows][ldacc]
   int64_t acc_slab, ldacc;
   int add;                // to what is there already
-  int dim;
+  void *out;              // not null: the finished gradient goes here, not to acc
+  int64_t ldout;
+  int out_type, out_wide, dim;
+  Rescale rescale;
 };
 
 __device__ __forceinline__ void store32(void *a, const uint32_t (&r)[8]) {
@@ -509,7 +568,7 @@ __device__ __forceinline__ uint32_t halves(float a, float b) {
 
 // 32 values to 16 bits at `to` (32-byte aligned), and what that lacks, times 2^11, `lo` elements on.
 template <bool BF16, bool LO>
-__device__ __forceinline__ void store_probs(uint16_t *to, int lo, const float (&x)[32]) {
+__device__ __forceinline__ void store_probs(uint16_t *to, int64_t lo, const float (&x)[32]) {
 #pragma unroll
   for (int b = 0; b < 2; b++) {
     uint32_t r[8], s[8];
@@ -529,7 +588,7 @@ __device__ __forceinline__ void store_probs(uint16_t *to, int lo, const float (&
 
 template <Use USE>
 __device__ __forceinline__ void tile_of(const Product &p, int t, int &m, int &n, int &k) {
-  if (USE == kGrad) {   // blocks that run together share a strip of d
+  if (is_grad(USE)) {   // blocks that run together share a strip of d
     n = t % p.nt;
     m = t / p.nt % p.mt;
     k = t / (p.nt * p.mt);
@@ -538,6 +597,39 @@ __device__ __forceinline__ void tile_of(const Product &p, int t, int &m, int &n,
     n = t / p.mt;
     k = 0;
   }
+}
+
+template <typename T>
+__device__ __forceinline__ void put_typed(T *to, bool wide, int have, const float (&v)[8]) {
+  if (wide && have == 8) store8(to, v);
+  else store_some(to, have, v);
+}
+
+// Eight columns of a gradient's tile, from column `col` of it.
+__device__ __forceinline__ void put_grad(const Product &p, int64_t r, int n, int k, int col, const float *x, float factor) {
+  const int at = n * p.ntile + col;
+  if (r >= p.rows || col >= p.ntile || at >= p.dim) return;
+  float v[8];
+#pragma unroll
+  for (int e = 0; e < 8; e++) v[e] = x[e];
+  if (p.out) {
+    const int have = min(8, p.dim - at);
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] *= factor;
+    const int64_t to = r * p.ldout + at;
+    if (p.out_type == W2V_F32) put_typed(static_cast<float *>(p.out) + to, p.out_wide, have, v);
+    else if (p.out_type == W2V_BF16) put_typed(static_cast<__nv_bfloat16 *>(p.out) + to, p.out_wide, have, v);
+    else put_typed(static_cast<__half *>(p.out) + to, p.out_wide, have, v);
+    return;
+  }
+  float *to = p.acc + k * p.acc_slab + r * p.ldacc + at;
+  if (p.add) {
+    float old[8];
+    load8(to, old);
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] += old[e];
+  }
+  store8(to, v);
 }
 
 template <Use USE>
@@ -581,9 +673,10 @@ __global__ void __launch_bounds__(kMmaThreads, 1) product_kernel(const __grid_co
       for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
         int m, n, k;
         tile_of<USE>(p, t, m, n, k);
-        const int k0 = first_k(k), k1 = first_k(k + 1);
+        const int kend = first_k(k + 1);
+        for (int k0 = first_k(k); ok && k0 < kend; k0 += p.segment)
         for (int q = 0; ok && q < p.pairs; q++)
-          for (int kb = k0; kb < k1; kb++, it++) {
+          for (int kb = k0; kb < min(kend, k0 + p.segment); kb++, it++) {
             const int s = it % kStages;
             if (!mbar_wait(&empty[s], (it / kStages + 1) & 1, gave_up)) {
               ok = false;
@@ -591,11 +684,13 @@ __global__ void __launch_bounds__(kMmaThreads, 1) product_kernel(const __grid_co
             }
             mbar_arrive_expect_tx(&full[s], bytes);
             unsigned char *sa = smem + s * (kBytesA + kBytesB), *sb = sa + kBytesA;
-            if (p.a_mn) {
-              for (int g = 0; g < 2; g++)
-                tma_load_2d(sa + g * 8192, &p.a, p.pa[q] + m * kM + g * 64, p.a_y + kb * kK, &full[s]);
-            } else {
+            if (!is_grad(USE)) {
               tma_load_2d(sa, &p.a, p.pa[q] + kb * kK, p.a_y + m * kM, &full[s]);
+            } else if (p.a_mn) {   // d transposed: 64 rows of two strips
+              for (int g = 0; g < 2; g++)
+                tma_load_2d(sa + g * 8192, &p.a, 0, p.pa[q] + (2 * m + g) * p.strip + kb * kK, &full[s]);
+            } else {               // 128 rows of a strip
+              tma_load_2d(sa, &p.a, 0, p.pa[q] + kb * p.strip + m * kM, &full[s]);
             }
             if (p.b_mn) {
               for (unsigned g = 0; g < groups_b; g++)
@@ -617,31 +712,39 @@ __global__ void __launch_bounds__(kMmaThreads, 1) product_kernel(const __grid_co
       bool ok = true;
       const uint32_t idesc = mma_desc(p.bf16, p.a_mn, p.b_mn, kM, p.ntile);
       const uint32_t step_a = p.a_mn ? 2048 >> 4 : 32 >> 4, step_b = p.b_mn ? 2048 >> 4 : 32 >> 4;
-      for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x, local++) {
+      for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
         int m, n, k;
         tile_of<USE>(p, t, m, n, k);
-        const int blocks = p.pairs * (first_k(k + 1) - first_k(k));
-        const int buf = local & 1;
-        if (!mbar_wait(&tempty[buf], (local / 2 + 1) & 1, gave_up)) {
-          ok = false;
-          break;
-        }
-        tmem_after_sync();
-        for (int b = 0; b < blocks; b++, it++) {
-          const int s = it % kStages;
-          if (!mbar_wait(&full[s], (it / kStages) & 1, gave_up)) {
+        const int kend = first_k(k + 1);
+        for (int k0 = first_k(k); ok && k0 < kend; k0 += p.segment, local++) {
+          const int buf = local & 1, k1 = min(kend, k0 + p.segment);
+          if (!mbar_wait(&tempty[buf], (local / 2 + 1) & 1, gave_up)) {
             ok = false;
             break;
           }
           tmem_after_sync();
-          const uint32_t sa = smem_addr(smem + s * (kBytesA + kBytesB)), sb = sa + kBytesA;
-          const uint64_t da = smem_desc(sa, p.a_mn ? 8192 : 16, 1024), db = smem_desc(sb, p.b_mn ? 8192 : 16, 1024);
+          bool add = false;
+          for (int q = 0; ok && q < p.pairs; q++)
+            for (int kb = k0; kb < k1; kb++, it++) {
+              const int s = it % kStages;
+              if (!mbar_wait(&full[s], (it / kStages) & 1, gave_up)) {
+                ok = false;
+                break;
+              }
+              tmem_after_sync();
+              const uint32_t sa = smem_addr(smem + s * (kBytesA + kBytesB)), sb = sa + kBytesA;
+              const uint64_t da = smem_desc(sa, p.a_mn ? 8192 : 16, 1024), db = smem_desc(sb, p.b_mn ? 8192 : 16, 1024);
+              const int steps = kb == p.kblocks - 1 ? p.k16 : kK / 16;
 #pragma unroll
-          for (int i = 0; i < kK / 16; i++)
-            mma_f16(tmem + buf * 256, da + i * step_a, db + i * step_b, idesc, b > 0 || i > 0);
-          mma_commit(&empty[s]);
+              for (int i = 0; i < kK / 16; i++)
+                if (i < steps) {
+                  mma_f16(tmem + buf * 256, da + i * step_a, db + i * step_b, idesc, add);
+                  add = true;
+                }
+              mma_commit(&empty[s]);
+            }
+          if (ok) mma_commit(&tfull[buf]);
         }
-        if (ok) mma_commit(&tfull[buf]);
       }
       if (!ok) {   // products in flight still read shared memory
         int none = 0;
@@ -655,23 +758,31 @@ __global__ void __launch_bounds__(kMmaThreads, 1) product_kernel(const __grid_co
     const int row = quarter * 32 + lane;
     const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
     float c = kLog2e;
-    if (USE != kGrad && p.split_scale)
+    if (!is_grad(USE) && p.split_scale)
       c = kLog2e * pow2(-scale_exp(p.sc->h, kOperandTop)) * pow2(-scale_exp(p.sc->w, kOperandTop));
+    const float factor = is_grad(USE) ? rescale_of(p.rescale) : 1.f;
     int local = 0;
     bool ok = true;
-    for (int t = blockIdx.x; t < tiles; t += gridDim.x, local++) {
-      int m, n, k;
-      tile_of<USE>(p, t, m, n, k);
-      const int buf = local & 1;
-      // a block that gave up fills its tiles with NaN: nothing it did not compute passes for a result
+    // a block that gave up fills its tiles with NaN: nothing it did not compute passes for a result
+    auto begin = [&](int buf) {
       ok = ok && mbar_wait(&tfull[buf], (local / 2) & 1, gave_up);
       ok = __all_sync(kFullMask, ok);
       tmem_after_sync();
-      const int chunks = (p.ntile + 31) / 32;
+    };
+    auto end = [&](int buf) {
+      tmem_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&tempty[buf]);
+      local++;
+    };
+    const int chunks = (p.ntile + 31) / 32;
+    for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
+      int m, n, k;
+      tile_of<USE>(p, t, m, n, k);
       const int64_t r = (int64_t)m * kM + row;
       auto fetch = [&](int ch, float (&x)[32]) {
         if (ok) {
-          tmem_load32(lanes + buf * 256 + ch * 32, x);
+          tmem_load32(lanes + (local & 1) * 256 + ch * 32, x);
           tmem_wait_load();
         } else {
 #pragma unroll
@@ -679,6 +790,8 @@ __global__ void __launch_bounds__(kMmaThreads, 1) product_kernel(const __grid_co
         }
       };
       if (USE == kLogits) {
+        const int buf = local & 1;
+        begin(buf);
         Part part{-INFINITY, 0.f};
         const int64_t left = p.vocab - (int64_t)n * kN;   // columns of the tile that are words
         for (int ch = half; ch < chunks; ch += 2) {
@@ -707,7 +820,9 @@ __global__ void __launch_bounds__(kMmaThreads, 1) product_kernel(const __grid_co
           part.s += s0 + s1;
         }
         if (r < p.rows) p.parts[(int64_t)(2 * n + half) * p.ldparts + r] = part;
+        end(buf);
       } else if (USE == kProbs) {
+        const int buf = local & 1;
         RowCoef rc{INFINITY, 0.f, 0.f, 0.f};
         if (r < p.rows) rc = p.coef[r];
         const int64_t left = p.vocab - p.word0 - (int64_t)n * kN;
@@ -719,6 +834,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) product_kernel(const __grid_co
             const int64_t at = y[j] - first;
             if (at >= 0 && at < kN) hits |= 1u << (at >> 5);
           }
+        begin(buf);
         for (int ch = half; ch < chunks; ch += 2) {
           float x[32];
           fetch(ch, x);
@@ -738,32 +854,52 @@ __global__ void __launch_bounds__(kMmaThreads, 1) product_kernel(const __grid_co
               }
             __syncwarp();
           }
-          uint16_t *to = p.probs + r * p.ldprobs + n * kN + ch * 32;
+          uint16_t *to = p.probs + ((int64_t)(n * (kN / 64) + ch / 2) * p.strip + r) * 64 + ch % 2 * 32;
           if (p.bf16) store_probs<true, false>(to, 0, x);
           else if (p.prob_lo) store_probs<false, true>(to, p.prob_lo, x);
           else store_probs<false, false>(to, 0, x);
         }
-      } else {
-        float *row_acc = p.acc + k * p.acc_slab + r * p.ldacc + n * p.ntile;
+        end(buf);
+      } else if (USE == kGrad) {
+        const int buf = local & 1;
+        begin(buf);
         for (int ch = half; ch < chunks; ch += 2) {
           float x[32];
           fetch(ch, x);
-          if (r >= p.rows) continue;
 #pragma unroll
-          for (int b = 0; b < 4; b++) {
-            const int col = ch * 32 + b * 8;
-            if (col >= p.ntile || n * p.ntile + col >= p.dim) break;
-            float v[8];
-            if (p.add) load8(row_acc + col, v);
+          for (int b = 0; b < 4; b++) put_grad(p, r, n, k, ch * 32 + b * 8, &x[b * 8], factor);
+        }
+        end(buf);
+      } else {
+        // the tensor cores truncate what they accumulate: after `segment` blocks of K the sum goes on in
+        // fp32 with rounding, in a scratch of the block's own that stays in L2 (a thread's eight values
+        // side by side, a warp's in one piece); registers for it would spill
+        float *mine = p.scratch + (int64_t)blockIdx.x * kM * kN + (threadIdx.x - 128) * 8;
+        const int kstart = first_k(k), kend = first_k(k + 1);
+        for (int k0 = kstart; k0 < kend; k0 += p.segment) {
+          const int buf = local & 1;
+          begin(buf);
+          for (int ch = half; ch < chunks; ch += 2) {
+            float x[32];
+            float *at = mine + ch / 2 * (4 * 256 * 8);
+            float old[4][8];
+            if (k0 > kstart) {
 #pragma unroll
-            for (int e = 0; e < 8; e++) v[e] = p.add ? v[e] + x[b * 8 + e] : x[b * 8 + e];
-            store8(row_acc + col, v);
+              for (int b = 0; b < 4; b++) load8(at + b * (256 * 8), old[b]);
+            }
+            fetch(ch, x);
+#pragma unroll
+            for (int b = 0; b < 4; b++) {
+              float v[8];
+#pragma unroll
+              for (int e = 0; e < 8; e++) v[e] = k0 > kstart ? x[b * 8 + e] + old[b][e] : x[b * 8 + e];
+              if (k0 + p.segment < kend) store8(at + b * (256 * 8), v);
+              else put_grad(p, r, n, k, ch * 32 + b * 8, v, factor);
+            }
           }
+          end(buf);
         }
       }
-      tmem_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&tempty[buf]);
     }
   }
   tmem_before_sync();
@@ -840,7 +976,8 @@ bool good_shape(const Shape &x) {
 
 constexpr int64_t kLossRows = 16384;            // rows whose parts are kept at a time
 constexpr int64_t kGradRows = 8192;             // rows of a piece of d
-constexpr int64_t kProbBytes = (int64_t)64 << 20;   // of a piece: half of L2
+constexpr int64_t kProbBytes = (int64_t)512 << 20;
+constexpr int kSegment = 8;                     // fp32 gradients: blocks of K between two roundings
 
 int few_blocks(int64_t vocab) {
   const int64_t need = (vocab + kFewThreads / 32 * kFewWords - 1) / (kFewThreads / 32 * kFewWords);
@@ -852,10 +989,11 @@ int few_dh_blocks(int64_t vocab) {
 int few_rows_of(int64_t n) { return n <= 1 ? 1 : n <= 2 ? 2 : n <= 4 ? 4 : 8; }
 
 struct Layout {
-  int64_t scalars, coef, hs, ws, parts, probs, acc_h, acc_w, total;
+  int64_t scalars, coef, hs, ws, parts, probs, scratch, acc_h, acc_w, total;
   int width, nparts;         // staged operands
   int64_t rows, words;       // of a piece of d
   int nt, ntile, hsplits, wsplits;
+  bool direct_h, direct_w;   // sums are complete in one go: no slabs
 };
 
 // Column tiles of a gradient: as few as hold dim, equally wide.
@@ -863,9 +1001,21 @@ void column_tiles(int dim, int *nt, int *ntile) {
   *nt = (dim + kN - 1) / kN;
   *ntile = (int)up((dim + *nt - 1) / *nt, 16);
 }
-int splits_for(int64_t tiles, int64_t kblocks) {
-  const int64_t s = device_sm_count() / std::max<int64_t>(tiles, 1);
-  return (int)std::max<int64_t>(1, std::min<int64_t>(s, kblocks / 4));
+// In how many parts K is cut, each with a slab of sums of its own: as many as fill the SMs' last round
+// best, where a slab costs about what 1 / 32 of a round does.
+int splits_for(int64_t tiles, int64_t kblocks, int most) {
+  const int sms = device_sm_count();
+  int best = 1;
+  double cost = 1e30;
+  for (int s = 1; s <= most && s * 4 <= std::max<int64_t>(kblocks, 4); s++) {
+    const double rounds = (double)((tiles * s + sms - 1) / sms) / s;
+    const double c = rounds * (1 + 0.03 * (s > 1)) + 0.03 * (s - 1) * rounds;
+    if (c < cost) {
+      cost = c;
+      best = s;
+    }
+  }
+  return best;
 }
 
 Layout plan(const Shape &x, bool grad) {
@@ -899,12 +1049,15 @@ Layout plan(const Shape &x, bool grad) {
     l.rows = up(std::min(x.n, kGradRows), kM);
     l.words = std::min(up(x.vocab, kN), std::max<int64_t>(kN, kProbBytes / (l.rows * bytes) / kN * kN));
     column_tiles(x.dim, &l.nt, &l.ntile);
-    l.hsplits = splits_for(l.rows / kM * l.nt, l.words / kK);
-    l.wsplits = splits_for(l.words / kM * l.nt, l.rows / kK);
+    l.hsplits = splits_for(l.rows / kM * l.nt, l.words / kK, 32);
+    l.wsplits = splits_for(l.words / kM * l.nt, l.rows / kK, 8);
     l.coef = take(x.n * sizeof(RowCoef));
     l.probs = take(l.rows * l.words * bytes);
-    l.acc_h = take((int64_t)l.hsplits * l.rows * l.nt * l.ntile * 4);
-    l.acc_w = take((int64_t)l.wsplits * up(x.vocab, kM) * l.nt * l.ntile * 4);
+    if (x.type == W2V_F32) l.scratch = take((int64_t)device_sm_count() * kM * kN * 4);
+    l.direct_h = l.hsplits == 1 && l.words >= x.vocab;
+    l.direct_w = l.wsplits == 1 && l.rows >= x.n;
+    if (!l.direct_h) l.acc_h = take((int64_t)l.hsplits * l.rows * l.nt * l.ntile * 4);
+    if (!l.direct_w) l.acc_w = take((int64_t)l.wsplits * up(x.vocab, kM) * l.nt * l.ntile * 4);
   }
   l.total = at;
   return l;
@@ -950,10 +1103,12 @@ Product logits_product(const Shape &x, const Operand &oh, const Operand &ow, con
   p.splits = 1;
   p.kblocks = (x.dim + kK - 1) / kK;
   p.pairs = split ? 3 : 1;
-  if (split) {   // hi hi, hi lo, lo hi
+  if (split) {   // lo hi, hi lo, hi hi
+    p.pa[0] = oh.width;
     p.pb[1] = ow.width;
-    p.pa[2] = oh.width;
   }
+  p.segment = p.kblocks;
+  p.k16 = (x.dim - (p.kblocks - 1) * kK + 15) / 16;
   p.bf16 = x.type == W2V_BF16;
   p.sc = sc;
   p.split_scale = split;
@@ -980,10 +1135,11 @@ template <typename T>
 int run_loss(const Shape &x, const Layout &l, const void *h, int64_t ldh, const void *w, int64_t ldw, const int *targets,
              float *loss, float *lse, char *ws, cudaStream_t s) {
   Part *parts = reinterpret_cast<Part *>(ws + l.parts);
+  const bool wide = aligned(h, 8 * sizeof(T)) && ldh % 8 == 0 && aligned(w, 8 * sizeof(T)) && ldw % 8 == 0;
   auto join_rows = [&](int count, int64_t ldp, int64_t r0, int rows) {
     loss_join_kernel<T><<<(rows + kJoinRows - 1) / kJoinRows, kJoinThreads, 0, s>>>(
         parts, count, ldp, rows, static_cast<const T *>(h) + r0 * ldh, ldh, static_cast<const T *>(w), ldw, x.vocab,
-        x.dim, targets + r0 * x.labels, x.labels, loss + r0, lse + r0);
+        x.dim, wide, targets + r0 * x.labels, x.labels, loss + r0, lse + r0);
     count_launch(1);
     return (int)cudaGetLastError();
   };
@@ -1031,8 +1187,8 @@ int few_grad(const Shape &x, const Layout &l, const void *h, int64_t ldh, const 
   const int blocks = few_dh_blocks(x.vocab);
   few_dh_kernel<T, RB><<<dim3(blocks, (x.dim + kFewThreads - 1) / kFewThreads), kFewThreads, 0, s>>>(wt, ldw, x.vocab,
                                                                                                     x.dim, d, acc);
-  slabs_kernel<T><<<(int)std::min<int64_t>((x.n * x.dim + 255) / 256, 1024), 256, 0, s>>>(
-      acc, blocks, (int64_t)RB * x.dim, x.dim, x.n, x.dim, static_cast<T *>(dh), lddh, nullptr, 0);
+  slabs_kernel<T><<<(int)std::min<int64_t>((x.n * ((x.dim + 255) / 256) + 7) / 8, 1024), 256, 0, s>>>(
+      acc, blocks, (int64_t)RB * x.dim, x.dim, x.n, x.dim, static_cast<T *>(dh), lddh, false, Rescale{nullptr, nullptr, 0});
   count_launch(3);
   return (int)cudaGetLastError();
 }
@@ -1059,10 +1215,15 @@ int run_grad(const Shape &x, const Layout &l, const void *h, int64_t ldh, const 
   row_coef_kernel<<<(int)((x.n + 255) / 256), 256, 0, s>>>(lse, gloss, ldg, targets, x.labels, x.vocab, x.n, sc, coef);
   count_launch(1);
   const int64_t ldacc = (int64_t)l.nt * l.ntile;
-  const Operand probs{ws + l.probs, l.words * (split ? 2 : 1), l.words * (split ? 2 : 1), l.rows, (int)l.words};
+  // d lies in strips of 64 columns, 128 bytes a row: what a warp writes of a tile, and what a load of
+  // either gradient's operand reads, is one piece of memory
+  const int strips = (int)(l.words / 64) * (split ? 2 : 1);
+  const Operand probs{ws + l.probs, 64, 64, strips * l.rows, (int)(l.words / 64 * l.rows)};
   float *acc_h = reinterpret_cast<float *>(ws + l.acc_h), *acc_w = reinterpret_cast<float *>(ws + l.acc_w);
   const int64_t acc_w_rows = up(x.vocab, kM);
   const int sums = device_sm_count() * 8;
+  const float *one_gloss = ldg ? nullptr : gloss;
+  const Rescale rescale_h{sc, one_gloss, split ? 1 : 0}, rescale_w{sc, one_gloss, split ? 2 : 0};
   for (int64_t r0 = 0; r0 < x.n; r0 += l.rows) {
     const int rows = (int)std::min(l.rows, x.n - r0);
     for (int64_t v0 = 0; v0 < x.vocab; v0 += l.words) {
@@ -1077,8 +1238,8 @@ int run_grad(const Shape &x, const Layout &l, const void *h, int64_t ldh, const 
       p.targets = targets + r0 * x.labels;
       p.labels = x.labels;
       p.probs = static_cast<uint16_t *>(const_cast<void *>(probs.p));
-      p.ldprobs = probs.ld;
-      p.prob_lo = split ? probs.width : 0;
+      p.strip = (int)l.rows;
+      p.prob_lo = split ? (int64_t)probs.width * 64 : 0;
       err = launch_product<kProbs>(p, oh, ow, s);
       if (err) return err;
       for (int which = 0; which < 2; which++) {   // dH, then dW
@@ -1092,32 +1253,47 @@ int run_grad(const Shape &x, const Layout &l, const void *h, int64_t ldh, const 
         // first piece, never the shorter one, has filled
         q.splits = std::min(which == 0 ? l.hsplits : l.wsplits, q.kblocks);
         q.pairs = split ? 3 : 1;
-        if (split) {   // hi hi, hi lo, (lo 2^11) (hi 2^-11)
+        if (split) {   // (lo 2^11) (hi 2^-11), hi lo, hi hi
+          q.pa[0] = probs.width;
+          q.pb[0] = 2 * o.width;
           q.pb[1] = o.width;
-          q.pa[2] = probs.width;
-          q.pb[2] = 2 * o.width;
         }
+        q.segment = split ? kSegment : q.kblocks;
+        q.k16 = kK / 16;
+        q.scratch = reinterpret_cast<float *>(ws + l.scratch);
+        q.strip = (int)l.rows;
         q.a_mn = which;
         q.b_mn = 1;
         q.b_y = (int)(which == 0 ? v0 : r0);
         q.bf16 = x.type == W2V_BF16;
         q.rows = which == 0 ? rows : words;
-        q.dim = (int)ldacc;
+        q.dim = x.dim;
         q.ldacc = ldacc;
         q.acc = which == 0 ? acc_h : acc_w + v0 * ldacc;
         q.acc_slab = (which == 0 ? l.rows : acc_w_rows) * ldacc;
         q.add = which == 0 ? v0 > 0 : r0 > 0;
-        err = launch_product<kGrad>(q, probs, o, s);
+        q.rescale = which == 0 ? rescale_h : rescale_w;
+        if (which == 0 ? l.direct_h : l.direct_w) {
+          q.out = which == 0 ? static_cast<T *>(dh) + r0 * lddh : static_cast<T *>(dw) + v0 * lddw;
+          q.ldout = which == 0 ? lddh : lddw;
+          q.out_type = x.type;
+          q.out_wide = aligned(q.out, 8 * sizeof(T)) && q.ldout % 8 == 0;
+        }
+        err = split ? launch_product<kGradSegments>(q, probs, o, s) : launch_product<kGrad>(q, probs, o, s);
         if (err) return err;
       }
     }
-    slabs_kernel<T><<<sums, 256, 0, s>>>(acc_h, l.hsplits, l.rows * ldacc, ldacc, rows, x.dim,
-                                         static_cast<T *>(dh) + r0 * lddh, lddh, sc, split ? 1 : 0);
+    if (!l.direct_h) {
+      slabs_kernel<T><<<sums, 256, 0, s>>>(acc_h, l.hsplits, l.rows * ldacc, ldacc, rows, x.dim,
+                                           static_cast<T *>(dh) + r0 * lddh, lddh, true, rescale_h);
+      count_launch(1);
+    }
+  }
+  if (!l.direct_w) {
+    slabs_kernel<T><<<sums, 256, 0, s>>>(acc_w, l.wsplits, acc_w_rows * ldacc, ldacc, x.vocab, x.dim,
+                                         static_cast<T *>(dw), lddw, true, rescale_w);
     count_launch(1);
   }
-  slabs_kernel<T><<<sums, 256, 0, s>>>(acc_w, l.wsplits, acc_w_rows * ldacc, ldacc, x.vocab, x.dim,
-                                       static_cast<T *>(dw), lddw, sc, split ? 2 : 0);
-  count_launch(1);
   return (int)cudaGetLastError();
 }
 
