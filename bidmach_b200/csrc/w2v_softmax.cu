@@ -507,8 +507,9 @@ __global__ void __launch_bounds__(256) row_coef_kernel(const float *lse, const f
 // ---------------------------------------------------------------------------------------------
 // The product
 // ---------------------------------------------------------------------------------------------
-constexpr int kM = 128, kN = 256, kK = 64, kStages = 4;
-constexpr int kBytesA = kM * kK * 2, kBytesB = kN * kK * 2;
+constexpr int kM = 128, kN = 256, kK = 64, kStages = 6;   // rows of each of a pair's CTAs, columns of both
+constexpr int kPairM = 2 * kM;
+constexpr int kBytesA = kM * kK * 2, kBytesB = kN / 2 * kK * 2;
 constexpr int kMmaThreads = 384;   // producer, issuer, two idle warps, eight that read the tiles
 constexpr int kSmem = kStages * (kBytesA + kBytesB) + 1024;
 
@@ -517,7 +518,7 @@ __host__ __device__ constexpr bool is_grad(Use u) { return u == kGrad || u == kG
 
 struct Product {
   CUtensorMap a, b;
-  int mt, nt, ntile;      // tiles, columns a tile (a multiple of 16)
+  int mt, nt, ntile;      // tiles of kPairM rows, columns a tile (a multiple of 32)
   int splits, kblocks;    // of 64, over all splits, for one pair of parts
   int pairs, pa[3], pb[3];// offsets of the parts that are multiplied, the smaller products first
   int k16;                // steps of 16 in the last block of K
@@ -633,7 +634,7 @@ __device__ __forceinline__ void put_grad(const Product &p, int64_t r, int n, int
 }
 
 template <Use USE>
-__global__ void __launch_bounds__(kMmaThreads, 1) product_kernel(const __grid_constant__ Product p) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) product_kernel(const __grid_constant__ Product p) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char *smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
   __shared__ u64 full[kStages], empty[kStages], tfull[2], tempty[2], done;
@@ -648,7 +649,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) product_kernel(const __grid_co
     }
     for (int i = 0; i < 2; i++) {
       mbar_init(&tfull[i], 1);
-      mbar_init(&tempty[i], 8);
+      mbar_init(&tempty[i], 16);   // the warps that read tiles, of both CTAs
     }
     mbar_init(&done, 1);
     gave_up_s = 0;
@@ -657,20 +658,22 @@ __global__ void __launch_bounds__(kMmaThreads, 1) product_kernel(const __grid_co
   }
   if (warp == 2) tmem_alloc(&tmem_at, 512);
   tmem_before_sync();
-  __syncthreads();
+  cluster_sync();
   tmem_after_sync();
   const uint32_t tmem = tmem_at;
+  const int rank = (int)cluster_rank(), pair = blockIdx.x / 2, npairs = gridDim.x / 2;
   const int tiles = p.mt * p.nt * p.splits;
   // blocks of K that a split starts with: every split has one at least (splits <= kblocks)
   auto first_k = [&](int k) { return (int)((int64_t)k * p.kblocks / p.splits); };
 
   if (warp == 0) {
-    if (lane == 0) {
+    if (elected()) {
       int it = 0;
       bool ok = true;
-      const unsigned groups_b = p.b_mn ? (p.ntile + 63) / 64 : 0;
-      const unsigned bytes = kBytesA + (p.b_mn ? groups_b * 8192 : kBytesB);
-      for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+      // each CTA brings its own rows of A and half of the columns of B; the leader counts both
+      const int half_n = p.ntile / 2, groups_b = (half_n + 63) / 64;
+      const unsigned bytes = 2 * (kBytesA + (is_grad(USE) ? groups_b * 8192 : kBytesB));
+      for (int t = pair; ok && t < tiles; t += npairs) {
         int m, n, k;
         tile_of<USE>(p, t, m, n, k);
         const int kend = first_k(k + 1);
@@ -682,66 +685,76 @@ __global__ void __launch_bounds__(kMmaThreads, 1) product_kernel(const __grid_co
               ok = false;
               break;
             }
-            mbar_arrive_expect_tx(&full[s], bytes);
+            const uint32_t bar = in_leader(&full[s]);
+            if (rank == 0) mbar_arrive_expect_tx(&full[s], bytes);
             unsigned char *sa = smem + s * (kBytesA + kBytesB), *sb = sa + kBytesA;
+            const int mrow = m * kPairM + rank * kM;
             if (!is_grad(USE)) {
-              tma_load_2d(sa, &p.a, p.pa[q] + kb * kK, p.a_y + m * kM, &full[s]);
-            } else if (p.a_mn) {   // d transposed: 64 rows of two strips
-              for (int g = 0; g < 2; g++)
-                tma_load_2d(sa + g * 8192, &p.a, 0, p.pa[q] + (2 * m + g) * p.strip + kb * kK, &full[s]);
-            } else {               // 128 rows of a strip
-              tma_load_2d(sa, &p.a, 0, p.pa[q] + kb * p.strip + m * kM, &full[s]);
-            }
-            if (p.b_mn) {
-              for (unsigned g = 0; g < groups_b; g++)
-                tma_load_2d(sb + g * 8192, &p.b, p.pb[q] + n * p.ntile + g * 64, p.b_y + kb * kK, &full[s]);
+              tma_load_2d(sa, &p.a, p.pa[q] + kb * kK, p.a_y + mrow, bar);
+              tma_load_2d(sb, &p.b, p.pb[q] + kb * kK, p.b_y + n * kN + rank * (kN / 2), bar);
             } else {
-              tma_load_2d(sb, &p.b, p.pb[q] + kb * kK, p.b_y + n * kN, &full[s]);
+              if (p.a_mn) {   // d transposed: 64 rows of two strips
+                for (int g = 0; g < 2; g++)
+                  tma_load_2d(sa + g * 8192, &p.a, 0, p.pa[q] + (mrow / 64 + g) * p.strip + kb * kK, bar);
+              } else {        // 128 rows of a strip
+                tma_load_2d(sa, &p.a, 0, p.pa[q] + kb * p.strip + mrow, bar);
+              }
+              for (int g = 0; g < groups_b; g++)
+                tma_load_2d(sb + g * 8192, &p.b, p.pb[q] + n * p.ntile + rank * half_n + g * 64, p.b_y + kb * kK, bar);
             }
           }
       }
       if (!ok) {   // copies in flight still write into this block's shared memory
         int none = 0;
-        for (int i = max(0, it - kStages); i < it; i++) mbar_wait(&full[i % kStages], (i / kStages) & 1, &none);
+        if (rank == 0)
+          for (int i = max(0, it - kStages); i < it; i++) mbar_wait(&full[i % kStages], (i / kStages) & 1, &none);
+        else   // they are counted in the other CTA: a millisecond is long enough for any copy
+          for (int i = 0; i < 1000; i++) __nanosleep(1000);
       }
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0) {
-      int it = 0, local = 0;
+    if (rank == 0 && elected()) {
+      int stage = 0, phase = 0, local = 0;
       bool ok = true;
-      const uint32_t idesc = mma_desc(p.bf16, p.a_mn, p.b_mn, kM, p.ntile);
+      const uint32_t idesc = mma_desc(p.bf16, p.a_mn, p.b_mn, kPairM, p.ntile);
       const uint32_t step_a = p.a_mn ? 2048 >> 4 : 32 >> 4, step_b = p.b_mn ? 2048 >> 4 : 32 >> 4;
-      for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+      const uint64_t da0 = smem_desc(smem_addr(smem), p.a_mn ? 8192 : 16, 1024);
+      const uint64_t db0 = smem_desc(smem_addr(smem) + kBytesA, p.b_mn ? 8192 : 16, 1024);
+      for (int t = pair; ok && t < tiles; t += npairs) {
         int m, n, k;
         tile_of<USE>(p, t, m, n, k);
         const int kend = first_k(k + 1);
         for (int k0 = first_k(k); ok && k0 < kend; k0 += p.segment, local++) {
           const int buf = local & 1, k1 = min(kend, k0 + p.segment);
-          if (!mbar_wait(&tempty[buf], (local / 2 + 1) & 1, gave_up)) {
+          if (!mbar_wait<true>(&tempty[buf], (local / 2 + 1) & 1, gave_up)) {
             ok = false;
             break;
           }
           tmem_after_sync();
+          const uint32_t d = tmem + buf * 256;
           bool add = false;
           for (int q = 0; ok && q < p.pairs; q++)
-            for (int kb = k0; kb < k1; kb++, it++) {
-              const int s = it % kStages;
-              if (!mbar_wait(&full[s], (it / kStages) & 1, gave_up)) {
+            for (int kb = k0; kb < k1; kb++) {
+              if (!mbar_wait(&full[stage], phase, gave_up)) {
                 ok = false;
                 break;
               }
               tmem_after_sync();
-              const uint32_t sa = smem_addr(smem + s * (kBytesA + kBytesB)), sb = sa + kBytesA;
-              const uint64_t da = smem_desc(sa, p.a_mn ? 8192 : 16, 1024), db = smem_desc(sb, p.b_mn ? 8192 : 16, 1024);
-              const int steps = kb == p.kblocks - 1 ? p.k16 : kK / 16;
+              const uint64_t da = da0 + stage * ((kBytesA + kBytesB) >> 4), db = db0 + stage * ((kBytesA + kBytesB) >> 4);
+              mma_f16(d, da, db, idesc, add);
+              if (is_grad(USE) || kb != p.kblocks - 1 || p.k16 == kK / 16) {
 #pragma unroll
-              for (int i = 0; i < kK / 16; i++)
-                if (i < steps) {
-                  mma_f16(tmem + buf * 256, da + i * step_a, db + i * step_b, idesc, add);
-                  add = true;
-                }
-              mma_commit(&empty[s]);
+                for (int i = 1; i < kK / 16; i++) mma_f16(d, da + i * step_a, db + i * step_b, idesc, true);
+              } else {
+                for (int i = 1; i < p.k16; i++) mma_f16(d, da + i * step_a, db + i * step_b, idesc, true);
+              }
+              add = true;
+              mma_commit(&empty[stage]);
+              if (++stage == kStages) {
+                stage = 0;
+                phase ^= 1;
+              }
             }
           if (ok) mma_commit(&tfull[buf]);
         }
@@ -757,6 +770,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) product_kernel(const __grid_co
     const int quarter = warp & 3, half = (warp - 4) / 4;
     const int row = quarter * 32 + lane;
     const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
+    const uint32_t tempty_at[2] = {in_leader(&tempty[0]), in_leader(&tempty[1])};
     float c = kLog2e;
     if (!is_grad(USE) && p.split_scale)
       c = kLog2e * pow2(-scale_exp(p.sc->h, kOperandTop)) * pow2(-scale_exp(p.sc->w, kOperandTop));
@@ -772,14 +786,14 @@ __global__ void __launch_bounds__(kMmaThreads, 1) product_kernel(const __grid_co
     auto end = [&](int buf) {
       tmem_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&tempty[buf]);
+      if (lane == 0) mbar_arrive_cluster(tempty_at[buf]);
       local++;
     };
     const int chunks = (p.ntile + 31) / 32;
-    for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
+    for (int t = pair; t < tiles; t += npairs) {
       int m, n, k;
       tile_of<USE>(p, t, m, n, k);
-      const int64_t r = (int64_t)m * kM + row;
+      const int64_t r = (int64_t)m * kPairM + rank * kM + row;
       auto fetch = [&](int ch, float (&x)[32]) {
         if (ok) {
           tmem_load32(lanes + (local & 1) * 256 + ch * 32, x);
@@ -902,8 +916,10 @@ __global__ void __launch_bounds__(kMmaThreads, 1) product_kernel(const __grid_co
       }
     }
   }
+  // neither CTA leaves while the other's products read its shared memory or its barriers are arrived on
   tmem_before_sync();
-  __syncthreads();
+  __syncwarp();
+  cluster_sync();
   tmem_after_sync();
   if (warp == 2) tmem_free(tmem, 512);
 }
@@ -952,13 +968,13 @@ struct Operand {
 template <Use USE>
 int launch_product(Product &p, const Operand &a, const Operand &b, cudaStream_t s) {
   int err = tensor_map(&p.a, a.p, a.inner, a.rows, a.ld, p.a_mn ? 64 : kM);
-  if (!err) err = tensor_map(&p.b, b.p, b.inner, b.rows, b.ld, p.b_mn ? 64 : kN);
+  if (!err) err = tensor_map(&p.b, b.p, b.inner, b.rows, b.ld, p.b_mn ? 64 : kN / 2);
   if (err) return err;
   // an attribute of the function on the current device, so it is set on every device that gets here
   const cudaError_t e = cudaFuncSetAttribute(product_kernel<USE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (e != cudaSuccess) return (int)e;
   const int tiles = p.mt * p.nt * p.splits;
-  product_kernel<USE><<<std::min(tiles, device_sm_count()), kMmaThreads, kSmem, s>>>(p);
+  product_kernel<USE><<<2 * std::max(1, std::min(tiles, device_sm_count() / 2)), kMmaThreads, kSmem, s>>>(p);
   count_launch(1);
   return (int)cudaGetLastError();
 }
@@ -969,7 +985,7 @@ struct Shape {
 };
 
 bool good_shape(const Shape &x) {
-  return x.n >= 0 && x.n < ((int64_t)1 << 31) - kM && x.vocab >= 1 && x.vocab < ((int64_t)1 << 31) - 512 && x.dim >= 1 &&
+  return x.n >= 0 && x.n < ((int64_t)1 << 31) - 1024 && x.vocab >= 1 && x.vocab < ((int64_t)1 << 31) - 512 && x.dim >= 1 &&
          x.dim <= kMaxDim && x.labels >= 1 && x.labels <= 1024 &&
          (x.type == W2V_F32 || x.type == W2V_BF16 || x.type == W2V_F16);
 }
@@ -999,12 +1015,12 @@ struct Layout {
 // Column tiles of a gradient: as few as hold dim, equally wide.
 void column_tiles(int dim, int *nt, int *ntile) {
   *nt = (dim + kN - 1) / kN;
-  *ntile = (int)up((dim + *nt - 1) / *nt, 16);
+  *ntile = (int)up((dim + *nt - 1) / *nt, 32);
 }
 // In how many parts K is cut, each with a slab of sums of its own: as many as fill the SMs' last round
 // best, where a slab costs about what 1 / 32 of a round does.
 int splits_for(int64_t tiles, int64_t kblocks, int most) {
-  const int sms = device_sm_count();
+  const int sms = device_sm_count() / 2;   // pairs of them
   int best = 1;
   double cost = 1e30;
   for (int s = 1; s <= most && s * 4 <= std::max<int64_t>(kblocks, 4); s++) {
@@ -1046,11 +1062,11 @@ Layout plan(const Shape &x, bool grad) {
     l.parts = take(2 * ((x.vocab + kN - 1) / kN) * std::min(x.n, kLossRows) * sizeof(Part));
   } else {
     const int bytes = x.type == W2V_F32 ? 4 : 2;
-    l.rows = up(std::min(x.n, kGradRows), kM);
+    l.rows = up(std::min(x.n, kGradRows), kPairM);
     l.words = std::min(up(x.vocab, kN), std::max<int64_t>(kN, kProbBytes / (l.rows * bytes) / kN * kN));
     column_tiles(x.dim, &l.nt, &l.ntile);
-    l.hsplits = splits_for(l.rows / kM * l.nt, l.words / kK, 32);
-    l.wsplits = splits_for(l.words / kM * l.nt, l.rows / kK, 8);
+    l.hsplits = splits_for(l.rows / kPairM * l.nt, l.words / kK, 32);
+    l.wsplits = splits_for(l.words / kPairM * l.nt, l.rows / kK, 8);
     l.coef = take(x.n * sizeof(RowCoef));
     l.probs = take(l.rows * l.words * bytes);
     if (x.type == W2V_F32) l.scratch = take((int64_t)device_sm_count() * kM * kN * 4);
@@ -1161,7 +1177,7 @@ int run_loss(const Shape &x, const Layout &l, const void *h, int64_t ldh, const 
   p.parts = parts;
   for (int64_t r0 = 0; r0 < x.n; r0 += kLossRows) {
     p.rows = (int)std::min(kLossRows, x.n - r0);
-    p.mt = (p.rows + kM - 1) / kM;
+    p.mt = (p.rows + kPairM - 1) / kPairM;
     p.a_y = (int)r0;
     p.ldparts = p.rows;
     err = launch_product<kLogits>(p, oh, ow, s);
@@ -1229,7 +1245,7 @@ int run_grad(const Shape &x, const Layout &l, const void *h, int64_t ldh, const 
     for (int64_t v0 = 0; v0 < x.vocab; v0 += l.words) {
       const int words = (int)std::min(l.words, x.vocab - v0);
       Product p = logits_product<T>(x, oh, ow, sc);
-      p.mt = (rows + kM - 1) / kM;
+      p.mt = (rows + kPairM - 1) / kPairM;
       p.nt = (words + kN - 1) / kN;
       p.a_y = (int)r0;
       p.b_y = p.word0 = (int)v0;
@@ -1247,7 +1263,7 @@ int run_grad(const Shape &x, const Layout &l, const void *h, int64_t ldh, const 
         Product q{};
         q.nt = l.nt;
         q.ntile = l.ntile;
-        q.mt = which == 0 ? p.mt : (words + kM - 1) / kM;
+        q.mt = which == 0 ? p.mt : (words + kPairM - 1) / kPairM;
         q.kblocks = which == 0 ? (words + kK - 1) / kK : (rows + kK - 1) / kK;
         // the last piece may be too short for all splits: it adds to some of the slabs, which the
         // first piece, never the shorter one, has filled

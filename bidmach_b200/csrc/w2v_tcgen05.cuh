@@ -10,20 +10,63 @@
 
 namespace w2v {
 
-__device__ __forceinline__ void mbar_arrive(u64 *bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
+// One lane of a converged warp.  Code behind it is known to run in one thread, which keeps what the
+// tensor and copy instructions take as uniform operands out of vector registers; `lane == 0` does not.
+__device__ __forceinline__ bool elected() {
+  uint32_t yes;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(yes));
+  return yes != 0;
+}
+
+// Two CTAs of a cluster work as a pair on one tile; the one of rank 0 issues their products.
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+// Address, in the cluster's window, of the same place in the shared memory of rank 0.
+__device__ __forceinline__ uint32_t in_leader(const void *p) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_addr(p)));
+  return a;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool mbar_try_cluster(u64 *bar, unsigned parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_addr(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
 }
 
 // Waits for the phase of `parity` to complete.  False when it did not within about two seconds or
 // when another role of the block has given up already (`gave_up`, in shared memory).
+// CLUSTER: what a thread of the other CTA did before it arrived has to be seen (an acquire of that
+// scope is a memory barrier, several hundred clocks: not for the waits of every block of K, where
+// the loads and products order themselves).
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool mbar_wait(u64 *bar, unsigned parity, volatile int *gave_up) {
-  if (mbar_try_wait(bar, parity)) return true;
+  auto tried = [&] { return CLUSTER ? mbar_try_cluster(bar, parity) : mbar_try_wait(bar, parity); };
+  if (tried()) return true;
   uint64_t begin, now;
   asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(begin));
   for (;;) {
 #pragma unroll 1
     for (int i = 0; i < 256; i++)
-      if (mbar_try_wait(bar, parity)) return true;
+      if (tried()) return true;
     if (*gave_up) return false;
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
     if (now - begin > 2000000000ull) {
@@ -33,11 +76,12 @@ __device__ __forceinline__ bool mbar_wait(u64 *bar, unsigned parity, volatile in
   }
 }
 
-__device__ __forceinline__ void tma_load_2d(void *dst, const CUtensorMap *map, int x, int y, u64 *bar) {
+// Into this CTA's shared memory; the bytes are counted on a barrier that may be the other CTA's.
+__device__ __forceinline__ void tma_load_2d(void *dst, const CUtensorMap *map, int x, int y, uint32_t bar) {
   asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
-          smem_addr(dst)),
-      "l"(map), "r"(x), "r"(y), "r"(smem_addr(bar))
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
+      "[%4];" ::"r"(smem_addr(dst)),
+      "l"(map), "r"(x), "r"(y), "r"(bar)
       : "memory");
 }
 
@@ -59,21 +103,25 @@ __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
       "setp.ne.u32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
       "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
       : "memory");
 }
+// Arrives on the barrier, in both CTAs, when the products issued so far are done.
 __device__ __forceinline__ void mma_commit(u64 *bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
-               : "memory");
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_addr(bar)),
+      "h"((uint16_t)3)
+      : "memory");
 }
 __device__ __forceinline__ void tmem_alloc(uint32_t *to, unsigned columns) {
-  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(to)), "r"(columns)
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(to)), "r"(columns)
                : "memory");
-  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
 }
 __device__ __forceinline__ void tmem_free(uint32_t addr, unsigned columns) {
-  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(columns));
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(columns));
 }
 __device__ __forceinline__ void tmem_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tmem_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
