@@ -53,7 +53,8 @@ __device__ __forceinline__ Part join(Part a, Part b) {
 
 // What the gradient needs of a row: d = exp2(l log2e - lse2) * coef - (targets here) * g.
 struct RowCoef {
-  float lse2, coef, g, pad;
+  float lse2, coef, g;
+  unsigned hits;   // chunks of 32 columns of the tile at hand that hold a target (only in shared memory)
 };
 
 // Found on the device before a product: largest magnitudes (as bits) of H, W and g_n k_n.
@@ -432,8 +433,16 @@ __global__ void __launch_bounds__(256) amax_kernel(Source h, Source w, int dim, 
     if (!s.p) return;
     const float *a = static_cast<const float *>(s.p);
     const int lane = threadIdx.x & 31;
+    const bool wide = reinterpret_cast<uintptr_t>(a) % 32 == 0 && s.ld % 8 == 0;
     for (int64_t r = (int64_t)blockIdx.x * 8 + threadIdx.x / 32; r < s.rows; r += (int64_t)gridDim.x * 8)
-      for (int c = lane; c < dim; c += 32) top = max(top, __float_as_uint(a[r * s.ld + c]) & 0x7fffffffu);
+      for (int c = lane * 8; c < dim; c += 256) {
+        const int have = min(8, dim - c);
+        float x[8];
+        if (wide && have == 8) load8(a + r * s.ld + c, x);
+        else load_some(a + r * s.ld + c, have, x);
+#pragma unroll
+        for (int e = 0; e < 8; e++) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+      }
     block_max(top, blockIdx.z == 0 ? &sc->h : &sc->w);
   } else if (gloss) {
     for (int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x; n < h.rows; n += (int64_t)gridDim.x * 256) {
@@ -501,7 +510,7 @@ __global__ void __launch_bounds__(256) row_coef_kernel(const float *lse, const f
   // lse log2e to twice the precision: what the rounded exponent lacks goes into the factor
   const float hi = lse[n] * kLog2e, lo = fmaf(lse[n], kLog2e, -hi);
   // a row without targets: exp2(l - inf) = 0, times 0
-  out[n] = k ? RowCoef{hi, g * (float)k * exp2f(-lo), g, 0.f} : RowCoef{INFINITY, 0.f, 0.f, 0.f};
+  out[n] = k ? RowCoef{hi, g * (float)k * exp2f(-lo), g, 0u} : RowCoef{INFINITY, 0.f, 0.f, 0u};
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -637,7 +646,8 @@ template <Use USE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) product_kernel(const __grid_constant__ Product p) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char *smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
-  __shared__ u64 full[kStages], empty[kStages], tfull[2], tempty[2], done;
+  __shared__ u64 full[kStages], empty[kStages], tfull[2], tempty[2], done, hfull[2], hempty[2];
+  __shared__ RowCoef coef_s[2][USE == kProbs ? kM : 1];
   __shared__ uint32_t tmem_at;
   __shared__ int gave_up_s;
   volatile int *gave_up = &gave_up_s;
@@ -650,6 +660,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) prod
     for (int i = 0; i < 2; i++) {
       mbar_init(&tfull[i], 1);
       mbar_init(&tempty[i], 16);   // the warps that read tiles, of both CTAs
+    }
+    for (int i = 0; i < 2; i++) {
+      mbar_init(&hfull[i], 2);
+      mbar_init(&hempty[i], 8);
     }
     mbar_init(&done, 1);
     gave_up_s = 0;
@@ -727,7 +741,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) prod
         const int kend = first_k(k + 1);
         for (int k0 = first_k(k); ok && k0 < kend; k0 += p.segment, local++) {
           const int buf = local & 1, k1 = min(kend, k0 + p.segment);
-          if (!mbar_wait<true>(&tempty[buf], (local / 2 + 1) & 1, gave_up)) {
+          if (!mbar_wait(&tempty[buf], (local / 2 + 1) & 1, gave_up)) {
             ok = false;
             break;
           }
@@ -766,6 +780,41 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) prod
       }
     }
     __syncwarp();
+  } else if (USE == kProbs && warp < 4) {
+    // one tile ahead of the warps that read it: what they need of each row, so that they never wait
+    // for global memory (ten targets a row cost as much as the tile itself)
+    bool ok = true;
+    int local = 0;
+    for (int t = pair; ok && t < tiles; t += npairs, local++) {
+      int m, n, k;
+      tile_of<USE>(p, t, m, n, k);
+      const int buf = local & 1;
+      ok = __all_sync(kFullMask, mbar_wait(&hempty[buf], (local / 2 + 1) & 1, gave_up));
+      const int64_t first = p.word0 + (int64_t)n * kN;
+      for (int i = (warp - 2) * 32 + lane; ok && i < kM; i += 64) {
+        const int64_t r = (int64_t)m * kPairM + rank * kM + i;
+        RowCoef rc{INFINITY, 0.f, 0.f, 0u};
+        if (r < p.rows) {
+          rc = p.coef[r];
+          const int *y = p.targets + r * p.labels;
+          for (int j = 0; j < p.labels; j += 8) {
+            int at[8];
+#pragma unroll
+            for (int q = 0; q < 8; q++) at[q] = j + q < p.labels ? y[j + q] : -1;
+#pragma unroll
+            for (int q = 0; q < 8; q++) {
+              const int64_t c = at[q] - first;
+              if (at[q] >= 0 && c >= 0 && c < kN) rc.hits |= 1u << (c >> 5);
+            }
+          }
+          if (rc.g == 0.f) rc.hits = 0;
+        }
+        coef_s[buf][i] = rc;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive_leader(smem_addr(&hfull[buf]));
+    }
+    __syncwarp();
   } else if (warp >= 4) {
     const int quarter = warp & 3, half = (warp - 4) / 4;
     const int row = quarter * 32 + lane;
@@ -786,7 +835,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) prod
     auto end = [&](int buf) {
       tmem_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(tempty_at[buf]);
+      if (lane == 0) mbar_arrive_leader(tempty_at[buf]);
       local++;
     };
     const int chunks = (p.ntile + 31) / 32;
@@ -837,17 +886,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) prod
         end(buf);
       } else if (USE == kProbs) {
         const int buf = local & 1;
-        RowCoef rc{INFINITY, 0.f, 0.f, 0.f};
-        if (r < p.rows) rc = p.coef[r];
+        ok = ok && mbar_wait(&hfull[buf], (local / 2) & 1, gave_up);
+        ok = __all_sync(kFullMask, ok);
+        const RowCoef rc = ok ? coef_s[buf][row] : RowCoef{INFINITY, 0.f, 0.f, 0u};
+        const unsigned hits = rc.hits;
         const int64_t left = p.vocab - p.word0 - (int64_t)n * kN;
         const int64_t first = p.word0 + (int64_t)n * kN;
-        unsigned hits = 0;   // chunks of the tile that hold a target of this row
         const int *y = p.targets + r * p.labels;
-        if (rc.g != 0.f)
-          for (int j = 0; j < p.labels; j++) {
-            const int64_t at = y[j] - first;
-            if (at >= 0 && at < kN) hits |= 1u << (at >> 5);
-          }
+        __syncwarp();
+        if (lane == 0) mbar_arrive_leader(smem_addr(&hempty[buf]));
         begin(buf);
         for (int ch = half; ch < chunks; ch += 2) {
           float x[32];
@@ -1017,17 +1064,19 @@ void column_tiles(int dim, int *nt, int *ntile) {
   *nt = (dim + kN - 1) / kN;
   *ntile = (int)up((dim + *nt - 1) / *nt, 32);
 }
-// In how many parts K is cut, each with a slab of sums of its own: as many as fill the SMs' last round
-// best, where a slab costs about what 1 / 32 of a round does.
-int splits_for(int64_t tiles, int64_t kblocks, int most) {
-  const int sms = device_sm_count() / 2;   // pairs of them
+// In how many parts K is cut, each with a slab of sums of its own, by an estimate in microseconds: the
+// rounds of tiles over the pairs of SMs, a block of K taking 512 clocks for 256 columns, against
+// writing the slabs and reading them again at about 5 TB/s.  With one part and `whole` there is no slab.
+int splits_for(int64_t tiles, int64_t kblocks, int pairs, int ntile, int64_t slab_bytes, bool whole) {
+  const int sms = std::max(1, device_sm_count() / 2);
   int best = 1;
   double cost = 1e30;
-  for (int s = 1; s <= most && s * 4 <= std::max<int64_t>(kblocks, 4); s++) {
-    const double rounds = (double)((tiles * s + sms - 1) / sms) / s;
-    const double c = rounds * (1 + 0.03 * (s > 1)) + 0.03 * (s - 1) * rounds;
-    if (c < cost) {
-      cost = c;
+  for (int s = 1; s <= 32 && (s == 1 || kblocks / s >= 4); s++) {
+    const double rounds = (double)((tiles * s + sms - 1) / sms);
+    const double product = rounds * ((double)kblocks / s * pairs * 512 * ntile / kN + 1500) / 1700;
+    const double slabs = s == 1 && whole ? 0 : 2.0 * s * slab_bytes / 5e6;
+    if (product + slabs < cost) {
+      cost = product + slabs;
       best = s;
     }
   }
@@ -1063,15 +1112,22 @@ Layout plan(const Shape &x, bool grad) {
   } else {
     const int bytes = x.type == W2V_F32 ? 4 : 2;
     l.rows = up(std::min(x.n, kGradRows), kPairM);
-    l.words = std::min(up(x.vocab, kN), std::max<int64_t>(kN, kProbBytes / (l.rows * bytes) / kN * kN));
+    // pieces of the vocabulary of equal width, up to a quarter more than kProbBytes
+    const int64_t most = std::max<int64_t>(kN, kProbBytes / (l.rows * bytes));
+    const int64_t pieces = std::max<int64_t>(1, (x.vocab + most * 5 / 4 - 1) / (most * 5 / 4));
+    l.words = up((x.vocab + pieces - 1) / pieces, kN);
     column_tiles(x.dim, &l.nt, &l.ntile);
-    l.hsplits = splits_for(l.rows / kPairM * l.nt, l.words / kK, 32);
-    l.wsplits = splits_for(l.words / kPairM * l.nt, l.rows / kK, 8);
+    const int pairs = x.type == W2V_F32 ? 3 : 1;
+    const int64_t cols = (int64_t)l.nt * l.ntile * 4;
+    l.hsplits = splits_for(l.rows / kPairM * l.nt, l.words / kK, pairs, l.ntile, l.rows * cols, l.words >= x.vocab && x.dim % 8 == 0);
+    l.wsplits = splits_for(l.words / kPairM * l.nt, l.rows / kK, pairs, l.ntile, l.words * cols,
+                           l.rows >= x.n && x.dim % 8 == 0);
     l.coef = take(x.n * sizeof(RowCoef));
     l.probs = take(l.rows * l.words * bytes);
     if (x.type == W2V_F32) l.scratch = take((int64_t)device_sm_count() * kM * kN * 4);
-    l.direct_h = l.hsplits == 1 && l.words >= x.vocab;
-    l.direct_w = l.wsplits == 1 && l.rows >= x.n;
+    // rows that are not a multiple of eight elements are better written by a warp each than by a thread each
+    l.direct_h = l.hsplits == 1 && l.words >= x.vocab && x.dim % 8 == 0;
+    l.direct_w = l.wsplits == 1 && l.rows >= x.n && x.dim % 8 == 0;
     if (!l.direct_h) l.acc_h = take((int64_t)l.hsplits * l.rows * l.nt * l.ntile * 4);
     if (!l.direct_w) l.acc_w = take((int64_t)l.wsplits * up(x.vocab, kM) * l.nt * l.ntile * 4);
   }

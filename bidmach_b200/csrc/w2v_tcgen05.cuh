@@ -37,36 +37,22 @@ __device__ __forceinline__ uint32_t in_leader(const void *p) {
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ bool mbar_try_cluster(u64 *bar, unsigned parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_addr(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
+// Arrives on a barrier of the other CTA.  What it tells is that tensor memory has been read, which the
+// tcgen05 fences order; a release at cluster scope would wait for the thread's stores to memory too.
+__device__ __forceinline__ void mbar_arrive_leader(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 // Waits for the phase of `parity` to complete.  False when it did not within about two seconds or
 // when another role of the block has given up already (`gave_up`, in shared memory).
-// CLUSTER: what a thread of the other CTA did before it arrived has to be seen (an acquire of that
-// scope is a memory barrier, several hundred clocks: not for the waits of every block of K, where
-// the loads and products order themselves).
-template <bool CLUSTER = false>
 __device__ __forceinline__ bool mbar_wait(u64 *bar, unsigned parity, volatile int *gave_up) {
-  auto tried = [&] { return CLUSTER ? mbar_try_cluster(bar, parity) : mbar_try_wait(bar, parity); };
-  if (tried()) return true;
+  if (mbar_try_wait(bar, parity)) return true;
   uint64_t begin, now;
   asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(begin));
   for (;;) {
 #pragma unroll 1
     for (int i = 0; i < 256; i++)
-      if (tried()) return true;
+      if (mbar_try_wait(bar, parity)) return true;
     if (*gave_up) return false;
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
     if (now - begin > 2000000000ull) {
