@@ -277,56 +277,46 @@ __global__ void __launch_bounds__(kFewThreads) few_dh_kernel(const T *w, int64_t
   }
 }
 
+// Power of two that d is stored with, so that fp16 holds it: `given`, where one factor for all rows is
+// left to the end and d is at most the number of targets, else from the largest |g_n k_n|.
+constexpr int kFromRows = 1 << 20;
+__device__ __forceinline__ int prob_exp(const Scalars *sc, int given) {
+  return given == kFromRows ? scale_exp(sc->g, kProbTop) : given;
+}
+
 // What a gradient's sums have to be multiplied with: the powers of two that d and the other operand
 // were scaled by, and the one factor for all rows where there is one.
 struct Rescale {
-  const Scalars *sc;   // null: 1
+  const Scalars *sc;
   const float *gloss;  // null: 1
-  int operand;         // 0: none scaled, 1: W, 2: H
+  int given;           // of prob_exp
+  int operand;         // 0: not scaled, 1: W, 2: H
 };
 __device__ __forceinline__ float rescale_of(const Rescale &r) {
-  float x = r.gloss ? *r.gloss : 1.f;
-  if (r.sc) {
-    x *= pow2(-scale_exp(r.sc->g, kProbTop));
-    if (r.operand) x *= pow2(-scale_exp(r.operand == 1 ? r.sc->w : r.sc->h, kOperandTop));
-  }
-  return x;
+  const float x = (r.gloss ? *r.gloss : 1.f) * pow2(-prob_exp(r.sc, r.given));
+  return r.operand ? x * pow2(-scale_exp(r.operand == 1 ? r.sc->w : r.sc->h, kOperandTop)) : x;
 }
 
-// out[r][c] = factor * sum over slabs, in their order; a warp a row.
+// out[r][c] = sum over slabs, in their order; a warp a row.
 template <typename T>
-__global__ void __launch_bounds__(256) slabs_kernel(const float *slabs, int count, int64_t slab, int64_t lds, int64_t rows,
-                                                    int dim, T *out, int64_t ldo, bool wide, const Rescale rescale) {
-  const float f = rescale_of(rescale);
+__global__ void __launch_bounds__(256) slabs_kernel(const float *slabs, int count, int64_t slab, int64_t rows, int dim,
+                                                    T *out, int64_t ldo) {
   const int lane = threadIdx.x & 31;
-  const int cols = (dim + 255) / 256;
-  const int64_t stride = (int64_t)gridDim.x * 8;
-  for (int64_t i = (int64_t)blockIdx.x * 8 + threadIdx.x / 32; i < rows * cols; i += stride) {
-    const int64_t r = cols == 1 ? i : i / cols;
-    const int c = (int)(i - r * cols) * 256 + lane * 8, have = min(8, dim - c);
-    if (have <= 0) continue;
-    const float *p = slabs + r * lds + c;
-    float x[8];
-    if (wide) load8(p, x);
-    else load_some(p, have, x);
-    for (int k = 1; k < count; k += 4) {
-      float y[4][8];
+  const int64_t cols = (dim + 31) / 32, i = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
+  if (i >= rows * cols) return;
+  const int64_t r = i / cols;
+  const int c = (int)(i % cols) * 32 + lane;
+  if (c >= dim) return;
+  const float *p = slabs + r * dim + c;
+  float x = 0.f;
+  for (int k = 0; k < count; k += 8) {
+    float y[8];
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        if (wide && k + j < count) load8(p + (k + j) * slab, y[j]);
-        else load_some(p + (k + j) * slab, k + j < count ? have : 0, y[j]);
-      }
+    for (int j = 0; j < 8; j++) y[j] = k + j < count ? p[(k + j) * slab] : 0.f;
 #pragma unroll
-      for (int j = 0; j < 4; j++)
-#pragma unroll
-        for (int e = 0; e < 8; e++) x[e] += y[j][e];
-    }
-#pragma unroll
-    for (int e = 0; e < 8; e++) x[e] *= f;
-    T *to = out + r * ldo + c;
-    if (have == 8 && reinterpret_cast<uintptr_t>(to) % (8 * sizeof(T)) == 0) store8(to, x);
-    else store_some(to, have, x);
+    for (int j = 0; j < 8; j++) x += y[j];
   }
+  out[r * ldo + c] = from_float<T>(x);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -425,7 +415,7 @@ __device__ __forceinline__ void block_max(unsigned top, unsigned *to) {
 }
 
 // Largest magnitudes of fp32 operands (z = 0: H, 1: W) and of the rows' g_n k_n (z = 2).
-__global__ void __launch_bounds__(256) amax_kernel(Source h, Source w, int dim, const float *gloss, int64_t ldg,
+__global__ void __launch_bounds__(256) amax_kernel(Source h, Source w, int dim, const float *gloss,
                                                    const int *targets, int labels, int64_t vocab, Scalars *sc) {
   unsigned top = 0;
   if (blockIdx.z < 2) {
@@ -447,7 +437,7 @@ __global__ void __launch_bounds__(256) amax_kernel(Source h, Source w, int dim, 
   } else if (gloss) {
     for (int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x; n < h.rows; n += (int64_t)gridDim.x * 256) {
       const int k = valid_targets(targets + n * labels, labels, vocab);
-      if (k) top = max(top, __float_as_uint((ldg ? gloss[n] : 1.f) * (float)k) & 0x7fffffffu);
+      if (k) top = max(top, __float_as_uint(gloss[n] * (float)k) & 0x7fffffffu);
     }
     block_max(top, &sc->g);
   }
@@ -499,65 +489,197 @@ __global__ void __launch_bounds__(256) stage_kernel(Source h, Source w, int dim,
   }
 }
 
-__global__ void __launch_bounds__(256) row_coef_kernel(const float *lse, const float *gloss, int64_t ldg,
-                                                       const int *targets, int labels, int64_t vocab, int64_t rows,
-                                                       const Scalars *sc, RowCoef *out) {
-  const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (n >= rows) return;
-  // one factor for all rows is left to the end: the targets' -1 then has no rounding in d
-  const float g = (ldg ? gloss[n] : 1.f) * pow2(scale_exp(sc->g, kProbTop));
-  const int k = valid_targets(targets + n * labels, labels, vocab);
-  // lse log2e to twice the precision: what the rounded exponent lacks goes into the factor
-  const float hi = lse[n] * kLog2e, lo = fmaf(lse[n], kLog2e, -hi);
-  // a row without targets: exp2(l - inf) = 0, times 0
-  out[n] = k ? RowCoef{hi, g * (float)k * exp2f(-lo), g, 0u} : RowCoef{INFINITY, 0.f, 0.f, 0u};
-}
-
 // ---------------------------------------------------------------------------------------------
-// The product
+// The products
 // ---------------------------------------------------------------------------------------------
 constexpr int kM = 128, kN = 256, kK = 64, kStages = 6;   // rows of each of a pair's CTAs, columns of both
 constexpr int kPairM = 2 * kM;
-constexpr int kBytesA = kM * kK * 2, kBytesB = kN / 2 * kK * 2;
-constexpr int kMmaThreads = 384;   // producer, issuer, two idle warps, eight that read the tiles
-constexpr int kSmem = kStages * (kBytesA + kBytesB) + 1024;
+constexpr int kBytesA = kM * kK * 2, kBytesB = kN / 2 * kK * 2, kBytesStage = kBytesA + kBytesB;
+constexpr int kMmaThreads = 384;   // producer, issuer, two helpers, eight that read the tiles
+constexpr int kSmem = kStages * kBytesStage + 1024;
 
-enum Use { kLogits, kProbs, kGrad, kGradSegments };
-__host__ __device__ constexpr bool is_grad(Use u) { return u == kGrad || u == kGradSegments; }
+// What the roles of a CTA share.
+struct Pipe {
+  u64 full[kStages], empty[kStages];   // operands: in the leader, counting both CTAs' bytes; read by the products
+  u64 tfull[2], tempty[2];             // halves of tensor memory: finished; read (in the leader, by both CTAs)
+  u64 hfull[2], hempty[2];             // rows' coefficients: there; read
+  u64 done;
+  uint32_t tmem;
+  int gave_up;
+};
+
+// Returns the address of the pair's tensor memory.
+__device__ __forceinline__ uint32_t pair_begin(Pipe &s) {
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; i++) {
+      mbar_init(&s.full[i], 1);
+      mbar_init(&s.empty[i], 1);
+    }
+    for (int i = 0; i < 2; i++) {
+      mbar_init(&s.tfull[i], 1);
+      mbar_init(&s.tempty[i], 16);
+      mbar_init(&s.hfull[i], 2);
+      mbar_init(&s.hempty[i], 8);
+    }
+    mbar_init(&s.done, 1);
+    s.gave_up = 0;
+    mbar_init_fence();
+    async_proxy_fence();
+  }
+  if (threadIdx.x / 32 == 2) tmem_alloc(&s.tmem, 512);
+  tmem_before_sync();
+  cluster_sync();
+  tmem_after_sync();
+  return s.tmem;
+}
+// Neither CTA leaves while the other's products read its shared memory or its barriers are arrived on.
+__device__ __forceinline__ void pair_end(uint32_t tmem) {
+  tmem_before_sync();
+  __syncwarp();
+  cluster_sync();
+  tmem_after_sync();
+  if (threadIdx.x / 32 == 2) tmem_free(tmem, 512);
+}
+
+// The producer's place in the ring of stages.
+struct Ring {
+  Pipe &s;
+  unsigned char *smem;
+  volatile int *gave_up;
+  int it = 0;
+
+  // The next stage's operands and the leader's barrier for them; false when the wait ran out.
+  __device__ __forceinline__ bool next(unsigned bytes, unsigned char *&a, unsigned char *&b, uint32_t &bar) {
+    const int i = it % kStages;
+    if (!mbar_wait(&s.empty[i], (it / kStages + 1) & 1, gave_up)) return false;
+    it++;
+    bar = in_leader(&s.full[i]);
+    if (cluster_rank() == 0) mbar_arrive_expect_tx(&s.full[i], bytes);
+    a = smem + i * kBytesStage;
+    b = a + kBytesA;
+    return true;
+  }
+  // Copies in flight still write into this CTA's shared memory.
+  __device__ __forceinline__ void settle() {
+    int none = 0;
+    if (cluster_rank() == 0)
+      for (int i = max(0, it - kStages); i < it; i++) mbar_wait(&s.full[i % kStages], (i / kStages) & 1, &none);
+    else   // they are counted in the other CTA: a millisecond is long enough for any copy
+      for (int i = 0; i < 1000; i++) __nanosleep(1000);
+  }
+};
+
+// The issuing thread's place: products of the stages in their order.
+struct Issue {
+  Pipe &s;
+  volatile int *gave_up;
+  uint32_t tmem;
+  uint32_t smem;
+  int stage = 0, phase = 0, local = 0;
+
+  // A half of tensor memory to accumulate in; false when the wait ran out.
+  __device__ __forceinline__ bool begin(uint32_t &d) {
+    const int buf = local & 1;
+    if (!mbar_wait(&s.tempty[buf], (local / 2 + 1) & 1, gave_up)) return false;
+    tmem_after_sync();
+    d = tmem + buf * 256;
+    return true;
+  }
+  __device__ __forceinline__ void end() { mma_commit(&s.tfull[local++ & 1]); }
+  // Descriptors of a stage whose rows run along K (`mn`) or across it.
+  __device__ __forceinline__ uint64_t desc(int offset, bool mn) const { return smem_desc(smem + offset, mn ? 8192 : 16, 1024); }
+  // One block of K: `steps` products of 16.
+  template <bool WHOLE>
+  __device__ __forceinline__ bool block(uint32_t d, uint64_t da0, uint64_t db0, uint32_t step_a, uint32_t step_b,
+                                        uint32_t idesc, bool add, int steps) {
+    if (!mbar_wait(&s.full[stage], phase, gave_up)) return false;
+    tmem_after_sync();
+    const uint64_t da = da0 + stage * (kBytesStage >> 4), db = db0 + stage * (kBytesStage >> 4);
+    mma_f16(d, da, db, idesc, add);
+    if (WHOLE || steps == kK / 16) {
+#pragma unroll
+      for (int i = 1; i < kK / 16; i++) mma_f16(d, da + i * step_a, db + i * step_b, idesc, true);
+    } else {
+      for (int i = 1; i < steps; i++) mma_f16(d, da + i * step_a, db + i * step_b, idesc, true);
+    }
+    mma_commit(&s.empty[stage]);
+    if (++stage == kStages) {
+      stage = 0;
+      phase ^= 1;
+    }
+    return true;
+  }
+  // Products in flight still read shared memory.
+  __device__ __forceinline__ void settle() {
+    int none = 0;
+    mma_commit(&s.done);
+    mbar_wait(&s.done, 0, &none);
+  }
+};
+
+// A reading warp's place: 32 rows of the halves of tensor memory, one after the other.
+struct Reader {
+  Pipe &s;
+  volatile int *gave_up;
+  uint32_t lanes, release[2];
+  int local = 0;
+  bool ok = true;
+
+  __device__ __forceinline__ Reader(Pipe &pipe, volatile int *g, uint32_t tmem) : s(pipe), gave_up(g) {
+    lanes = tmem + ((uint32_t)(threadIdx.x / 32 % 4 * 32) << 16);
+    release[0] = in_leader(&s.tempty[0]);
+    release[1] = in_leader(&s.tempty[1]);
+  }
+  __device__ __forceinline__ bool wait(u64 *bars) {
+    ok = ok && mbar_wait(&bars[local & 1], (local / 2) & 1, gave_up);
+    ok = __all_sync(kFullMask, ok);
+    return ok;
+  }
+  __device__ __forceinline__ void begin() {
+    wait(s.tfull);
+    tmem_after_sync();
+  }
+  // A warp that gave up reads NaN: nothing that was not computed passes for a result.
+  __device__ __forceinline__ void fetch(int col, float (&x)[32]) const {
+    if (ok) {
+      tmem_load32(lanes + (local & 1) * 256 + col, x);
+      tmem_wait_load();
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; i++) x[i] = __int_as_float(0x7fffffff);
+    }
+  }
+  __device__ __forceinline__ void end() {
+    tmem_before_sync();
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive_leader(release[local & 1]);
+    local++;
+  }
+};
+
+// ---- logits, and d ---------------------------------------------------------------------------
+enum Use { kLogits, kProbs };
 
 struct Product {
-  CUtensorMap a, b;
-  int mt, nt, ntile;      // tiles of kPairM rows, columns a tile (a multiple of 32)
-  int splits, kblocks;    // of 64, over all splits, for one pair of parts
-  int pairs, pa[3], pb[3];// offsets of the parts that are multiplied, the smaller products first
-  int k16;                // steps of 16 in the last block of K
-  int a_mn, b_mn;         // operands whose rows run along K
-  int a_y, b_y;           // first row of each in its matrix
+  CUtensorMap a, b;         // H and W
+  int mt, nt;               // tiles
+  int kblocks, k16;         // of 64 for one pair of parts; steps of 16 in the last one
+  int pairs, pa[3], pb[3];  // offsets of the parts that are multiplied, the smaller products first
+  int a_y, b_y;             // first row of each
   int bf16;
-  // logits and probabilities
   const Scalars *sc;
-  int split_scale;        // operands carry the scales of sc
+  int split_scale;          // operands carry the scales of sc
   int64_t vocab;
-  int word0;              // word of the first column
-  int rows;               // rows that exist
+  int rows;                 // rows that exist
   Part *parts;
   int64_t ldparts;
-  const RowCoef *coef;
+  const float *lse, *gloss;   // gloss: null where one factor is left to the end
+  int given;                  // of prob_exp
   const int *targets;
   int labels;
-  uint16_t *probs;        // d in strips of 64 columns: [part][strip][row][64]
-  int strip;              // rows of a strip
-  int64_t prob_lo;        // offset of the second part, 0 for none
-  // gradients
-  int segment;            // blocks of K that are accumulated in tensor memory at a time
-  float *scratch;         // kM x kN for each block
-  float *acc;             // [splits][acc_rows][ldacc]
-  int64_t acc_slab, ldacc;
-  int add;                // to what is there already
-  void *out;              // not null: the finished gradient goes here, not to acc
-  int64_t ldout;
-  int out_type, out_wide, dim;
-  Rescale rescale;
+  uint16_t *probs;          // d in strips of 64 columns: [part][strip][row][64]
+  int strip;                // rows of a strip
+  int64_t prob_lo;          // offset of the second part, 0 for none
 };
 
 __device__ __forceinline__ void store32(void *a, const uint32_t (&r)[8]) {
@@ -597,269 +719,115 @@ __device__ __forceinline__ void store_probs(uint16_t *to, int64_t lo, const floa
 }
 
 template <Use USE>
-__device__ __forceinline__ void tile_of(const Product &p, int t, int &m, int &n, int &k) {
-  if (is_grad(USE)) {   // blocks that run together share a strip of d
-    n = t % p.nt;
-    m = t / p.nt % p.mt;
-    k = t / (p.nt * p.mt);
-  } else {              // ... and a few tiles of W, against all rows
-    m = t % p.mt;
-    n = t / p.mt;
-    k = 0;
-  }
-}
-
-template <typename T>
-__device__ __forceinline__ void put_typed(T *to, bool wide, int have, const float (&v)[8]) {
-  if (wide && have == 8) store8(to, v);
-  else store_some(to, have, v);
-}
-
-// Eight columns of a gradient's tile, from column `col` of it.
-__device__ __forceinline__ void put_grad(const Product &p, int64_t r, int n, int k, int col, const float *x, float factor) {
-  const int at = n * p.ntile + col;
-  if (r >= p.rows || col >= p.ntile || at >= p.dim) return;
-  float v[8];
-#pragma unroll
-  for (int e = 0; e < 8; e++) v[e] = x[e];
-  if (p.out) {
-    const int have = min(8, p.dim - at);
-#pragma unroll
-    for (int e = 0; e < 8; e++) v[e] *= factor;
-    const int64_t to = r * p.ldout + at;
-    if (p.out_type == W2V_F32) put_typed(static_cast<float *>(p.out) + to, p.out_wide, have, v);
-    else if (p.out_type == W2V_BF16) put_typed(static_cast<__nv_bfloat16 *>(p.out) + to, p.out_wide, have, v);
-    else put_typed(static_cast<__half *>(p.out) + to, p.out_wide, have, v);
-    return;
-  }
-  float *to = p.acc + k * p.acc_slab + r * p.ldacc + at;
-  if (p.add) {
-    float old[8];
-    load8(to, old);
-#pragma unroll
-    for (int e = 0; e < 8; e++) v[e] += old[e];
-  }
-  store8(to, v);
-}
-
-template <Use USE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) product_kernel(const __grid_constant__ Product p) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char *smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
-  __shared__ u64 full[kStages], empty[kStages], tfull[2], tempty[2], done, hfull[2], hempty[2];
+  __shared__ Pipe pipe;
   __shared__ RowCoef coef_s[2][USE == kProbs ? kM : 1];
-  __shared__ uint32_t tmem_at;
-  __shared__ int gave_up_s;
-  volatile int *gave_up = &gave_up_s;
+  volatile int *gave_up = &pipe.gave_up;
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < kStages; i++) {
-      mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 1);
-    }
-    for (int i = 0; i < 2; i++) {
-      mbar_init(&tfull[i], 1);
-      mbar_init(&tempty[i], 16);   // the warps that read tiles, of both CTAs
-    }
-    for (int i = 0; i < 2; i++) {
-      mbar_init(&hfull[i], 2);
-      mbar_init(&hempty[i], 8);
-    }
-    mbar_init(&done, 1);
-    gave_up_s = 0;
-    mbar_init_fence();
-    async_proxy_fence();
-  }
-  if (warp == 2) tmem_alloc(&tmem_at, 512);
-  tmem_before_sync();
-  cluster_sync();
-  tmem_after_sync();
-  const uint32_t tmem = tmem_at;
+  const uint32_t tmem = pair_begin(pipe);
   const int rank = (int)cluster_rank(), pair = blockIdx.x / 2, npairs = gridDim.x / 2;
-  const int tiles = p.mt * p.nt * p.splits;
-  // blocks of K that a split starts with: every split has one at least (splits <= kblocks)
-  auto first_k = [&](int k) { return (int)((int64_t)k * p.kblocks / p.splits); };
+  const int tiles = p.mt * p.nt;
+  // pairs that run together share a few tiles of W, against all rows
+  auto first_row = [&](int t) { return t % p.mt * kPairM + rank * kM; };
+  auto column_tile = [&](int t) { return t / p.mt; };
 
   if (warp == 0) {
     if (elected()) {
-      int it = 0;
+      Ring ring{pipe, smem, gave_up};
       bool ok = true;
-      // each CTA brings its own rows of A and half of the columns of B; the leader counts both
-      const int half_n = p.ntile / 2, groups_b = (half_n + 63) / 64;
-      const unsigned bytes = 2 * (kBytesA + (is_grad(USE) ? groups_b * 8192 : kBytesB));
       for (int t = pair; ok && t < tiles; t += npairs) {
-        int m, n, k;
-        tile_of<USE>(p, t, m, n, k);
-        const int kend = first_k(k + 1);
-        for (int k0 = first_k(k); ok && k0 < kend; k0 += p.segment)
+        const int row = p.a_y + first_row(t), col = p.b_y + column_tile(t) * kN + rank * (kN / 2);
         for (int q = 0; ok && q < p.pairs; q++)
-          for (int kb = k0; kb < min(kend, k0 + p.segment); kb++, it++) {
-            const int s = it % kStages;
-            if (!mbar_wait(&empty[s], (it / kStages + 1) & 1, gave_up)) {
-              ok = false;
-              break;
-            }
-            const uint32_t bar = in_leader(&full[s]);
-            if (rank == 0) mbar_arrive_expect_tx(&full[s], bytes);
-            unsigned char *sa = smem + s * (kBytesA + kBytesB), *sb = sa + kBytesA;
-            const int mrow = m * kPairM + rank * kM;
-            if (!is_grad(USE)) {
-              tma_load_2d(sa, &p.a, p.pa[q] + kb * kK, p.a_y + mrow, bar);
-              tma_load_2d(sb, &p.b, p.pb[q] + kb * kK, p.b_y + n * kN + rank * (kN / 2), bar);
-            } else {
-              if (p.a_mn) {   // d transposed: 64 rows of two strips
-                for (int g = 0; g < 2; g++)
-                  tma_load_2d(sa + g * 8192, &p.a, 0, p.pa[q] + (mrow / 64 + g) * p.strip + kb * kK, bar);
-              } else {        // 128 rows of a strip
-                tma_load_2d(sa, &p.a, 0, p.pa[q] + kb * p.strip + mrow, bar);
-              }
-              for (int g = 0; g < groups_b; g++)
-                tma_load_2d(sb + g * 8192, &p.b, p.pb[q] + n * p.ntile + rank * half_n + g * 64, p.b_y + kb * kK, bar);
-            }
+          for (int kb = 0; kb < p.kblocks; kb++) {
+            unsigned char *a, *b;
+            uint32_t bar;
+            if (!(ok = ring.next(2 * kBytesStage, a, b, bar))) break;
+            tma_load_2d(a, &p.a, p.pa[q] + kb * kK, row, bar);
+            tma_load_2d(b, &p.b, p.pb[q] + kb * kK, col, bar);
           }
       }
-      if (!ok) {   // copies in flight still write into this block's shared memory
-        int none = 0;
-        if (rank == 0)
-          for (int i = max(0, it - kStages); i < it; i++) mbar_wait(&full[i % kStages], (i / kStages) & 1, &none);
-        else   // they are counted in the other CTA: a millisecond is long enough for any copy
-          for (int i = 0; i < 1000; i++) __nanosleep(1000);
-      }
+      if (!ok) ring.settle();
     }
     __syncwarp();
   } else if (warp == 1) {
     if (rank == 0 && elected()) {
-      int stage = 0, phase = 0, local = 0;
+      Issue issue{pipe, gave_up, tmem, smem_addr(smem)};
       bool ok = true;
-      const uint32_t idesc = mma_desc(p.bf16, p.a_mn, p.b_mn, kPairM, p.ntile);
-      const uint32_t step_a = p.a_mn ? 2048 >> 4 : 32 >> 4, step_b = p.b_mn ? 2048 >> 4 : 32 >> 4;
-      const uint64_t da0 = smem_desc(smem_addr(smem), p.a_mn ? 8192 : 16, 1024);
-      const uint64_t db0 = smem_desc(smem_addr(smem) + kBytesA, p.b_mn ? 8192 : 16, 1024);
+      const uint32_t idesc = mma_desc(p.bf16, false, false, kPairM, kN);
+      const uint64_t da = issue.desc(0, false), db = issue.desc(kBytesA, false);
       for (int t = pair; ok && t < tiles; t += npairs) {
-        int m, n, k;
-        tile_of<USE>(p, t, m, n, k);
-        const int kend = first_k(k + 1);
-        for (int k0 = first_k(k); ok && k0 < kend; k0 += p.segment, local++) {
-          const int buf = local & 1, k1 = min(kend, k0 + p.segment);
-          if (!mbar_wait(&tempty[buf], (local / 2 + 1) & 1, gave_up)) {
-            ok = false;
-            break;
+        uint32_t d;
+        if (!(ok = issue.begin(d))) break;
+        bool add = false;
+        for (int q = 0; ok && q < p.pairs; q++)
+          for (int kb = 0; ok && kb < p.kblocks; kb++) {
+            ok = issue.block<false>(d, da, db, 2, 2, idesc, add, kb == p.kblocks - 1 ? p.k16 : kK / 16);
+            add = true;
           }
-          tmem_after_sync();
-          const uint32_t d = tmem + buf * 256;
-          bool add = false;
-          for (int q = 0; ok && q < p.pairs; q++)
-            for (int kb = k0; kb < k1; kb++) {
-              if (!mbar_wait(&full[stage], phase, gave_up)) {
-                ok = false;
-                break;
-              }
-              tmem_after_sync();
-              const uint64_t da = da0 + stage * ((kBytesA + kBytesB) >> 4), db = db0 + stage * ((kBytesA + kBytesB) >> 4);
-              mma_f16(d, da, db, idesc, add);
-              if (is_grad(USE) || kb != p.kblocks - 1 || p.k16 == kK / 16) {
-#pragma unroll
-                for (int i = 1; i < kK / 16; i++) mma_f16(d, da + i * step_a, db + i * step_b, idesc, true);
-              } else {
-                for (int i = 1; i < p.k16; i++) mma_f16(d, da + i * step_a, db + i * step_b, idesc, true);
-              }
-              add = true;
-              mma_commit(&empty[stage]);
-              if (++stage == kStages) {
-                stage = 0;
-                phase ^= 1;
-              }
-            }
-          if (ok) mma_commit(&tfull[buf]);
-        }
+        if (ok) issue.end();
       }
-      if (!ok) {   // products in flight still read shared memory
-        int none = 0;
-        mma_commit(&done);
-        mbar_wait(&done, 0, &none);
-      }
+      if (!ok) issue.settle();
     }
     __syncwarp();
   } else if (USE == kProbs && warp < 4) {
     // one tile ahead of the warps that read it: what they need of each row, so that they never wait
     // for global memory (ten targets a row cost as much as the tile itself)
+    const float scale = pow2(prob_exp(p.sc, p.given));
     bool ok = true;
     int local = 0;
     for (int t = pair; ok && t < tiles; t += npairs, local++) {
-      int m, n, k;
-      tile_of<USE>(p, t, m, n, k);
       const int buf = local & 1;
-      ok = __all_sync(kFullMask, mbar_wait(&hempty[buf], (local / 2 + 1) & 1, gave_up));
-      const int64_t first = p.word0 + (int64_t)n * kN;
+      ok = __all_sync(kFullMask, mbar_wait(&pipe.hempty[buf], (local / 2 + 1) & 1, gave_up));
+      const int64_t first = p.b_y + (int64_t)column_tile(t) * kN;
       for (int i = (warp - 2) * 32 + lane; ok && i < kM; i += 64) {
-        const int64_t r = (int64_t)m * kPairM + rank * kM + i;
-        RowCoef rc{INFINITY, 0.f, 0.f, 0u};
+        const int64_t r = first_row(t) + i;
+        RowCoef rc{INFINITY, 0.f, 0.f, 0u};   // a row without targets: exp2(l - inf) = 0, times 0
         if (r < p.rows) {
-          rc = p.coef[r];
+          const float lse = p.lse[r], g = (p.gloss ? p.gloss[r] : 1.f) * scale;
           const int *y = p.targets + r * p.labels;
+          int k = 0;
           for (int j = 0; j < p.labels; j += 8) {
             int at[8];
 #pragma unroll
             for (int q = 0; q < 8; q++) at[q] = j + q < p.labels ? y[j + q] : -1;
 #pragma unroll
             for (int q = 0; q < 8; q++) {
+              if (at[q] < 0 || at[q] >= p.vocab) continue;
               const int64_t c = at[q] - first;
-              if (at[q] >= 0 && c >= 0 && c < kN) rc.hits |= 1u << (c >> 5);
+              k++;
+              if (c >= 0 && c < kN) rc.hits |= 1u << (c >> 5);
             }
           }
-          if (rc.g == 0.f) rc.hits = 0;
+          if (k) {
+            // lse log2e to twice the precision: what the rounded exponent lacks goes into the factor
+            rc.lse2 = lse * kLog2e;
+            rc.coef = g * (float)k * exp2f(-fmaf(lse, kLog2e, -rc.lse2));
+            rc.g = g;
+          }
         }
         coef_s[buf][i] = rc;
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive_leader(smem_addr(&hfull[buf]));
+      if (lane == 0) mbar_arrive_leader(smem_addr(&pipe.hfull[buf]));
     }
     __syncwarp();
   } else if (warp >= 4) {
-    const int quarter = warp & 3, half = (warp - 4) / 4;
-    const int row = quarter * 32 + lane;
-    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
-    const uint32_t tempty_at[2] = {in_leader(&tempty[0]), in_leader(&tempty[1])};
+    const int half = (warp - 4) / 4, row = (warp & 3) * 32 + lane;
     float c = kLog2e;
-    if (!is_grad(USE) && p.split_scale)
-      c = kLog2e * pow2(-scale_exp(p.sc->h, kOperandTop)) * pow2(-scale_exp(p.sc->w, kOperandTop));
-    const float factor = is_grad(USE) ? rescale_of(p.rescale) : 1.f;
-    int local = 0;
-    bool ok = true;
-    // a block that gave up fills its tiles with NaN: nothing it did not compute passes for a result
-    auto begin = [&](int buf) {
-      ok = ok && mbar_wait(&tfull[buf], (local / 2) & 1, gave_up);
-      ok = __all_sync(kFullMask, ok);
-      tmem_after_sync();
-    };
-    auto end = [&](int buf) {
-      tmem_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_leader(tempty_at[buf]);
-      local++;
-    };
-    const int chunks = (p.ntile + 31) / 32;
+    if (p.split_scale) c = kLog2e * pow2(-scale_exp(p.sc->h, kOperandTop)) * pow2(-scale_exp(p.sc->w, kOperandTop));
+    Reader reader(pipe, gave_up, tmem);
     for (int t = pair; t < tiles; t += npairs) {
-      int m, n, k;
-      tile_of<USE>(p, t, m, n, k);
-      const int64_t r = (int64_t)m * kPairM + rank * kM + row;
-      auto fetch = [&](int ch, float (&x)[32]) {
-        if (ok) {
-          tmem_load32(lanes + (local & 1) * 256 + ch * 32, x);
-          tmem_wait_load();
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; i++) x[i] = __int_as_float(0x7fffffff);
-        }
-      };
+      const int n = column_tile(t);
+      const int64_t r = first_row(t) + row;
+      const int64_t first = p.b_y + (int64_t)n * kN, left = p.vocab - first;   // columns of the tile that are words
       if (USE == kLogits) {
-        const int buf = local & 1;
-        begin(buf);
+        reader.begin();
         Part part{-INFINITY, 0.f};
-        const int64_t left = p.vocab - (int64_t)n * kN;   // columns of the tile that are words
-        for (int ch = half; ch < chunks; ch += 2) {
+        for (int ch = half; ch < kN / 32; ch += 2) {
           float x[32];
-          fetch(ch, x);
+          reader.fetch(ch * 32, x);
           if (left < kN) {
 #pragma unroll
             for (int i = 0; i < 32; i++)
@@ -883,22 +851,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) prod
           part.s += s0 + s1;
         }
         if (r < p.rows) p.parts[(int64_t)(2 * n + half) * p.ldparts + r] = part;
-        end(buf);
-      } else if (USE == kProbs) {
-        const int buf = local & 1;
-        ok = ok && mbar_wait(&hfull[buf], (local / 2) & 1, gave_up);
-        ok = __all_sync(kFullMask, ok);
-        const RowCoef rc = ok ? coef_s[buf][row] : RowCoef{INFINITY, 0.f, 0.f, 0u};
-        const unsigned hits = rc.hits;
-        const int64_t left = p.vocab - p.word0 - (int64_t)n * kN;
-        const int64_t first = p.word0 + (int64_t)n * kN;
-        const int *y = p.targets + r * p.labels;
+      } else {
+        const bool there = reader.wait(pipe.hfull);
+        const RowCoef rc = there ? coef_s[reader.local & 1][row] : RowCoef{INFINITY, 0.f, 0.f, 0u};
         __syncwarp();
-        if (lane == 0) mbar_arrive_leader(smem_addr(&hempty[buf]));
-        begin(buf);
-        for (int ch = half; ch < chunks; ch += 2) {
+        if (lane == 0) mbar_arrive_leader(smem_addr(&pipe.hempty[reader.local & 1]));
+        reader.begin();
+        const int *y = p.targets + r * p.labels;
+        for (int ch = half; ch < kN / 32; ch += 2) {
           float x[32];
-          fetch(ch, x);
+          reader.fetch(ch * 32, x);
 #pragma unroll
           for (int i = 0; i < 32; i++) x[i] = exp2_fast(fmaf(x[i], c, -rc.lse2)) * rc.coef;
           if (left < kN) {
@@ -906,8 +868,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) prod
             for (int i = 0; i < 32; i++)
               if (ch * 32 + i >= left) x[i] = 0.f;
           }
-          if (__any_sync(kFullMask, hits >> ch & 1)) {
-            if (hits >> ch & 1)
+          if (__any_sync(kFullMask, rc.hits >> ch & 1)) {
+            if (rc.hits >> ch & 1)
               for (int j = 0; j < p.labels; j++) {
                 const int64_t at = y[j] - first - ch * 32;
 #pragma unroll
@@ -920,55 +882,352 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) prod
           else if (p.prob_lo) store_probs<false, true>(to, p.prob_lo, x);
           else store_probs<false, false>(to, 0, x);
         }
-        end(buf);
-      } else if (USE == kGrad) {
-        const int buf = local & 1;
-        begin(buf);
+      }
+      reader.end();
+    }
+  }
+  pair_end(tmem);
+}
+
+// ---- gradients from a piece of d -------------------------------------------------------------
+//
+// One launch computes the tiles of both gradients.  The pairs take whole tiles in turn (those that run
+// together share a strip of d) as long as there is one for each; what is left of both is cut into equal
+// shares of blocks of K, so that all pairs finish together, whatever the sizes.  A tile that was cut
+// leaves its pieces in memory, at most two a pair, and pieces_kernel adds them in their order.
+struct Side {
+  CUtensorMap a, b;         // d or its transpose, and the operand
+  int kblocks, tiles, whole;// of 64; tiles, and how many each pair takes whole
+  int a_mn;                 // d transposed
+  int b_y;                  // first row of the operand
+  int pa[3], pb[3];
+  int rows;
+  float *acc;               // sums of earlier launches, or of this one for later ones
+  int add, last;
+  void *out;
+  int64_t ldout;
+  int out_wide;
+  Rescale rescale;
+  __host__ __device__ __forceinline__ int rest(int npairs) const { return tiles > whole * npairs ? tiles - whole * npairs : 0; }
+};
+
+struct Gradients {
+  Side side[2];             // dW, dH
+  int nt, ntile;            // column tiles, and their width (a multiple of 32)
+  int npairs, sharers;      // pairs of CTAs; how many of them share what is left
+  int64_t left;             // its blocks of K
+  int pairs, segment;       // pairs of parts; blocks of K that are accumulated in tensor memory at a time
+  int bf16, strip, dim, out_type;
+  int64_t ldacc;
+  float *scratch;           // kM x kN for each CTA
+  float *pieces;            // [pair][2][kPairM][ntile]
+};
+
+struct Piece {
+  int side, tile, k0, k1, slot;   // slot -1: a whole tile; 0: it was begun by another pair; 1: begun here
+};
+
+__host__ __device__ __forceinline__ int64_t share_begin(const Gradients &g, int pair) { return pair * g.left / g.sharers; }
+
+// The side, tile and block of K at a place in what is left.  A tile counts for kReading blocks more than
+// it has: what reading it from tensor memory takes.
+constexpr int kReading = 8;
+__device__ __forceinline__ void place(const Gradients &g, int64_t at, int &side, int &tile, int &k) {
+  const int64_t first = (int64_t)g.side[0].rest(g.npairs) * (g.side[0].kblocks + kReading);
+  side = at >= first;
+  const int64_t q = side ? at - first : at;
+  const Side &s = g.side[side];
+  tile = s.whole * g.npairs + (int)(q / (s.kblocks + kReading));
+  k = (int)(q % (s.kblocks + kReading));
+}
+
+struct Walk {
+  const Gradients &g;
+  int pair, i = 0;
+  int64_t at, end;
+
+  __device__ __forceinline__ Walk(const Gradients &grads, int p) : g(grads), pair(p) {
+    at = p < g.sharers ? share_begin(g, p) : 0;
+    end = p < g.sharers ? share_begin(g, p + 1) : 0;
+  }
+  __device__ __forceinline__ bool next(Piece &p) {
+    const int w0 = g.side[0].whole, w1 = g.side[1].whole;
+    while (i < w0 + w1) {
+      p.side = i >= w0;
+      p.tile = (i - (p.side ? w0 : 0)) * g.npairs + pair;
+      p.k0 = 0;
+      p.k1 = g.side[p.side].kblocks;
+      p.slot = -1;
+      i++;
+      if (p.tile < g.side[p.side].tiles) return true;
+    }
+    while (at < end) {
+      place(g, at, p.side, p.tile, p.k0);
+      const int all = g.side[p.side].kblocks, to = (int)min((int64_t)(all + kReading), p.k0 + (end - at));
+      at += to - p.k0;
+      p.k1 = min(all, to);
+      p.slot = p.k0 == 0 ? (p.k1 == all ? -1 : 1) : 0;
+      if (p.k0 < p.k1) return true;
+    }
+    return false;
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ void put16(T *to, const float (&v)[16]) {
+#pragma unroll
+  for (int b = 0; b < 2; b++) {
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) x[e] = v[b * 8 + e];
+    store8(to + b * 8, x);
+  }
+}
+
+// A column of every other row, from row `first`, of the `rows` that exist.
+template <typename T>
+__device__ __forceinline__ void put_rows(T *to, int64_t step, const float *from, int first, int rows) {
+  float x[16];
+#pragma unroll
+  for (int i = 0; i < 16; i++) x[i] = from[i * 34];
+#pragma unroll
+  for (int i = 0; i < 16; i++)
+    if (first + 2 * i < rows) to[i * step] = from_float<T>(x[i]);
+}
+
+// 32 rows x 16 columns of a finished tile, a row a lane (row0: lane 0's).  Rows that no wide store fits
+// go through `stage`, 32 x 17 floats of this warp's, so that half a warp writes a row's 16 in one piece.
+__device__ __forceinline__ void put_tile(const Gradients &g, const Side &s, int64_t row0, int at, const float *x, float factor,
+                                         float *stage) {
+  if (at >= g.dim) return;
+  const int lane = threadIdx.x & 31;
+  const int64_t r = row0 + lane;
+  float v[16];
+#pragma unroll
+  for (int e = 0; e < 16; e++) v[e] = x[e];
+  float *acc = s.acc + r * g.ldacc + at;
+  if (s.add && r < s.rows) {
+#pragma unroll
+    for (int b = 0; b < 2; b++) {
+      float old[8];
+      load8(acc + b * 8, old);
+#pragma unroll
+      for (int e = 0; e < 8; e++) v[b * 8 + e] += old[e];
+    }
+  }
+  if (!s.last) {
+    if (r < s.rows) put16(acc, v);
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 16; e++) v[e] *= factor;
+  if (s.out_wide && at + 16 <= g.dim) {
+    if (r >= s.rows) return;
+    const int64_t to = r * s.ldout + at;
+    if (g.out_type == W2V_F32) put16(static_cast<float *>(s.out) + to, v);
+    else if (g.out_type == W2V_BF16) put16(static_cast<__nv_bfloat16 *>(s.out) + to, v);
+    else put16(static_cast<__half *>(s.out) + to, v);
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 16; e++) stage[lane * 17 + e] = v[e];
+  __syncwarp();
+  const int c = lane % 16, first = lane / 16;
+  const int rows = at + c < g.dim ? (int)min((int64_t)32, s.rows - row0) : 0;
+  const int64_t to = (row0 + first) * s.ldout + at + c;
+  if (g.out_type == W2V_F32) put_rows(static_cast<float *>(s.out) + to, 2 * s.ldout, stage + first * 17 + c, first, rows);
+  else if (g.out_type == W2V_BF16)
+    put_rows(static_cast<__nv_bfloat16 *>(s.out) + to, 2 * s.ldout, stage + first * 17 + c, first, rows);
+  else put_rows(static_cast<__half *>(s.out) + to, 2 * s.ldout, stage + first * 17 + c, first, rows);
+  __syncwarp();
+}
+
+template <bool SEGMENTS>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) grad_kernel(const __grid_constant__ Gradients g) {
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char *smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
+  __shared__ Pipe pipe;
+  __shared__ float stage_s[8][32 * 17];
+  volatile int *gave_up = &pipe.gave_up;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+  const uint32_t tmem = pair_begin(pipe);
+  const int rank = (int)cluster_rank();
+  Walk walk(g, blockIdx.x / 2);
+  Piece p;
+
+  if (warp == 0) {
+    if (elected()) {
+      Ring ring{pipe, smem, gave_up};
+      bool ok = true;
+      // each CTA brings its own rows of d and half of the operand's columns
+      const int half_n = g.ntile / 2, groups = (half_n + 63) / 64;
+      const unsigned bytes = 2 * (kBytesA + groups * 8192);
+      while (ok && walk.next(p)) {
+        const Side &s = g.side[p.side];
+        const int row = p.tile / g.nt * kPairM + rank * kM, col = p.tile % g.nt * g.ntile + rank * half_n;
+        for (int k0 = p.k0; ok && k0 < p.k1; k0 += g.segment)
+          for (int q = 0; ok && q < g.pairs; q++)
+            for (int kb = k0; kb < min(p.k1, k0 + g.segment); kb++) {
+              unsigned char *a, *b;
+              uint32_t bar;
+              if (!(ok = ring.next(bytes, a, b, bar))) break;
+              if (s.a_mn) {   // 64 rows of two strips
+                for (int i = 0; i < 2; i++)
+                  tma_load_2d(a + i * 8192, &s.a, 0, s.pa[q] + (row / 64 + i) * g.strip + kb * kK, bar);
+              } else {        // 128 rows of a strip
+                tma_load_2d(a, &s.a, 0, s.pa[q] + kb * g.strip + row, bar);
+              }
+              for (int i = 0; i < groups; i++)
+                tma_load_2d(b + i * 8192, &s.b, s.pb[q] + col + i * 64, s.b_y + kb * kK, bar);
+            }
+      }
+      if (!ok) ring.settle();
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (rank == 0 && elected()) {
+      Issue issue{pipe, gave_up, tmem, smem_addr(smem)};
+      bool ok = true;
+      while (ok && walk.next(p)) {
+        const bool mn = g.side[p.side].a_mn;
+        const uint32_t idesc = mma_desc(g.bf16, mn, true, kPairM, g.ntile);
+        const uint64_t da = issue.desc(0, mn), db = issue.desc(kBytesA, true);
+        const uint32_t step_a = mn ? 2048 >> 4 : 32 >> 4;
+        for (int k0 = p.k0; ok && k0 < p.k1; k0 += g.segment) {
+          uint32_t d;
+          if (!(ok = issue.begin(d))) break;
+          const int blocks = g.pairs * (min(p.k1, k0 + g.segment) - k0);
+          for (int b = 0; ok && b < blocks; b++) ok = issue.block<true>(d, da, db, step_a, 2048 >> 4, idesc, b > 0, kK / 16);
+          if (ok) issue.end();
+        }
+      }
+      if (!ok) issue.settle();
+    }
+    __syncwarp();
+  } else if (warp >= 4) {
+    const int half = (warp - 4) / 4, row = (warp & 3) * 32;
+    const int chunks = g.ntile / 32;
+    float *stage = stage_s[warp - 4];
+    const float factor[2] = {rescale_of(g.side[0].rescale), rescale_of(g.side[1].rescale)};
+    Reader reader(pipe, gave_up, tmem);
+    while (walk.next(p)) {
+      const Side &s = g.side[p.side];
+      const int n = p.tile % g.nt;
+      const int64_t row0 = (int64_t)(p.tile / g.nt) * kPairM + rank * kM + row;
+      float *piece = g.pieces + ((int64_t)(walk.pair * 2 + max(p.slot, 0)) * kPairM + rank * kM + row + lane) * g.ntile;
+      // 32 columns of the sum over the piece
+      auto finish = [&](int ch, const float (&x)[32]) {
+        if (p.slot < 0) {
+          put_tile(g, s, row0, n * g.ntile + ch * 32, x, factor[p.side], stage);
+          put_tile(g, s, row0, n * g.ntile + ch * 32 + 16, x + 16, factor[p.side], stage);
+        } else {
+#pragma unroll
+          for (int b = 0; b < 4; b++) {
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] = x[b * 8 + e];
+            store8(piece + ch * 32 + b * 8, v);
+          }
+        }
+      };
+      if (!SEGMENTS) {
+        reader.begin();
         for (int ch = half; ch < chunks; ch += 2) {
           float x[32];
-          fetch(ch, x);
-#pragma unroll
-          for (int b = 0; b < 4; b++) put_grad(p, r, n, k, ch * 32 + b * 8, &x[b * 8], factor);
+          reader.fetch(ch * 32, x);
+          finish(ch, x);
         }
-        end(buf);
+        reader.end();
       } else {
         // the tensor cores truncate what they accumulate: after `segment` blocks of K the sum goes on in
-        // fp32 with rounding, in a scratch of the block's own that stays in L2 (a thread's eight values
+        // fp32 with rounding, in a scratch of the CTA's own that stays in L2 (a thread's eight values
         // side by side, a warp's in one piece); registers for it would spill
-        float *mine = p.scratch + (int64_t)blockIdx.x * kM * kN + (threadIdx.x - 128) * 8;
-        const int kstart = first_k(k), kend = first_k(k + 1);
-        for (int k0 = kstart; k0 < kend; k0 += p.segment) {
-          const int buf = local & 1;
-          begin(buf);
+        float *mine = g.scratch + (int64_t)blockIdx.x * kM * kN + (threadIdx.x - 128) * 8;
+        for (int k0 = p.k0; k0 < p.k1; k0 += g.segment) {
+          reader.begin();
           for (int ch = half; ch < chunks; ch += 2) {
-            float x[32];
+            float x[32], old[4][8];
             float *at = mine + ch / 2 * (4 * 256 * 8);
-            float old[4][8];
-            if (k0 > kstart) {
+            if (k0 > p.k0) {
 #pragma unroll
               for (int b = 0; b < 4; b++) load8(at + b * (256 * 8), old[b]);
             }
-            fetch(ch, x);
+            reader.fetch(ch * 32, x);
+            if (k0 > p.k0) {
 #pragma unroll
-            for (int b = 0; b < 4; b++) {
-              float v[8];
+              for (int i = 0; i < 32; i++) x[i] += old[i / 8][i % 8];
+            }
+            if (k0 + g.segment < p.k1) {
 #pragma unroll
-              for (int e = 0; e < 8; e++) v[e] = k0 > kstart ? x[b * 8 + e] + old[b][e] : x[b * 8 + e];
-              if (k0 + p.segment < kend) store8(at + b * (256 * 8), v);
-              else put_grad(p, r, n, k, ch * 32 + b * 8, v, factor);
+              for (int b = 0; b < 4; b++) {
+                float v[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) v[e] = x[b * 8 + e];
+                store8(at + b * (256 * 8), v);
+              }
+            } else {
+              finish(ch, x);
             }
           }
-          end(buf);
+          reader.end();
         }
       }
     }
   }
-  // neither CTA leaves while the other's products read its shared memory or its barriers are arrived on
-  tmem_before_sync();
-  __syncwarp();
-  cluster_sync();
-  tmem_after_sync();
-  if (warp == 2) tmem_free(tmem, 512);
+  pair_end(tmem);
+}
+
+// The tiles that were cut: blockIdx.x is the tile in what is left, a warp a row.
+template <typename T>
+__global__ void __launch_bounds__(256) pieces_kernel(const __grid_constant__ Gradients g) {
+  const int t = blockIdx.x, rest0 = g.side[0].rest(g.npairs);
+  const Side &s = g.side[t >= rest0];
+  const int64_t begin = t < rest0 ? (int64_t)t * (g.side[0].kblocks + kReading)
+                                  : (int64_t)rest0 * (g.side[0].kblocks + kReading) +
+                                        (int64_t)(t - rest0) * (g.side[1].kblocks + kReading);
+  // the pair whose share holds a place: the last one that begins at or before it
+  auto pair_at = [&](int64_t at) { return (int)(((at + 1) * g.sharers - 1) / g.left); };
+  const int first = pair_at(begin), last = pair_at(begin + s.kblocks - 1);
+  if (first == last) return;
+  const int tile = s.whole * g.npairs + (t < rest0 ? t : t - rest0);
+  const int row = blockIdx.y * 8 + threadIdx.x / 32, lane = threadIdx.x & 31;
+  const int64_t r = (int64_t)(tile / g.nt) * kPairM + row;
+  if (r >= s.rows) return;
+  const float factor = rescale_of(s.rescale);
+  const int col = lane * 8, at = tile % g.nt * g.ntile + col;
+  if (col >= g.ntile || at >= g.dim) return;
+  float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  for (int q = first; q <= last; q += 4) {
+    float x[4][8];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const int pair = min(q + j, last);
+      load8(g.pieces + ((int64_t)(pair * 2 + (pair == first)) * kPairM + row) * g.ntile + col, x[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      if (q + j <= last) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] += x[j][e];
+      }
+  }
+  float *acc = s.acc + r * g.ldacc + at;
+  if (s.add) {
+    float old[8];
+    load8(acc, old);
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] += old[e];
+  }
+  if (!s.last) {
+    store8(acc, v);
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; e++) v[e] *= factor;
+  T *to = static_cast<T *>(s.out) + r * s.ldout + at;
+  const int have = min(8, g.dim - at);
+  if (s.out_wide && have == 8) store8(to, v);
+  else store_some(to, have, v);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -1012,17 +1271,35 @@ struct Operand {
   int width;   // offset between parts
 };
 
+// An attribute of the function on the current device, so it is set before every launch.
+template <typename K>
+int allow_smem(K kernel, size_t bytes) {
+  return (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+}
+int sm_pairs() { return std::max(1, device_sm_count() / 2); }
+
 template <Use USE>
-int launch_product(Product &p, const Operand &a, const Operand &b, cudaStream_t s) {
-  int err = tensor_map(&p.a, a.p, a.inner, a.rows, a.ld, p.a_mn ? 64 : kM);
-  if (!err) err = tensor_map(&p.b, b.p, b.inner, b.rows, b.ld, p.b_mn ? 64 : kN / 2);
+int launch_product(const Product &p, cudaStream_t s) {
+  const int err = allow_smem(product_kernel<USE>, kSmem);
   if (err) return err;
-  // an attribute of the function on the current device, so it is set on every device that gets here
-  const cudaError_t e = cudaFuncSetAttribute(product_kernel<USE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
-  if (e != cudaSuccess) return (int)e;
-  const int tiles = p.mt * p.nt * p.splits;
-  product_kernel<USE><<<2 * std::max(1, std::min(tiles, device_sm_count() / 2)), kMmaThreads, kSmem, s>>>(p);
+  product_kernel<USE><<<2 * std::min(p.mt * p.nt, sm_pairs()), kMmaThreads, kSmem, s>>>(p);
   count_launch(1);
+  return (int)cudaGetLastError();
+}
+
+template <typename T>
+int launch_gradients(const Gradients &g, cudaStream_t s) {
+  constexpr bool split = sizeof(T) == 4;
+  const int err = allow_smem(grad_kernel<split>, kSmem);
+  if (err) return err;
+  const bool whole = g.side[0].whole || g.side[1].whole;
+  grad_kernel<split><<<2 * (whole ? g.npairs : g.sharers), kMmaThreads, kSmem, s>>>(g);
+  count_launch(1);
+  const int rest = g.side[0].rest(g.npairs) + g.side[1].rest(g.npairs);
+  if (rest > 0 && g.sharers > 1) {
+    pieces_kernel<T><<<dim3(rest, kPairM / 8), 256, 0, s>>>(g);
+    count_launch(1);
+  }
   return (int)cudaGetLastError();
 }
 
@@ -1052,35 +1329,16 @@ int few_dh_blocks(int64_t vocab) {
 int few_rows_of(int64_t n) { return n <= 1 ? 1 : n <= 2 ? 2 : n <= 4 ? 4 : 8; }
 
 struct Layout {
-  int64_t scalars, coef, hs, ws, parts, probs, scratch, acc_h, acc_w, total;
+  int64_t scalars, hs, ws, parts, probs, scratch, pieces, acc_h, acc_w, total;
   int width, nparts;         // staged operands
   int64_t rows, words;       // of a piece of d
-  int nt, ntile, hsplits, wsplits;
-  bool direct_h, direct_w;   // sums are complete in one go: no slabs
+  int nt, ntile;
 };
 
 // Column tiles of a gradient: as few as hold dim, equally wide.
 void column_tiles(int dim, int *nt, int *ntile) {
   *nt = (dim + kN - 1) / kN;
   *ntile = (int)up((dim + *nt - 1) / *nt, 32);
-}
-// In how many parts K is cut, each with a slab of sums of its own, by an estimate in microseconds: the
-// rounds of tiles over the pairs of SMs, a block of K taking 512 clocks for 256 columns, against
-// writing the slabs and reading them again at about 5 TB/s.  With one part and `whole` there is no slab.
-int splits_for(int64_t tiles, int64_t kblocks, int pairs, int ntile, int64_t slab_bytes, bool whole) {
-  const int sms = std::max(1, device_sm_count() / 2);
-  int best = 1;
-  double cost = 1e30;
-  for (int s = 1; s <= 32 && (s == 1 || kblocks / s >= 4); s++) {
-    const double rounds = (double)((tiles * s + sms - 1) / sms);
-    const double product = rounds * ((double)kblocks / s * pairs * 512 * ntile / kN + 1500) / 1700;
-    const double slabs = s == 1 && whole ? 0 : 2.0 * s * slab_bytes / 5e6;
-    if (product + slabs < cost) {
-      cost = product + slabs;
-      best = s;
-    }
-  }
-  return best;
 }
 
 Layout plan(const Shape &x, bool grad) {
@@ -1117,19 +1375,12 @@ Layout plan(const Shape &x, bool grad) {
     const int64_t pieces = std::max<int64_t>(1, (x.vocab + most * 5 / 4 - 1) / (most * 5 / 4));
     l.words = up((x.vocab + pieces - 1) / pieces, kN);
     column_tiles(x.dim, &l.nt, &l.ntile);
-    const int pairs = x.type == W2V_F32 ? 3 : 1;
     const int64_t cols = (int64_t)l.nt * l.ntile * 4;
-    l.hsplits = splits_for(l.rows / kPairM * l.nt, l.words / kK, pairs, l.ntile, l.rows * cols, l.words >= x.vocab && x.dim % 8 == 0);
-    l.wsplits = splits_for(l.words / kPairM * l.nt, l.rows / kK, pairs, l.ntile, l.words * cols,
-                           l.rows >= x.n && x.dim % 8 == 0);
-    l.coef = take(x.n * sizeof(RowCoef));
     l.probs = take(l.rows * l.words * bytes);
-    if (x.type == W2V_F32) l.scratch = take((int64_t)device_sm_count() * kM * kN * 4);
-    // rows that are not a multiple of eight elements are better written by a warp each than by a thread each
-    l.direct_h = l.hsplits == 1 && l.words >= x.vocab && x.dim % 8 == 0;
-    l.direct_w = l.wsplits == 1 && l.rows >= x.n && x.dim % 8 == 0;
-    if (!l.direct_h) l.acc_h = take((int64_t)l.hsplits * l.rows * l.nt * l.ntile * 4);
-    if (!l.direct_w) l.acc_w = take((int64_t)l.wsplits * up(x.vocab, kM) * l.nt * l.ntile * 4);
+    if (x.type == W2V_F32) l.scratch = take((int64_t)sm_pairs() * kPairM * kN * 4);
+    l.pieces = take((int64_t)sm_pairs() * 2 * kPairM * l.ntile * 4);
+    if (l.words < x.vocab) l.acc_h = take(l.rows * cols);
+    if (l.rows < x.n) l.acc_w = take(up(x.vocab, kPairM) * cols);
   }
   l.total = at;
   return l;
@@ -1143,17 +1394,17 @@ bool direct(const void *p, int64_t ld) {   // TMA can read the caller's matrix
 // Operands for the products: the caller's own where TMA can read them, else staged ones.
 template <typename T>
 int stage(const Shape &x, const Layout &l, const void *h, int64_t ldh, const void *w, int64_t ldw, const float *gloss,
-          int64_t ldg, const int *targets, char *ws, Operand *oh, Operand *ow, cudaStream_t s) {
+          const int *targets, char *ws, Operand *oh, Operand *ow, cudaStream_t s) {
   constexpr bool split = sizeof(T) == 4;
   Scalars *sc = reinterpret_cast<Scalars *>(ws + l.scalars);
   const Source sh{h, ldh, x.n}, sw{w, ldw, x.vocab};
-  cudaError_t e = cudaMemsetAsync(sc, 0, sizeof(Scalars), s);
-  if (e != cudaSuccess) return (int)e;
   const int blocks = device_sm_count() * 8;
   if (split || gloss) {
+    const cudaError_t e = cudaMemsetAsync(sc, 0, sizeof(Scalars), s);
+    if (e != cudaSuccess) return (int)e;
     const Source none{nullptr, 0, x.n};
     amax_kernel<<<dim3(split ? blocks : 64, 1, 3), 256, 0, s>>>(split ? sh : none, split ? sw : Source{nullptr, 0, 0},
-                                                                 x.dim, gloss, ldg, targets, x.labels, x.vocab, sc);
+                                                                 x.dim, gloss, targets, x.labels, x.vocab, sc);
     count_launch(1);
   }
   void *hs = direct<T>(h, ldh) ? nullptr : ws + l.hs, *wst = direct<T>(w, ldw) ? nullptr : ws + l.ws;
@@ -1168,24 +1419,24 @@ int stage(const Shape &x, const Layout &l, const void *h, int64_t ldh, const voi
 }
 
 template <typename T>
-Product logits_product(const Shape &x, const Operand &oh, const Operand &ow, const Scalars *sc) {
+int logits_product(const Shape &x, const Operand &oh, const Operand &ow, const Scalars *sc, Product *to) {
   Product p{};
   constexpr bool split = sizeof(T) == 4;
-  p.ntile = kN;
-  p.splits = 1;
+  int err = tensor_map(&p.a, oh.p, oh.inner, oh.rows, oh.ld, kM);
+  if (!err) err = tensor_map(&p.b, ow.p, ow.inner, ow.rows, ow.ld, kN / 2);
   p.kblocks = (x.dim + kK - 1) / kK;
+  p.k16 = (x.dim - (p.kblocks - 1) * kK + 15) / 16;
   p.pairs = split ? 3 : 1;
   if (split) {   // lo hi, hi lo, hi hi
     p.pa[0] = oh.width;
     p.pb[1] = ow.width;
   }
-  p.segment = p.kblocks;
-  p.k16 = (x.dim - (p.kblocks - 1) * kK + 15) / 16;
   p.bf16 = x.type == W2V_BF16;
   p.sc = sc;
   p.split_scale = split;
   p.vocab = x.vocab;
-  return p;
+  *to = p;
+  return err;
 }
 
 template <typename T, int RB>
@@ -1226,9 +1477,11 @@ int run_loss(const Shape &x, const Layout &l, const void *h, int64_t ldh, const 
     return err ? err : join_rows(count, x.n, 0, (int)x.n);
   }
   Operand oh, ow;
-  int err = stage<T>(x, l, h, ldh, w, ldw, nullptr, 0, nullptr, ws, &oh, &ow, s);
+  int err = stage<T>(x, l, h, ldh, w, ldw, nullptr, nullptr, ws, &oh, &ow, s);
   if (err) return err;
-  Product p = logits_product<T>(x, oh, ow, reinterpret_cast<const Scalars *>(ws + l.scalars));
+  Product p;
+  err = logits_product<T>(x, oh, ow, reinterpret_cast<const Scalars *>(ws + l.scalars), &p);
+  if (err) return err;
   p.nt = (int)((x.vocab + kN - 1) / kN);
   p.parts = parts;
   for (int64_t r0 = 0; r0 < x.n; r0 += kLossRows) {
@@ -1236,7 +1489,7 @@ int run_loss(const Shape &x, const Layout &l, const void *h, int64_t ldh, const 
     p.mt = (p.rows + kPairM - 1) / kPairM;
     p.a_y = (int)r0;
     p.ldparts = p.rows;
-    err = launch_product<kLogits>(p, oh, ow, s);
+    err = launch_product<kLogits>(p, s);
     if (!err) err = join_rows(2 * p.nt, p.ldparts, r0, p.rows);
     if (err) return err;
   }
@@ -1259,8 +1512,8 @@ int few_grad(const Shape &x, const Layout &l, const void *h, int64_t ldh, const 
   const int blocks = few_dh_blocks(x.vocab);
   few_dh_kernel<T, RB><<<dim3(blocks, (x.dim + kFewThreads - 1) / kFewThreads), kFewThreads, 0, s>>>(wt, ldw, x.vocab,
                                                                                                     x.dim, d, acc);
-  slabs_kernel<T><<<(int)std::min<int64_t>((x.n * ((x.dim + 255) / 256) + 7) / 8, 1024), 256, 0, s>>>(
-      acc, blocks, (int64_t)RB * x.dim, x.dim, x.n, x.dim, static_cast<T *>(dh), lddh, false, Rescale{nullptr, nullptr, 0});
+  slabs_kernel<T><<<(int)((x.n * ((x.dim + 31) / 32) + 7) / 8), 256, 0, s>>>(acc, blocks, (int64_t)RB * x.dim, x.n, x.dim,
+                                                                           static_cast<T *>(dh), lddh);
   count_launch(3);
   return (int)cudaGetLastError();
 }
@@ -1279,94 +1532,92 @@ int run_grad(const Shape &x, const Layout &l, const void *h, int64_t ldh, const 
     }
   }
   constexpr bool split = sizeof(T) == 4;
+  const float *each_gloss = ldg ? gloss : nullptr, *one_gloss = ldg ? nullptr : gloss;
   Operand oh, ow;
-  int err = stage<T>(x, l, h, ldh, w, ldw, gloss, ldg, targets, ws, &oh, &ow, s);
+  int err = stage<T>(x, l, h, ldh, w, ldw, each_gloss, targets, ws, &oh, &ow, s);
   if (err) return err;
   const Scalars *sc = reinterpret_cast<const Scalars *>(ws + l.scalars);
-  RowCoef *coef = reinterpret_cast<RowCoef *>(ws + l.coef);
-  row_coef_kernel<<<(int)((x.n + 255) / 256), 256, 0, s>>>(lse, gloss, ldg, targets, x.labels, x.vocab, x.n, sc, coef);
-  count_launch(1);
-  const int64_t ldacc = (int64_t)l.nt * l.ntile;
+  // one factor for all rows is left to the end: the targets' -1 then has no rounding in d
+  int given = kFromRows;
+  if (one_gloss)
+    for (given = kProbTop; (1 << (kProbTop - given)) < x.labels;) given--;
   // d lies in strips of 64 columns, 128 bytes a row: what a warp writes of a tile, and what a load of
   // either gradient's operand reads, is one piece of memory
-  const int strips = (int)(l.words / 64) * (split ? 2 : 1);
-  const Operand probs{ws + l.probs, 64, 64, strips * l.rows, (int)(l.words / 64 * l.rows)};
+  const int strip_rows = (int)(l.words / 64 * l.rows);
+  Product p;
+  err = logits_product<T>(x, oh, ow, sc, &p);
+  p.labels = x.labels;
+  p.given = given;
+  p.probs = reinterpret_cast<uint16_t *>(ws + l.probs);
+  p.strip = (int)l.rows;
+  p.prob_lo = split ? (int64_t)strip_rows * 64 : 0;
+
+  Gradients g{};
+  g.nt = l.nt;
+  g.ntile = l.ntile;
+  g.npairs = sm_pairs();
+  g.pairs = split ? 3 : 1;
+  g.segment = split ? kSegment : 1 << 30;
+  g.bf16 = x.type == W2V_BF16;
+  g.strip = (int)l.rows;
+  g.dim = x.dim;
+  g.out_type = x.type;
+  g.ldacc = (int64_t)l.nt * l.ntile;
+  g.scratch = reinterpret_cast<float *>(ws + l.scratch);
+  g.pieces = reinterpret_cast<float *>(ws + l.pieces);
+  for (int i = 0; i < 2 && !err; i++) {
+    Side &side = g.side[i];
+    const Operand &o = i == 0 ? oh : ow;
+    side.a_mn = i == 0;
+    err = tensor_map(&side.a, ws + l.probs, 64, (int64_t)strip_rows * (split ? 2 : 1), 64, side.a_mn ? 64 : kM);
+    if (!err) err = tensor_map(&side.b, o.p, o.inner, o.rows, o.ld, 64);
+    if (split) {   // (lo 2^11) (hi 2^-11), hi lo, hi hi
+      side.pa[0] = strip_rows;
+      side.pb[0] = 2 * o.width;
+      side.pb[1] = o.width;
+    }
+    side.rescale = Rescale{sc, one_gloss, given, split ? (i == 0 ? 2 : 1) : 0};
+    side.ldout = i == 0 ? lddw : lddh;
+  }
+  if (err) return err;
   float *acc_h = reinterpret_cast<float *>(ws + l.acc_h), *acc_w = reinterpret_cast<float *>(ws + l.acc_w);
-  const int64_t acc_w_rows = up(x.vocab, kM);
-  const int sums = device_sm_count() * 8;
-  const float *one_gloss = ldg ? nullptr : gloss;
-  const Rescale rescale_h{sc, one_gloss, split ? 1 : 0}, rescale_w{sc, one_gloss, split ? 2 : 0};
   for (int64_t r0 = 0; r0 < x.n; r0 += l.rows) {
     const int rows = (int)std::min(l.rows, x.n - r0);
     for (int64_t v0 = 0; v0 < x.vocab; v0 += l.words) {
       const int words = (int)std::min(l.words, x.vocab - v0);
-      Product p = logits_product<T>(x, oh, ow, sc);
       p.mt = (rows + kPairM - 1) / kPairM;
       p.nt = (words + kN - 1) / kN;
       p.a_y = (int)r0;
-      p.b_y = p.word0 = (int)v0;
+      p.b_y = (int)v0;
       p.rows = rows;
-      p.coef = coef + r0;
+      p.lse = lse + r0;
+      p.gloss = each_gloss ? each_gloss + r0 : nullptr;
       p.targets = targets + r0 * x.labels;
-      p.labels = x.labels;
-      p.probs = static_cast<uint16_t *>(const_cast<void *>(probs.p));
-      p.strip = (int)l.rows;
-      p.prob_lo = split ? (int64_t)probs.width * 64 : 0;
-      err = launch_product<kProbs>(p, oh, ow, s);
+      err = launch_product<kProbs>(p, s);
       if (err) return err;
-      for (int which = 0; which < 2; which++) {   // dH, then dW
-        const Operand &o = which == 0 ? ow : oh;
-        Product q{};
-        q.nt = l.nt;
-        q.ntile = l.ntile;
-        q.mt = which == 0 ? p.mt : (words + kPairM - 1) / kPairM;
-        q.kblocks = which == 0 ? (words + kK - 1) / kK : (rows + kK - 1) / kK;
-        // the last piece may be too short for all splits: it adds to some of the slabs, which the
-        // first piece, never the shorter one, has filled
-        q.splits = std::min(which == 0 ? l.hsplits : l.wsplits, q.kblocks);
-        q.pairs = split ? 3 : 1;
-        if (split) {   // (lo 2^11) (hi 2^-11), hi lo, hi hi
-          q.pa[0] = probs.width;
-          q.pb[0] = 2 * o.width;
-          q.pb[1] = o.width;
-        }
-        q.segment = split ? kSegment : q.kblocks;
-        q.k16 = kK / 16;
-        q.scratch = reinterpret_cast<float *>(ws + l.scratch);
-        q.strip = (int)l.rows;
-        q.a_mn = which;
-        q.b_mn = 1;
-        q.b_y = (int)(which == 0 ? v0 : r0);
-        q.bf16 = x.type == W2V_BF16;
-        q.rows = which == 0 ? rows : words;
-        q.dim = x.dim;
-        q.ldacc = ldacc;
-        q.acc = which == 0 ? acc_h : acc_w + v0 * ldacc;
-        q.acc_slab = (which == 0 ? l.rows : acc_w_rows) * ldacc;
-        q.add = which == 0 ? v0 > 0 : r0 > 0;
-        q.rescale = which == 0 ? rescale_h : rescale_w;
-        if (which == 0 ? l.direct_h : l.direct_w) {
-          q.out = which == 0 ? static_cast<T *>(dh) + r0 * lddh : static_cast<T *>(dw) + v0 * lddw;
-          q.ldout = which == 0 ? lddh : lddw;
-          q.out_type = x.type;
-          q.out_wide = aligned(q.out, 8 * sizeof(T)) && q.ldout % 8 == 0;
-        }
-        err = split ? launch_product<kGradSegments>(q, probs, o, s) : launch_product<kGrad>(q, probs, o, s);
-        if (err) return err;
+      g.left = 0;
+      for (int i = 0; i < 2; i++) {
+        Side &side = g.side[i];
+        side.rows = i == 0 ? words : rows;
+        side.kblocks = ((i == 0 ? rows : words) + kK - 1) / kK;
+        side.tiles = (i == 0 ? (words + kPairM - 1) / kPairM : p.mt) * l.nt;
+        // tiles of few blocks of K are not worth cutting: reading one costs as much
+        side.whole = side.kblocks < 16 ? (side.tiles + g.npairs - 1) / g.npairs : side.tiles / g.npairs;
+        side.b_y = (int)(i == 0 ? r0 : v0);
+        side.acc = i == 0 ? acc_w + v0 * g.ldacc : acc_h;
+        side.add = i == 0 ? r0 > 0 : v0 > 0;
+        side.last = i == 0 ? r0 + l.rows >= x.n : v0 + l.words >= x.vocab;
+        side.out = i == 0 ? static_cast<T *>(dw) + v0 * lddw : static_cast<T *>(dh) + r0 * lddh;
+        side.out_wide = aligned(side.out, 8 * sizeof(T)) && side.ldout % 8 == 0;
+        g.left += (int64_t)side.rest(g.npairs) * (side.kblocks + kReading);
       }
-    }
-    if (!l.direct_h) {
-      slabs_kernel<T><<<sums, 256, 0, s>>>(acc_h, l.hsplits, l.rows * ldacc, ldacc, rows, x.dim,
-                                           static_cast<T *>(dh) + r0 * lddh, lddh, true, rescale_h);
-      count_launch(1);
+      // a share of fewer than sixteen blocks of K would not pay for a piece
+      g.sharers = (int)std::max<int64_t>(1, std::min<int64_t>(g.npairs, (g.left + 15) / 16));
+      err = launch_gradients<T>(g, s);
+      if (err) return err;
     }
   }
-  if (!l.direct_w) {
-    slabs_kernel<T><<<sums, 256, 0, s>>>(acc_w, l.wsplits, acc_w_rows * ldacc, ldacc, x.vocab, x.dim,
-                                         static_cast<T *>(dw), lddw, true, rescale_w);
-    count_launch(1);
-  }
-  return (int)cudaGetLastError();
+  return 0;
 }
 
 }  // namespace
