@@ -492,15 +492,16 @@ __global__ void __launch_bounds__(256) stage_kernel(Source h, Source w, int dim,
 // ---------------------------------------------------------------------------------------------
 // The products
 // ---------------------------------------------------------------------------------------------
-constexpr int kM = 128, kN = 256, kK = 64, kStages = 6;   // rows of each of a pair's CTAs, columns of both
+constexpr int kM = 128, kN = 256, kK = 64;   // rows of each of a pair's CTAs, columns of both
 constexpr int kPairM = 2 * kM;
 constexpr int kBytesA = kM * kK * 2, kBytesB = kN / 2 * kK * 2, kBytesStage = kBytesA + kBytesB;
 constexpr int kMmaThreads = 384;   // producer, issuer, two helpers, eight that read the tiles
-constexpr int kSmem = kStages * kBytesStage + 1024;
+constexpr int kMostStages = 6;
+constexpr int smem_bytes(int stages, int more) { return stages * kBytesStage + more + 1024; }
 
 // What the roles of a CTA share.
 struct Pipe {
-  u64 full[kStages], empty[kStages];   // operands: in the leader, counting both CTAs' bytes; read by the products
+  u64 full[kMostStages], empty[kMostStages];   // operands: in the leader, counting both CTAs' bytes; read by the products
   u64 tfull[2], tempty[2];             // halves of tensor memory: finished; read (in the leader, by both CTAs)
   u64 hfull[2], hempty[2];             // rows' coefficients: there; read
   u64 done;
@@ -511,7 +512,7 @@ struct Pipe {
 // Returns the address of the pair's tensor memory.
 __device__ __forceinline__ uint32_t pair_begin(Pipe &s) {
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kStages; i++) {
+    for (int i = 0; i < kMostStages; i++) {
       mbar_init(&s.full[i], 1);
       mbar_init(&s.empty[i], 1);
     }
@@ -542,6 +543,7 @@ __device__ __forceinline__ void pair_end(uint32_t tmem) {
 }
 
 // The producer's place in the ring of stages.
+template <int STAGES>
 struct Ring {
   Pipe &s;
   unsigned char *smem;
@@ -550,8 +552,8 @@ struct Ring {
 
   // The next stage's operands and the leader's barrier for them; false when the wait ran out.
   __device__ __forceinline__ bool next(unsigned bytes, unsigned char *&a, unsigned char *&b, uint32_t &bar) {
-    const int i = it % kStages;
-    if (!mbar_wait(&s.empty[i], (it / kStages + 1) & 1, gave_up)) return false;
+    const int i = it % STAGES;
+    if (!mbar_wait(&s.empty[i], (it / STAGES + 1) & 1, gave_up)) return false;
     it++;
     bar = in_leader(&s.full[i]);
     if (cluster_rank() == 0) mbar_arrive_expect_tx(&s.full[i], bytes);
@@ -563,13 +565,14 @@ struct Ring {
   __device__ __forceinline__ void settle() {
     int none = 0;
     if (cluster_rank() == 0)
-      for (int i = max(0, it - kStages); i < it; i++) mbar_wait(&s.full[i % kStages], (i / kStages) & 1, &none);
+      for (int i = max(0, it - STAGES); i < it; i++) mbar_wait(&s.full[i % STAGES], (i / STAGES) & 1, &none);
     else   // they are counted in the other CTA: a millisecond is long enough for any copy
       for (int i = 0; i < 1000; i++) __nanosleep(1000);
   }
 };
 
 // The issuing thread's place: products of the stages in their order.
+template <int STAGES>
 struct Issue {
   Pipe &s;
   volatile int *gave_up;
@@ -603,7 +606,7 @@ struct Issue {
       for (int i = 1; i < steps; i++) mma_f16(d, da + i * step_a, db + i * step_b, idesc, true);
     }
     mma_commit(&s.empty[stage]);
-    if (++stage == kStages) {
+    if (++stage == STAGES) {
       stage = 0;
       phase ^= 1;
     }
@@ -677,16 +680,10 @@ struct Product {
   int given;                  // of prob_exp
   const int *targets;
   int labels;
-  uint16_t *probs;          // d in strips of 64 columns: [part][strip][row][64]
+  uint16_t *probs;          // d in strips of 64 columns: [part][strip][row][64], see put_strip
   int strip;                // rows of a strip
   int64_t prob_lo;          // offset of the second part, 0 for none
 };
-
-__device__ __forceinline__ void store32(void *a, const uint32_t (&r)[8]) {
-  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(a), "r"(r[0]), "r"(r[1]), "r"(r[2]),
-               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-               : "memory");
-}
 
 template <bool BF16>
 __device__ __forceinline__ uint32_t halves(float a, float b) {
@@ -698,25 +695,46 @@ __device__ __forceinline__ uint32_t halves(float a, float b) {
   return *reinterpret_cast<const uint32_t *>(&p);
 }
 
-// 32 values to 16 bits at `to` (32-byte aligned), and what that lacks, times 2^11, `lo` elements on.
+// 32 values as 16 bits, and for LO what those lack, times 2^11.
 template <bool BF16, bool LO>
-__device__ __forceinline__ void store_probs(uint16_t *to, int64_t lo, const float (&x)[32]) {
+__device__ __forceinline__ void pack32(const float (&x)[32], uint32_t *hi, uint32_t *lo) {
 #pragma unroll
-  for (int b = 0; b < 2; b++) {
-    uint32_t r[8], s[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-      const float u = x[b * 16 + 2 * i], v = x[b * 16 + 2 * i + 1];
-      r[i] = halves<BF16>(u, v);
-      if (LO) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&r[i]));
-        s[i] = halves<false>((u - f.x) * 2048.f, (v - f.y) * 2048.f);
-      }
+  for (int i = 0; i < 16; i++) {
+    hi[i] = halves<BF16>(x[2 * i], x[2 * i + 1]);
+    if (LO) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi[i]));
+      lo[i] = halves<false>((x[2 * i] - f.x) * 2048.f, (x[2 * i + 1] - f.y) * 2048.f);
     }
-    store32(to + b * 16, r);
-    if (LO) store32(to + lo + b * 16, s);
   }
 }
+
+// A warp's 32 rows of a strip, a row a lane, through shared memory to memory in one bulk copy of 4 KB.
+// Each row's eight 16-byte pieces are put in the order that the operands of a product have in shared
+// memory (piece j of row r at j ^ (r & 7)): no two lanes meet in a bank, and the loads need not swizzle.
+// A row a lane straight to memory would take 62 passes of the L1 for 1 KB, as many as the tensor cores'
+// own reads.
+__device__ __forceinline__ void put_strip(unsigned char *buffer, uint16_t *to, const uint32_t (&x)[32]) {
+  const int lane = threadIdx.x & 31;
+  if (lane == 0) bulk_wait_group_read<0>();   // the copy before this one has read the buffer
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < 8; j++)
+    *reinterpret_cast<uint4 *>(buffer + lane * 128 + ((j ^ (lane & 7)) * 16)) =
+        make_uint4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
+  async_proxy_fence();
+  __syncwarp();
+  if (lane == 0) {
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], 4096;" ::"l"(to), "r"(smem_addr(buffer))
+                 : "memory");
+    bulk_commit_group();
+  }
+}
+
+// Stages, and shared memory behind them: a strip's buffer for each warp that writes d.
+template <Use USE>
+constexpr int kProductStages = USE == kProbs ? 5 : 6;
+template <Use USE>
+constexpr int kProductSmem = smem_bytes(kProductStages<USE>, USE == kProbs ? 8 * 4096 : 0);
 
 template <Use USE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) product_kernel(const __grid_constant__ Product p) {
@@ -725,6 +743,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) prod
   __shared__ Pipe pipe;
   __shared__ RowCoef coef_s[2][USE == kProbs ? kM : 1];
   volatile int *gave_up = &pipe.gave_up;
+  constexpr int STAGES = kProductStages<USE>;
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
   const uint32_t tmem = pair_begin(pipe);
   const int rank = (int)cluster_rank(), pair = blockIdx.x / 2, npairs = gridDim.x / 2;
@@ -735,7 +754,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) prod
 
   if (warp == 0) {
     if (elected()) {
-      Ring ring{pipe, smem, gave_up};
+      Ring<STAGES> ring{pipe, smem, gave_up};
       bool ok = true;
       for (int t = pair; ok && t < tiles; t += npairs) {
         const int row = p.a_y + first_row(t), col = p.b_y + column_tile(t) * kN + rank * (kN / 2);
@@ -753,7 +772,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) prod
     __syncwarp();
   } else if (warp == 1) {
     if (rank == 0 && elected()) {
-      Issue issue{pipe, gave_up, tmem, smem_addr(smem)};
+      Issue<STAGES> issue{pipe, gave_up, tmem, smem_addr(smem)};
       bool ok = true;
       const uint32_t idesc = mma_desc(p.bf16, false, false, kPairM, kN);
       const uint64_t da = issue.desc(0, false), db = issue.desc(kBytesA, false);
@@ -763,7 +782,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) prod
         bool add = false;
         for (int q = 0; ok && q < p.pairs; q++)
           for (int kb = 0; ok && kb < p.kblocks; kb++) {
-            ok = issue.block<false>(d, da, db, 2, 2, idesc, add, kb == p.kblocks - 1 ? p.k16 : kK / 16);
+            ok = issue.template block<false>(d, da, db, 2, 2, idesc, add, kb == p.kblocks - 1 ? p.k16 : kK / 16);
             add = true;
           }
         if (ok) issue.end();
@@ -858,33 +877,42 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) prod
         if (lane == 0) mbar_arrive_leader(smem_addr(&pipe.hempty[reader.local & 1]));
         reader.begin();
         const int *y = p.targets + r * p.labels;
-        for (int ch = half; ch < kN / 32; ch += 2) {
-          float x[32];
-          reader.fetch(ch * 32, x);
+        unsigned char *buffer = smem + STAGES * kBytesStage + (warp - 4) * 4096;
+        for (int strip = 2 * half; strip < 2 * half + 2; strip++) {
+          uint32_t hi[32], lo[32];
 #pragma unroll
-          for (int i = 0; i < 32; i++) x[i] = exp2_fast(fmaf(x[i], c, -rc.lse2)) * rc.coef;
-          if (left < kN) {
+          for (int b = 0; b < 2; b++) {
+            const int ch = 2 * strip + b;
+            float x[32];
+            reader.fetch(ch * 32, x);
 #pragma unroll
-            for (int i = 0; i < 32; i++)
-              if (ch * 32 + i >= left) x[i] = 0.f;
+            for (int i = 0; i < 32; i++) x[i] = exp2_fast(fmaf(x[i], c, -rc.lse2)) * rc.coef;
+            if (left < kN) {
+#pragma unroll
+              for (int i = 0; i < 32; i++)
+                if (ch * 32 + i >= left) x[i] = 0.f;
+            }
+            if (__any_sync(kFullMask, rc.hits >> ch & 1)) {
+              if (rc.hits >> ch & 1)
+                for (int j = 0; j < p.labels; j++) {
+                  const int64_t at = y[j] - first - ch * 32;
+#pragma unroll
+                  for (int i = 0; i < 32; i++) x[i] -= at == i ? rc.g : 0.f;
+                }
+              __syncwarp();
+            }
+            if (p.bf16) pack32<true, false>(x, hi + 16 * b, nullptr);
+            else if (p.prob_lo) pack32<false, true>(x, hi + 16 * b, lo + 16 * b);
+            else pack32<false, false>(x, hi + 16 * b, nullptr);
           }
-          if (__any_sync(kFullMask, rc.hits >> ch & 1)) {
-            if (rc.hits >> ch & 1)
-              for (int j = 0; j < p.labels; j++) {
-                const int64_t at = y[j] - first - ch * 32;
-#pragma unroll
-                for (int i = 0; i < 32; i++) x[i] -= at == i ? rc.g : 0.f;
-              }
-            __syncwarp();
-          }
-          uint16_t *to = p.probs + ((int64_t)(n * (kN / 64) + ch / 2) * p.strip + r) * 64 + ch % 2 * 32;
-          if (p.bf16) store_probs<true, false>(to, 0, x);
-          else if (p.prob_lo) store_probs<false, true>(to, p.prob_lo, x);
-          else store_probs<false, false>(to, 0, x);
+          uint16_t *to = p.probs + ((int64_t)(n * (kN / 64) + strip) * p.strip + r - lane) * 64;
+          put_strip(buffer, to, hi);
+          if (p.prob_lo) put_strip(buffer, to + p.prob_lo, lo);
         }
       }
       reader.end();
     }
+    if (USE == kProbs && lane == 0) bulk_wait_group_all();
   }
   pair_end(tmem);
 }
@@ -1042,6 +1070,8 @@ __device__ __forceinline__ void put_tile(const Gradients &g, const Side &s, int6
   __syncwarp();
 }
 
+constexpr int kGradSmem = smem_bytes(kMostStages, 0);
+
 template <bool SEGMENTS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) grad_kernel(const __grid_constant__ Gradients g) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
@@ -1057,7 +1087,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) grad
 
   if (warp == 0) {
     if (elected()) {
-      Ring ring{pipe, smem, gave_up};
+      Ring<kMostStages> ring{pipe, smem, gave_up};
       bool ok = true;
       // each CTA brings its own rows of d and half of the operand's columns
       const int half_n = g.ntile / 2, groups = (half_n + 63) / 64;
@@ -1086,7 +1116,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) grad
     __syncwarp();
   } else if (warp == 1) {
     if (rank == 0 && elected()) {
-      Issue issue{pipe, gave_up, tmem, smem_addr(smem)};
+      Issue<kMostStages> issue{pipe, gave_up, tmem, smem_addr(smem)};
       bool ok = true;
       while (ok && walk.next(p)) {
         const bool mn = g.side[p.side].a_mn;
@@ -1097,7 +1127,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) grad
           uint32_t d;
           if (!(ok = issue.begin(d))) break;
           const int blocks = g.pairs * (min(p.k1, k0 + g.segment) - k0);
-          for (int b = 0; ok && b < blocks; b++) ok = issue.block<true>(d, da, db, step_a, 2048 >> 4, idesc, b > 0, kK / 16);
+          for (int b = 0; ok && b < blocks; b++) ok = issue.template block<true>(d, da, db, step_a, 2048 >> 4, idesc, b > 0, kK / 16);
           if (ok) issue.end();
         }
       }
@@ -1252,14 +1282,17 @@ EncodeTiled encoder() {
   return fn;
 }
 
-// A matrix of 16-bit elements, `inner` a row, rows `ld` elements apart; boxes of 64 x box_rows.
-int tensor_map(CUtensorMap *map, const void *base, int64_t inner, int64_t rows, int64_t ld, int box_rows) {
+// A matrix of 16-bit elements, `inner` a row, rows `ld` elements apart; boxes of 64 x box_rows, which arrive with the
+// 128-byte swizzle of a product's operands unless they are `swizzled` in memory.
+int tensor_map(CUtensorMap *map, const void *base, int64_t inner, int64_t rows, int64_t ld, int box_rows,
+               bool swizzled = false) {
   const EncodeTiled encode = encoder();
   if (!encode) return (int)cudaErrorNotSupported;
   const cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)ld * 2};
   const cuuint32_t box[2] = {64, (cuuint32_t)box_rows}, ones[2] = {1, 1};
   const CUresult e = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void *>(base), dims, strides, box, ones,
-                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            swizzled ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return e == CUDA_SUCCESS ? 0 : (int)cudaErrorInvalidValue;
 }
@@ -1280,9 +1313,9 @@ int sm_pairs() { return std::max(1, device_sm_count() / 2); }
 
 template <Use USE>
 int launch_product(const Product &p, cudaStream_t s) {
-  const int err = allow_smem(product_kernel<USE>, kSmem);
+  const int err = allow_smem(product_kernel<USE>, kProductSmem<USE>);
   if (err) return err;
-  product_kernel<USE><<<2 * std::min(p.mt * p.nt, sm_pairs()), kMmaThreads, kSmem, s>>>(p);
+  product_kernel<USE><<<2 * std::min(p.mt * p.nt, sm_pairs()), kMmaThreads, kProductSmem<USE>, s>>>(p);
   count_launch(1);
   return (int)cudaGetLastError();
 }
@@ -1290,10 +1323,10 @@ int launch_product(const Product &p, cudaStream_t s) {
 template <typename T>
 int launch_gradients(const Gradients &g, cudaStream_t s) {
   constexpr bool split = sizeof(T) == 4;
-  const int err = allow_smem(grad_kernel<split>, kSmem);
+  const int err = allow_smem(grad_kernel<split>, kGradSmem);
   if (err) return err;
   const bool whole = g.side[0].whole || g.side[1].whole;
-  grad_kernel<split><<<2 * (whole ? g.npairs : g.sharers), kMmaThreads, kSmem, s>>>(g);
+  grad_kernel<split><<<2 * (whole ? g.npairs : g.sharers), kMmaThreads, kGradSmem, s>>>(g);
   count_launch(1);
   const int rest = g.side[0].rest(g.npairs) + g.side[1].rest(g.npairs);
   if (rest > 0 && g.sharers > 1) {
@@ -1316,7 +1349,7 @@ bool good_shape(const Shape &x) {
 
 constexpr int64_t kLossRows = 16384;            // rows whose parts are kept at a time
 constexpr int64_t kGradRows = 8192;             // rows of a piece of d
-constexpr int64_t kProbBytes = (int64_t)512 << 20;
+constexpr int64_t kProbBytes = (int64_t)256 << 20;
 constexpr int kSegment = 8;                     // fp32 gradients: blocks of K between two roundings
 
 int few_blocks(int64_t vocab) {
@@ -1569,7 +1602,7 @@ int run_grad(const Shape &x, const Layout &l, const void *h, int64_t ldh, const 
     Side &side = g.side[i];
     const Operand &o = i == 0 ? oh : ow;
     side.a_mn = i == 0;
-    err = tensor_map(&side.a, ws + l.probs, 64, (int64_t)strip_rows * (split ? 2 : 1), 64, side.a_mn ? 64 : kM);
+    err = tensor_map(&side.a, ws + l.probs, 64, (int64_t)strip_rows * (split ? 2 : 1), 64, side.a_mn ? 64 : kM, true);
     if (!err) err = tensor_map(&side.b, o.p, o.inner, o.rows, o.ld, 64);
     if (split) {   // (lo 2^11) (hi 2^-11), hi lo, hi hi
       side.pa[0] = strip_rows;
