@@ -95,6 +95,7 @@ class AdamW:
         n = len(self.params)
         self._sizes = [p.numel() for p in self.params]
         self._types = [p.dtype for p in self.params]
+        self._kinds = (C.c_int * n)(*[TYPES[t] for t in self._types])
         self._table = (_lib.W2VAdamwTensor * n)()
         for i, p in enumerate(self.params):
             self._table[i] = _lib.W2VAdamwTensor(
@@ -135,6 +136,13 @@ class AdamW:
             else (None, None)
         return given("m", sizes, dtype), given("v", sizes, dtype), *scales, int(state["t"])
 
+    def _like(self, tensors, sizes, what):
+        """Refuses tensors that are not contiguous ones of this device and these sizes (in few passes:
+        a model may have hundreds)."""
+        if list(map(torch.Tensor.numel, tensors)) != sizes or not all(map(torch.Tensor.is_contiguous, tensors)) \
+                or set(map(torch.Tensor.get_device, tensors)) != {self.device.index}:
+            raise ValueError(what)
+
     def step(self, grads, lrate: "float | torch.Tensor | None" = None):
         """One step.  ``grads``: a tensor for each parameter, same number of elements, contiguous, fp32
         or the parameter's type.  ``lrate`` replaces the option's: a number, or a one-element fp32
@@ -142,15 +150,15 @@ class AdamW:
         n = len(self._sizes)
         if len(grads) != n:
             raise ValueError(f"{len(grads)} gradients for {n} parameters")
-        dev, types = self.device, self._types
-        kinds = []
-        for g, size, t in zip(grads, self._sizes, types):
-            d = g.dtype
-            if d is not t and d is not torch.float32:
-                raise ValueError("a gradient is fp32 or of its parameter's type")
-            if g.numel() != size or g.device != dev or not g.is_contiguous():
-                raise ValueError("a gradient has its parameter's device and size and is contiguous")
-            kinds.append(TYPES[d])
+        dev = self.device
+        self._like(grads, self._sizes, "a gradient has its parameter's device and size and is contiguous")
+        types = [g.dtype for g in grads]
+        if types == self._types:
+            kinds = self._kinds
+        elif all(t is torch.float32 or t is p for t, p in zip(types, self._types)):
+            kinds = (C.c_int * n)(*[TYPES[t] for t in types])
+        else:
+            raise ValueError("a gradient is fp32 or of its parameter's type")
         o = self.opts
         rate, rate_ptr = o.lrate, None
         if isinstance(lrate, torch.Tensor):
@@ -162,7 +170,7 @@ class AdamW:
         opts = _lib.W2VAdamwOpts(rate, o.beta1, o.beta2, o.eps, o.wdecay)
         with on_device(dev):
             check(_lib.load().w2v_adamw_step(self._table, (C.c_void_p * n)(*[g.data_ptr() for g in grads]),
-                                             (C.c_int * n)(*kinds), n, o.bits, C.byref(opts), rate_ptr,
+                                             kinds, n, o.bits, C.byref(opts), rate_ptr,
                                              self._clock.data_ptr(), stream_of(dev)), "w2v_adamw_step")
 
     def moments(self, mout=None, vout=None):
@@ -180,9 +188,11 @@ class AdamW:
         if len(mout) != n or len(vout) != n:
             raise ValueError("mout and vout have a tensor for each parameter")
         dev = self.device
-        for x, k in zip([*mout, *vout], self._sizes * 2):
-            if x.dtype != torch.float32 or x.numel() != k or x.device != dev or not x.is_contiguous():
-                raise ValueError("mout and vout: contiguous fp32 tensors of the parameters' device and sizes")
+        what = "mout and vout: contiguous fp32 tensors of the parameters' device and sizes"
+        both = [*mout, *vout]
+        self._like(both, self._sizes * 2, what)
+        if any(x.dtype is not torch.float32 for x in both):
+            raise ValueError(what)
         with on_device(dev):
             check(_lib.load().w2v_adamw_moments(self._table, (C.c_void_p * n)(*[x.data_ptr() for x in mout]),
                                                 (C.c_void_p * n)(*[x.data_ptr() for x in vout]), n,

@@ -10,9 +10,9 @@
 // table in device memory: nothing has to be uploaded before a step, and a captured step holds
 // its own.
 //
-// Each operation is rounded on its own (no contraction to fused multiply-adds), so the result does
-// not depend on how a compiler groups them: next to the border of two 8-bit codes that would
-// change a stored moment by a whole step.
+// Each operation on the moments is rounded on its own (no contraction to fused multiply-adds), so the
+// result does not depend on how a compiler groups them: next to the border of two 8-bit codes that
+// would change a stored moment by a whole step.
 //
 // 8-bit moments.  A unit is also the block that shares a scale, the largest magnitude in it.  A
 // code is the leading bits of the fp32 number y = x / scale (0 < |y| <= 1), rounded to nearest
@@ -89,7 +89,8 @@ __device__ __forceinline__ void step8(float (&p)[8], const float (&g)[8], float 
     v[i] = __fadd_rn(__fmul_rn(v[i], c.b2), __fmul_rn(__fmul_rn(g[i], g[i]), c.ob2));
     root[i] = __fsqrt_rn(v[i]);
     const float d = __fadd_rn(__fmul_rn(root[i], c.rc2), c.eps);
-    p[i] = __fsub_rn(__fmul_rn(p[i], c.keep), __fdiv_rn(__fmul_rn(m[i], c.lrc1), d));
+    // the quotient reaches the parameter only, not a stored moment: two units in its last place will do
+    p[i] = __fsub_rn(__fmul_rn(p[i], c.keep), __fdividef(__fmul_rn(m[i], c.lrc1), d));
   }
 }
 
@@ -110,16 +111,20 @@ __device__ __forceinline__ float unit_scale(const float (&x)[8]) {
 template <bool SIGNED>
 __device__ __forceinline__ void encode8(const float (&x)[8], float scale, unsigned (&code)[2]) {
   constexpr int shift = SIGNED ? 20 : 19, top = SIGNED ? 127 : 255, offset = (kOne >> shift) - top;
-  const float r = scale > 0.f ? __fdiv_rn(1.f, scale) : 0.f;   // false for a NaN scale
   code[0] = code[1] = 0;
+  if (!(scale > 0.f)) return;   // all zero, or not finite: the scale says which
+  const float r = __fdiv_rn(1.f, scale);
 #pragma unroll
   for (int i = 0; i < 8; i++) {
-    const float y = __fmul_rn(x[i], r);
-    const int bits = __float_as_int(y) & 0x7fffffff;
-    int c = ((bits + ((1 << (shift - 1)) - 1) + ((bits >> shift) & 1)) >> shift) - offset;
-    c = min(max(c, SIGNED ? 0 : 1), top);
-    if (bits == 0 || !(scale > 0.f)) c = 0;
-    if (SIGNED && y < 0.f && c > 0) c |= 128;
+    // |y| <= 1 and a little more, which rounds to 1: the topmost code needs no clamp
+    const unsigned y = __float_as_uint(__fmul_rn(x[i], r));
+    const unsigned bits = SIGNED ? y & 0x7fffffffu : y;
+    int c = (int)((bits + ((1u << (shift - 1)) - 1u) + ((bits >> shift) & 1u)) >> shift) - offset;
+    if (SIGNED) {
+      c = c > 0 ? (int)((y >> 24 & 0x80u) | (unsigned)c) : 0;
+    } else {
+      c = max(c, bits != 0 ? 1 : 0);
+    }
     code[i >> 2] |= (unsigned)c << (8 * (i & 3));
   }
 }
@@ -129,11 +134,11 @@ __device__ __forceinline__ void decode8(const unsigned (&code)[2], float scale, 
   constexpr int shift = SIGNED ? 20 : 19, top = SIGNED ? 127 : 255, offset = (kOne >> shift) - top;
 #pragma unroll
   for (int i = 0; i < 8; i++) {
-    const int c = (code[i >> 2] >> (8 * (i & 3))) & 255;
-    const int low = SIGNED ? c & 127 : c;
-    float y = low > 0 ? __int_as_float((low + offset) << shift) : 0.f;
-    if (SIGNED && (c & 128)) y = -y;
-    x[i] = __fmul_rn(y, scale);
+    const unsigned c = __byte_perm(code[i >> 2], 0, 0x4440u | (unsigned)(i & 3));
+    const unsigned low = SIGNED ? c & 127u : c;
+    unsigned bits = (low << shift) + ((unsigned)offset << shift);
+    if (SIGNED) bits |= (c & 128u) << 24;
+    x[i] = low ? __fmul_rn(__uint_as_float(bits), scale) : __fmul_rn(0.f, scale);
   }
 }
 
@@ -170,6 +175,15 @@ __device__ __forceinline__ void put8(T *a, bool wide, int n, const float (&x)[8]
   else store_some(a, n, x);
 }
 
+// A warp works on consecutive units, so that it looks its tensor up once and again only at its end.
+struct Span {
+  int64_t begin, end;
+};
+__device__ __forceinline__ Span span_of(int64_t units) {
+  const int64_t warps = (int64_t)gridDim.x * (kThreads / 32), w = (int64_t)blockIdx.x * (kThreads / 32) + threadIdx.x / 32;
+  return Span{w * units / warps, (w + 1) * units / warps};
+}
+
 // The tensor that unit `u` belongs to.
 template <int CAP>
 __device__ __forceinline__ int tensor_of(const Table<CAP> &t, int64_t u) {
@@ -191,9 +205,10 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
   const Consts c = shared_consts;
   const int lane = threadIdx.x & 31;
   const int64_t units = t.first[t.count];
-  const int64_t stride = (int64_t)gridDim.x * (kThreads / 32);
-  for (int64_t u = (int64_t)blockIdx.x * (kThreads / 32) + threadIdx.x / 32; u < units; u += stride) {
-    const int k = tensor_of(t, u);
+  const Span span = span_of(units);
+  int k = span.begin < span.end ? tensor_of(t, span.begin) : 0;
+  for (int64_t u = span.begin; u < span.end; u++) {
+    while (u >= t.first[k + 1]) k++;
     const int64_t block = u - t.first[k];
     const int64_t at = block * kUnit + lane * 8;
     const int n = (int)min((int64_t)8, max((int64_t)0, t.n[k] - at));
@@ -254,9 +269,10 @@ template <int CAP>
 __global__ void __launch_bounds__(kThreads) moments_kernel(const __grid_constant__ Table<CAP> t) {
   const int lane = threadIdx.x & 31;
   const int64_t units = t.first[t.count];
-  const int64_t stride = (int64_t)gridDim.x * (kThreads / 32);
-  for (int64_t u = (int64_t)blockIdx.x * (kThreads / 32) + threadIdx.x / 32; u < units; u += stride) {
-    const int k = tensor_of(t, u);
+  const Span span = span_of(units);
+  int k = span.begin < span.end ? tensor_of(t, span.begin) : 0;
+  for (int64_t u = span.begin; u < span.end; u++) {
+    while (u >= t.first[k + 1]) k++;
     const int64_t block = u - t.first[k];
     const int64_t at = block * kUnit + lane * 8;
     const int n = (int)min((int64_t)8, max((int64_t)0, t.n[k] - at));
@@ -279,10 +295,14 @@ __global__ void clock_kernel(Clock *c, double b1t, double b2t) { *c = Clock{b1t,
 bool aligned(const void *a, size_t to) { return reinterpret_cast<uintptr_t>(a) % to == 0; }
 size_t type_size(int type) { return type == W2V_F32 ? 4 : 2; }
 
+// Blocks: as many as fit on the SMs, and up to eight times that as long as each warp has eight units left
+// (each block begins with a few hundred clocks of constants in 64 bits, but many short ones use the
+// memory better than few long ones: 51 million elements in 224 us against 245).
 int grid_for(int64_t units) {
-  // four blocks of eight warps an SM keep 32 KB in flight there with fp32 moments
-  const int64_t need = (units + kThreads / 32 - 1) / (kThreads / 32);
-  return (int)std::max<int64_t>(1, std::min<int64_t>(need, (int64_t)w2v::device_sm_count() * 8));
+  constexpr int warps = kThreads / 32;
+  const int64_t fit = (int64_t)w2v::device_sm_count() * 4, need = (units + warps - 1) / warps;
+  const int64_t most = std::min<int64_t>(fit * 8, units / (warps * 8));
+  return (int)std::max<int64_t>(1, std::min(need, std::max(fit, most)));
 }
 
 template <typename PT, typename GT, int CAP>

@@ -33,22 +33,37 @@ __device__ __forceinline__ void store8(float *a, const float (&x)[8]) {
                "f"(x[2]), "f"(x[3]), "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7])
                : "memory");
 }
+// Two 16-bit values in a word.
+__device__ __forceinline__ void unpack2(uint32_t w, float &a, float &b, __nv_bfloat16) {
+  a = __uint_as_float(w << 16);
+  b = __uint_as_float(w & 0xffff0000u);
+}
+__device__ __forceinline__ void unpack2(uint32_t w, float &a, float &b, __half) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w));
+  a = f.x;
+  b = f.y;
+}
+__device__ __forceinline__ uint32_t packed2(float a, float b, __nv_bfloat16) {
+  const __nv_bfloat162 p = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&p);
+}
+__device__ __forceinline__ uint32_t packed2(float a, float b, __half) {
+  const __half2 p = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&p);
+}
 template <typename T>
 __device__ __forceinline__ void load8(const T *a, float (&x)[8]) {
   static_assert(sizeof(T) == 2, "a 16-bit type");
   const uint4 raw = *reinterpret_cast<const uint4 *>(a);
-  const T *e = reinterpret_cast<const T *>(&raw);
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-  for (int i = 0; i < 8; i++) x[i] = to_float(e[i]);
+  for (int i = 0; i < 4; i++) unpack2(w[i], x[2 * i], x[2 * i + 1], T());
 }
 template <typename T>
 __device__ __forceinline__ void store8(T *a, const float (&x)[8]) {
   static_assert(sizeof(T) == 2, "a 16-bit type");
-  uint4 raw;
-  T *e = reinterpret_cast<T *>(&raw);
-#pragma unroll
-  for (int i = 0; i < 8; i++) e[i] = from_float<T>(x[i]);
-  *reinterpret_cast<uint4 *>(a) = raw;
+  *reinterpret_cast<uint4 *>(a) = make_uint4(packed2(x[0], x[1], T()), packed2(x[2], x[3], T()), packed2(x[4], x[5], T()),
+                                             packed2(x[6], x[7], T()));
 }
 
 // The first `n` of 8 elements, one at a time: any alignment; the others read as zero.
