@@ -26,7 +26,8 @@ SOURCES = ["w2v_kernels.cu", "w2v_batch.cu", "w2v_noalloc.cu", "w2v_exchange.cu"
 # measuring aid of bench.py, a library of its own: nothing of it is in the C-ABI library
 PROBE_SOURCE = "bench_rowprobe.cu"
 PROBE_LIB_PATH = os.path.join(PKG, "libw2vrowprobe.so")
-HEADERS = ["w2v_device.cuh", "w2v_internal.h", "w2v_rows.cuh", "w2v_types.cuh", "w2v_tcgen05.cuh", "jni_min.h",
+HEADERS = ["w2v_device.cuh", "w2v_internal.h", "w2v_rows.cuh", "w2v_types.cuh", "w2v_tcgen05.cuh", "w2v_chain.cuh",
+           "jni_min.h",
            os.path.join("..", "..", "include", "bidmach_b200.h")]
 
 NVCC_FLAGS = [

@@ -15,14 +15,17 @@
 #include <algorithm>
 
 #include "../../include/bidmach_b200.h"
+#include "w2v_chain.cuh"
 #include "w2v_device.cuh"
 #include "w2v_internal.h"
 #include "w2v_types.cuh"
 
 namespace {
 
+using w2v::chain_wait;
 using w2v::from_float;
 using w2v::kFullMask;
+using w2v::launch_chained;
 
 constexpr int kThreads = 256;
 constexpr int kMostChunk = 32;      // sorted tokens a warp walks, one a lane while their ids are looked up
@@ -39,6 +42,7 @@ __device__ __forceinline__ uint4 load_once(const void *a) {
 template <typename T, int G>
 __global__ void __launch_bounds__(kThreads) rows_kernel(const int *ids, int64_t n, const T *m, int64_t ldm,
                                                         int64_t vocab, int dim, T *out, int64_t ldo, int each) {
+  chain_wait();
   constexpr int per = 16 / sizeof(T);
   const int lane = threadIdx.x & 31;
   const int64_t r0 = ((int64_t)blockIdx.x * (kThreads / 32) + threadIdx.x / 32) * each;
@@ -74,6 +78,7 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const int *ids, int64_t 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) rows_any_kernel(const int *ids, int64_t n, const T *m, int64_t ldm,
                                                             int64_t vocab, int dim, T *out, int64_t ldo) {
+  chain_wait();
   const int lane = threadIdx.x & 31;
   const int64_t stride = (int64_t)gridDim.x * (kThreads / 32);
   for (int64_t i = (int64_t)blockIdx.x * (kThreads / 32) + threadIdx.x / 32; i < n; i += stride) {
@@ -91,6 +96,7 @@ __device__ __forceinline__ int key_of(int id, int vocab) { return id >= 0 && id 
 
 __global__ void __launch_bounds__(kThreads) keys_kernel(const int *ids, int n, int vocab, int *keys, int *order,
                                                         int *nowners) {
+  chain_wait();
   const int i = blockIdx.x * kThreads + threadIdx.x;
   if (i == 0) *nowners = 0;
   if (i >= n) return;
@@ -105,6 +111,7 @@ __global__ void __launch_bounds__(THREADS) small_sort_kernel(const int *ids, int
   using Sort = cub::BlockRadixSort<int, THREADS, 8, int, 5>;
   __shared__ typename Sort::TempStorage temp;
   int key[8], at[8];
+  chain_wait();
 #pragma unroll
   for (int j = 0; j < 8; j++) {
     at[j] = threadIdx.x * 8 + j;
@@ -179,6 +186,7 @@ __device__ __forceinline__ void get_part(const float *a, float (&x)[VEC]) {
 template <typename T, int VEC, int G>
 __global__ void __launch_bounds__(kThreads) runs_kernel(const Runs r, const T *grad, int64_t ldg, T *out, int64_t ldo) {
   const int chunk = blockIdx.x * (kThreads / 32) + threadIdx.x / 32, lane = threadIdx.x & 31;
+  chain_wait();
   if (chunk >= r.chunks) return;
   const int lo = chunk * r.chunk, cnt = min(r.chunk, r.n - lo);
   const int my_key = lane < cnt ? r.keys[lo + lane] : -1;
@@ -272,6 +280,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Runs r, T *out
   constexpr int warps = kJoinThreads / 32;
   __shared__ float sums[warps][32 * VEC + 1];
   __shared__ int longer[warps], nlonger, count_s;
+  chain_wait();
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, owners = *r.nowners;
   const int c = blockIdx.y * 32 * VEC + lane * VEC;
   for (int64_t k0 = blockIdx.x; k0 < owners; k0 += (int64_t)gridDim.x * warps) {
@@ -393,34 +402,28 @@ int run_rows(const int *ids, int64_t n, const void *m, int64_t ldm, int64_t voca
     const int each = (int)std::max<int64_t>(2, std::min<int64_t>(32, n / (w2v::device_sm_count() * 64) / 2 * 2));
     const int64_t block = (int64_t)each * (kThreads / 32);
     const dim3 grid((unsigned)((n + block - 1) / block), (groups + 3) / 4);
-    if (groups == 1) rows_kernel<T, 1><<<grid, kThreads, 0, s>>>(ids, n, src, ldm, vocab, dim, dst, ldo, each);
-    else if (groups == 2) rows_kernel<T, 2><<<grid, kThreads, 0, s>>>(ids, n, src, ldm, vocab, dim, dst, ldo, each);
-    else if (groups == 3) rows_kernel<T, 3><<<grid, kThreads, 0, s>>>(ids, n, src, ldm, vocab, dim, dst, ldo, each);
-    else rows_kernel<T, 4><<<grid, kThreads, 0, s>>>(ids, n, src, ldm, vocab, dim, dst, ldo, each);
-  } else {
-    const int64_t need = (n + kThreads / 32 - 1) / (kThreads / 32);
-    const int grid = (int)std::min<int64_t>(need, (int64_t)w2v::device_sm_count() * 32);
-    rows_any_kernel<T><<<grid, kThreads, 0, s>>>(ids, n, src, ldm, vocab, dim, dst, ldo);
+    const auto k = groups == 1 ? rows_kernel<T, 1> : groups == 2 ? rows_kernel<T, 2> : groups == 3 ? rows_kernel<T, 3>
+                                                                                           : rows_kernel<T, 4>;
+    return launch_chained(k, grid, kThreads, 0, s, ids, n, src, ldm, vocab, dim, dst, ldo, each);
   }
-  w2v::count_launch(1);
-  return (int)cudaGetLastError();
+  const int64_t need = (n + kThreads / 32 - 1) / (kThreads / 32);
+  const int grid = (int)std::min<int64_t>(need, (int64_t)w2v::device_sm_count() * 32);
+  return launch_chained(rows_any_kernel<T>, grid, kThreads, 0, s, ids, n, src, ldm, vocab, dim, dst, ldo);
 }
 
 template <typename T, int VEC>
-void run_runs(const Runs &r, const T *g, int64_t ldg, T *o, int64_t ldo, cudaStream_t s) {
+int run_runs(const Runs &r, const T *g, int64_t ldg, T *o, int64_t ldo, cudaStream_t s) {
   const int groups = (r.dim + 32 * VEC - 1) / (32 * VEC);
   constexpr int most = VEC == 8 ? 2 : 4;
   const dim3 grid((r.chunks + kThreads / 32 - 1) / (kThreads / 32), (groups + most - 1) / most);
-  if (groups == 1) runs_kernel<T, VEC, 1><<<grid, kThreads, 0, s>>>(r, g, ldg, o, ldo);
-  else if (groups == 2 || most == 2) runs_kernel<T, VEC, 2><<<grid, kThreads, 0, s>>>(r, g, ldg, o, ldo);
-  else if (groups == 3) runs_kernel<T, VEC, most == 2 ? 2 : 3><<<grid, kThreads, 0, s>>>(r, g, ldg, o, ldo);
-  else runs_kernel<T, VEC, most><<<grid, kThreads, 0, s>>>(r, g, ldg, o, ldo);
-  if (r.chunks < 2) {
-    w2v::count_launch(1);
-    return;
-  }
-  join_kernel<T, VEC><<<dim3(std::min(r.chunks / 2, w2v::device_sm_count() * 2), groups), kJoinThreads, 0, s>>>(r, o, ldo);
-  w2v::count_launch(2);
+  const auto k = groups == 1   ? runs_kernel<T, VEC, 1>
+                 : groups == 2 ? runs_kernel<T, VEC, 2>
+                 : groups == 3 ? runs_kernel<T, VEC, most == 2 ? 2 : 3>
+                               : runs_kernel<T, VEC, most>;
+  const int err = launch_chained(k, grid, kThreads, 0, s, r, g, ldg, o, ldo);
+  if (err || r.chunks < 2) return err;
+  return launch_chained(join_kernel<T, VEC>, dim3(std::min(r.chunks / 2, w2v::device_sm_count() * 2), groups), kJoinThreads,
+                        0, s, r, o, ldo);
 }
 
 template <typename T>
@@ -433,22 +436,22 @@ int run_grad(const Layout &l, const int *ids, int n, const void *grad, int64_t l
   cudaError_t e = ldo == dim ? cudaMemsetAsync(out, 0, (size_t)vocab * dim * sizeof(T), s)
                              : cudaMemset2DAsync(out, ldo * sizeof(T), 0, dim * sizeof(T), vocab, s);
   if (e != cudaSuccess || n == 0) return (int)e;
+  int err = 0;
   if (n <= 128 * 8) {
-    small_sort_kernel<128><<<1, 128, 0, s>>>(ids, n, vocab, l.bits, keys, order, r.nowners);
+    err = launch_chained(small_sort_kernel<128>, 1, 128, 0, s, ids, n, vocab, l.bits, keys, order, r.nowners);
   } else if (n <= kSmallSort) {
-    small_sort_kernel<512><<<1, 512, 0, s>>>(ids, n, vocab, l.bits, keys, order, r.nowners);
+    err = launch_chained(small_sort_kernel<512>, 1, 512, 0, s, ids, n, vocab, l.bits, keys, order, r.nowners);
   } else {
-    keys_kernel<<<(n + kThreads - 1) / kThreads, kThreads, 0, s>>>(ids, n, vocab, keys_in, order_in, r.nowners);
+    err = launch_chained(keys_kernel, (n + kThreads - 1) / kThreads, kThreads, 0, s, ids, n, vocab, keys_in, order_in, r.nowners);
     size_t bytes = l.sort_bytes;
-    e = cub::DeviceRadixSort::SortPairs(ws + l.sort, bytes, keys_in, keys, order_in, order, n, 0, l.bits, s);
-    if (e != cudaSuccess) return (int)e;
+    if (!err)
+      err = (int)cub::DeviceRadixSort::SortPairs(ws + l.sort, bytes, keys_in, keys, order_in, order, n, 0, l.bits, s);
   }
-  w2v::count_launch(1);
+  if (err) return err;
   const T *g = static_cast<const T *>(grad);
   T *o = static_cast<T *>(out);
-  if (pieces<T>(g, ldg, dim) && pieces<T>(o, ldo, dim)) run_runs<T, 16 / sizeof(T)>(r, g, ldg, o, ldo, s);
-  else run_runs<T, 1>(r, g, ldg, o, ldo, s);
-  return (int)cudaGetLastError();
+  if (pieces<T>(g, ldg, dim) && pieces<T>(o, ldo, dim)) return run_runs<T, 16 / sizeof(T)>(r, g, ldg, o, ldo, s);
+  return run_runs<T, 1>(r, g, ldg, o, ldo, s);
 }
 
 }  // namespace

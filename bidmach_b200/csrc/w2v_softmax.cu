@@ -28,6 +28,7 @@
 #include <algorithm>
 
 #include "../../include/bidmach_b200.h"
+#include "w2v_chain.cuh"
 #include "w2v_device.cuh"
 #include "w2v_internal.h"
 #include "w2v_tcgen05.cuh"
@@ -154,6 +155,7 @@ __global__ void __launch_bounds__(kFewThreads) few_loss_kernel(const T *h, int64
                                                                int64_t vocab, int dim, bool wide, Part *parts) {
   extern __shared__ __align__(16) float sh[];
   __shared__ Part sums[kFewThreads / 32][RB];
+  chain_wait();
   stage_rows<T, RB>(h, ldh, rows, dim, sh);
   __syncthreads();
   constexpr int M = kFewWords * RB, each = 32 / M;
@@ -192,6 +194,7 @@ __global__ void __launch_bounds__(kFewThreads) few_grad_kernel(const T *h, int64
   extern __shared__ __align__(16) float sh[];
   __shared__ float lse_s[RB], g_s[RB], k_s[RB];
   __shared__ __align__(16) float d_s[kFewThreads / 32][RB][kFewWords];
+  chain_wait();
   stage_rows<T, RB>(h, ldh, rows, dim, sh);
   if (threadIdx.x < RB) {
     const int r = threadIdx.x;
@@ -253,6 +256,7 @@ __global__ void __launch_bounds__(kFewThreads) few_grad_kernel(const T *h, int64
 template <typename T, int RB>
 __global__ void __launch_bounds__(kFewThreads) few_dh_kernel(const T *w, int64_t ldw, int64_t vocab, int dim,
                                                              const float *d, float *parts) {
+  chain_wait();
   const int64_t each = (vocab + gridDim.x - 1) / gridDim.x;
   const int64_t lo = blockIdx.x * each, hi = min(vocab, lo + each);
   for (int c = blockIdx.y * kFewThreads + threadIdx.x; c < dim; c += gridDim.y * kFewThreads) {
@@ -301,6 +305,7 @@ __device__ __forceinline__ float rescale_of(const Rescale &r) {
 template <typename T>
 __global__ void __launch_bounds__(256) slabs_kernel(const float *slabs, int count, int64_t slab, int64_t rows, int dim,
                                                     T *out, int64_t ldo) {
+  chain_wait();
   const int lane = threadIdx.x & 31;
   const int64_t cols = (dim + 31) / 32, i = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
   if (i >= rows * cols) return;
@@ -333,6 +338,7 @@ __global__ void __launch_bounds__(kJoinThreads) loss_join_kernel(const Part *par
                                                                  int64_t vocab, int dim, bool wide, const int *targets,
                                                                  int labels, float *loss, float *lse) {
   __shared__ Part sums[kJoinThreads / 32][kJoinRows];
+  chain_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x / 32, warps = kJoinThreads / 32;
   const int r0 = blockIdx.x * kJoinRows, here = min(kJoinRows, rows - r0);
   Part p{-INFINITY, 0.f};
@@ -417,6 +423,7 @@ __device__ __forceinline__ void block_max(unsigned top, unsigned *to) {
 // Largest magnitudes of fp32 operands (z = 0: H, 1: W) and of the rows' g_n k_n (z = 2).
 __global__ void __launch_bounds__(256) amax_kernel(Source h, Source w, int dim, const float *gloss,
                                                    const int *targets, int labels, int64_t vocab, Scalars *sc) {
+  chain_wait();
   unsigned top = 0;
   if (blockIdx.z < 2) {
     const Source s = blockIdx.z == 0 ? h : w;
@@ -478,6 +485,7 @@ __device__ __forceinline__ void stage_row<float>(const float *src, int dim, floa
 template <typename T>
 __global__ void __launch_bounds__(256) stage_kernel(Source h, Source w, int dim, void *hs, void *ws, int width, int parts,
                                                     const Scalars *sc) {
+  chain_wait();
   const Source s = blockIdx.z == 0 ? h : w;
   void *to = blockIdx.z == 0 ? hs : ws;
   if (!to) return;
@@ -531,6 +539,7 @@ __device__ __forceinline__ uint32_t pair_begin(Pipe &s) {
   tmem_before_sync();
   cluster_sync();
   tmem_after_sync();
+  chain_wait();
   return s.tmem;
 }
 // Neither CTA leaves while the other's products read its shared memory or its barriers are arrived on.
@@ -1210,6 +1219,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) grad
 // The tiles that were cut: blockIdx.x is the tile in what is left, a warp a row.
 template <typename T>
 __global__ void __launch_bounds__(256) pieces_kernel(const __grid_constant__ Gradients g) {
+  chain_wait();
   const int t = blockIdx.x, rest0 = g.side[0].rest(g.npairs);
   const Side &s = g.side[t >= rest0];
   const int64_t begin = t < rest0 ? (int64_t)t * (g.side[0].kblocks + kReading)
@@ -1315,25 +1325,19 @@ template <Use USE>
 int launch_product(const Product &p, cudaStream_t s) {
   const int err = allow_smem(product_kernel<USE>, kProductSmem<USE>);
   if (err) return err;
-  product_kernel<USE><<<2 * std::min(p.mt * p.nt, sm_pairs()), kMmaThreads, kProductSmem<USE>, s>>>(p);
-  count_launch(1);
-  return (int)cudaGetLastError();
+  return launch_chained(product_kernel<USE>, 2 * std::min(p.mt * p.nt, sm_pairs()), kMmaThreads, kProductSmem<USE>, s, p);
 }
 
 template <typename T>
 int launch_gradients(const Gradients &g, cudaStream_t s) {
   constexpr bool split = sizeof(T) == 4;
-  const int err = allow_smem(grad_kernel<split>, kGradSmem);
+  int err = allow_smem(grad_kernel<split>, kGradSmem);
   if (err) return err;
   const bool whole = g.side[0].whole || g.side[1].whole;
-  grad_kernel<split><<<2 * (whole ? g.npairs : g.sharers), kMmaThreads, kGradSmem, s>>>(g);
-  count_launch(1);
+  err = launch_chained(grad_kernel<split>, 2 * (whole ? g.npairs : g.sharers), kMmaThreads, kGradSmem, s, g);
   const int rest = g.side[0].rest(g.npairs) + g.side[1].rest(g.npairs);
-  if (rest > 0 && g.sharers > 1) {
-    pieces_kernel<T><<<dim3(rest, kPairM / 8), 256, 0, s>>>(g);
-    count_launch(1);
-  }
-  return (int)cudaGetLastError();
+  if (!err && rest > 0 && g.sharers > 1) err = launch_chained(pieces_kernel<T>, dim3(rest, kPairM / 8), 256, 0, s, g);
+  return err;
 }
 
 struct Shape {
@@ -1436,19 +1440,19 @@ int stage(const Shape &x, const Layout &l, const void *h, int64_t ldh, const voi
     const cudaError_t e = cudaMemsetAsync(sc, 0, sizeof(Scalars), s);
     if (e != cudaSuccess) return (int)e;
     const Source none{nullptr, 0, x.n};
-    amax_kernel<<<dim3(split ? blocks : 64, 1, 3), 256, 0, s>>>(split ? sh : none, split ? sw : Source{nullptr, 0, 0},
-                                                                 x.dim, gloss, targets, x.labels, x.vocab, sc);
-    count_launch(1);
+    const int err = launch_chained(amax_kernel, dim3(split ? blocks : 64, 1, 3), 256, 0, s, split ? sh : none,
+                                   split ? sw : Source{nullptr, 0, 0}, x.dim, gloss, targets, x.labels, x.vocab, sc);
+    if (err) return err;
   }
   void *hs = direct<T>(h, ldh) ? nullptr : ws + l.hs, *wst = direct<T>(w, ldw) ? nullptr : ws + l.ws;
   if (hs || wst) {
-    stage_kernel<T><<<dim3(blocks, 1, 2), 256, 0, s>>>(sh, sw, x.dim, hs, wst, l.width, l.nparts, sc);
-    count_launch(1);
+    const int err = launch_chained(stage_kernel<T>, dim3(blocks, 1, 2), 256, 0, s, sh, sw, x.dim, hs, wst, l.width, l.nparts, sc);
+    if (err) return err;
   }
   const int64_t staged = (int64_t)l.width * l.nparts;
   *oh = hs ? Operand{hs, staged, staged, x.n, l.width} : Operand{h, ldh, x.dim, x.n, 0};
   *ow = wst ? Operand{wst, staged, staged, x.vocab, l.width} : Operand{w, ldw, x.dim, x.vocab, 0};
-  return (int)cudaGetLastError();
+  return 0;
 }
 
 template <typename T>
@@ -1481,10 +1485,8 @@ int few_loss(const Shape &x, const Layout &l, const void *h, int64_t ldh, const 
   if (e != cudaSuccess) return (int)e;
   const bool wide = aligned(w, 8 * sizeof(T)) && ldw % 8 == 0;
   *count = few_blocks(x.vocab);
-  k<<<*count, kFewThreads, smem, s>>>(static_cast<const T *>(h), ldh, (int)x.n, static_cast<const T *>(w), ldw, x.vocab,
-                                      x.dim, wide, reinterpret_cast<Part *>(ws + l.parts));
-  count_launch(1);
-  return (int)cudaGetLastError();
+  return launch_chained(k, *count, kFewThreads, smem, s, static_cast<const T *>(h), ldh, (int)x.n,
+                        static_cast<const T *>(w), ldw, x.vocab, x.dim, wide, reinterpret_cast<Part *>(ws + l.parts));
 }
 
 template <typename T>
@@ -1493,11 +1495,9 @@ int run_loss(const Shape &x, const Layout &l, const void *h, int64_t ldh, const 
   Part *parts = reinterpret_cast<Part *>(ws + l.parts);
   const bool wide = aligned(h, 8 * sizeof(T)) && ldh % 8 == 0 && aligned(w, 8 * sizeof(T)) && ldw % 8 == 0;
   auto join_rows = [&](int count, int64_t ldp, int64_t r0, int rows) {
-    loss_join_kernel<T><<<(rows + kJoinRows - 1) / kJoinRows, kJoinThreads, 0, s>>>(
-        parts, count, ldp, rows, static_cast<const T *>(h) + r0 * ldh, ldh, static_cast<const T *>(w), ldw, x.vocab,
-        x.dim, wide, targets + r0 * x.labels, x.labels, loss + r0, lse + r0);
-    count_launch(1);
-    return (int)cudaGetLastError();
+    return launch_chained(loss_join_kernel<T>, (rows + kJoinRows - 1) / kJoinRows, kJoinThreads, 0, s, parts, count, ldp,
+                          rows, static_cast<const T *>(h) + r0 * ldh, ldh, static_cast<const T *>(w), ldw, x.vocab, x.dim,
+                          wide, targets + r0 * x.labels, x.labels, loss + r0, lse + r0);
   };
   if (x.n <= kFewRows) {
     int count = 0, err = 0;
@@ -1540,15 +1540,16 @@ int few_grad(const Shape &x, const Layout &l, const void *h, int64_t ldh, const 
   const bool wide = aligned(w, 8 * sizeof(T)) && ldw % 8 == 0, wout = aligned(dw, 8 * sizeof(T)) && lddw % 8 == 0;
   float *d = reinterpret_cast<float *>(ws + l.probs), *acc = reinterpret_cast<float *>(ws + l.acc_h);
   const T *wt = static_cast<const T *>(w);
-  k<<<few_blocks(x.vocab), kFewThreads, smem, s>>>(static_cast<const T *>(h), ldh, (int)x.n, wt, ldw, x.vocab, x.dim, wide,
-                                                   targets, x.labels, lse, gloss, ldg, static_cast<T *>(dw), lddw, wout, d);
+  int err = launch_chained(k, few_blocks(x.vocab), kFewThreads, smem, s, static_cast<const T *>(h), ldh, (int)x.n, wt, ldw,
+                           x.vocab, x.dim, wide, targets, x.labels, lse, gloss, ldg, static_cast<T *>(dw), lddw, wout, d);
   const int blocks = few_dh_blocks(x.vocab);
-  few_dh_kernel<T, RB><<<dim3(blocks, (x.dim + kFewThreads - 1) / kFewThreads), kFewThreads, 0, s>>>(wt, ldw, x.vocab,
-                                                                                                    x.dim, d, acc);
-  slabs_kernel<T><<<(int)((x.n * ((x.dim + 31) / 32) + 7) / 8), 256, 0, s>>>(acc, blocks, (int64_t)RB * x.dim, x.n, x.dim,
-                                                                           static_cast<T *>(dh), lddh);
-  count_launch(3);
-  return (int)cudaGetLastError();
+  if (!err)
+    err = launch_chained(few_dh_kernel<T, RB>, dim3(blocks, (x.dim + kFewThreads - 1) / kFewThreads), kFewThreads, 0, s, wt,
+                         ldw, x.vocab, x.dim, d, acc);
+  if (!err)
+    err = launch_chained(slabs_kernel<T>, (unsigned)((x.n * ((x.dim + 31) / 32) + 7) / 8), 256, 0, s, acc, blocks,
+                         (int64_t)RB * x.dim, x.n, x.dim, static_cast<T *>(dh), lddh);
+  return err;
 }
 
 template <typename T>
