@@ -118,6 +118,8 @@ SIGNATURES = {
     "w2v_set_timing": (_I, [_P, _I]),
     "w2v_get_timing": (_I, [_P, C.POINTER(W2VTiming)]),
     "w2v_launch_count": (C.c_longlong, []),
+    "w2v_window_rows_workspace": (C.c_int64, [_I]),
+    "w2v_window_rows": (_I, [_P, _P, _P, _I, _I, _P, _P, _P, _P, C.c_int64, _P]),
     "w2v_softmax_workspace": (C.c_int64, [C.c_int64, C.c_int64, _I, _I, _I, _I]),
     "w2v_softmax_loss": (_I, [_P, C.c_int64, _P, C.c_int64, _P, C.c_int64, C.c_int64, _I, _I, _I, _P, _P, _P,
                               C.c_int64, _P]),

@@ -22,7 +22,8 @@ LIB_PATH = os.path.join(PKG, LIB_NAME)
 OBJ_DIR = os.path.join(HERE, "build")
 
 SOURCES = ["w2v_kernels.cu", "w2v_batch.cu", "w2v_noalloc.cu", "w2v_exchange.cu", "w2v_adamw.cu",
-           "w2v_embed.cu", "w2v_softmax.cu", "jni_shim.cpp", "matio_codec.cpp"]
+           "w2v_embed.cu", "w2v_softmax.cu", "w2v_windows.cu",
+           "jni_shim.cpp", "matio_codec.cpp"]
 # measuring aid of bench.py, a library of its own: nothing of it is in the C-ABI library
 PROBE_SOURCE = "bench_rowprobe.cu"
 PROBE_LIB_PATH = os.path.join(PKG, "libw2vrowprobe.so")

@@ -18,7 +18,10 @@ import numpy as np
 import torch
 
 from . import _lib, modelio
+from .adamw import AdamW
 from .cumach import CUMACH, CUMACHSlice, cuda_error_string
+from .embed import EmbedRows
+from .softmax import Softmax
 
 
 @dataclasses.dataclass
@@ -49,6 +52,13 @@ class Opts:
     useGPU: bool = True
     seed: int = 0
     sortPermute: bool = False   # True: shuffle the pair list by sorting random keys (the reference's GPU branch)
+    # not in the reference: the exact objective that negative sampling stands for, with AdamW
+    fullSoftmax: bool = False
+    beta1: float = 0.9
+    beta2: float = 0.999
+    adamEps: float = 1e-8
+    wdecay: float = 0.0
+    momentBits: int = 32        # 32 or 8
 
     def to_c(self) -> _lib.W2VOpts:
         return _lib.W2VOpts(self.dim, self.nskip, self.nneg, self.nreuse, self.vocabSize,
@@ -84,7 +94,13 @@ class Word2Vec:
     With ``nSlices > 1`` the model holds one vocabulary slice (Word2Vec.scala:104-135, 665-672):
     the ``nHeadTerms`` most frequent words, which every slice has, followed by the words with
     ``id % nSlices == iSlice``; the matrices then have ``sliceRows()`` rows, minibatches still
-    carry global ids, and every slice of a job sees every minibatch."""
+    carry global ids, and every slice of a job sees every minibatch.
+
+    With ``fullSoftmax`` a minibatch trains the exact softmax: the mean over its positive pairs of
+    ``-log p(centre | context)``, ``p`` over all words from ``modelmats[1] @ modelmats[0][context]``,
+    by one AdamW step (``lrate`` decays as usual, ``beta1, beta2, adamEps, wdecay, momentBits``), and
+    ``evalbatch`` returns the mean of ``log p``.  Not for vocabulary slices.  The moments are not
+    part of a checkpoint: a loaded model starts them at zero."""
 
     Opts = Opts
 
@@ -97,6 +113,8 @@ class Word2Vec:
                                       "CPU kernels; this build has no CPU path")
         if self.opts.nSlices < 1 or not 0 <= self.opts.iSlice < self.opts.nSlices or self.opts.nHeadTerms < 0:
             raise ValueError("need nSlices >= 1, 0 <= iSlice < nSlices, nHeadTerms >= 0")
+        if self.opts.fullSoftmax and self.opts.nSlices > 1:
+            raise ValueError("fullSoftmax needs the whole vocabulary: nSlices must be 1")
         self.device = torch.device(device if device is not None else "cuda")
         self.modelmats: list[torch.Tensor] = []
         self.ncols = 0
@@ -108,6 +126,9 @@ class Word2Vec:
         self._mc = 0         # NVLink multicast address of the model buffer (0: not in symmetric memory)
         self._symm = None
         self._tick = None
+        self._updater = None   # AdamW of fullSoftmax, made by its first minibatch
+        self._adam_steps = 0
+        self._firstPos = None
 
     def sliceRows(self) -> int:
         """Rows of each matrix: nHeadTerms + 1 + (vocabSize - nHeadTerms - 1) / nSlices
@@ -134,6 +155,8 @@ class Word2Vec:
                 _check(lib.w2v_init_model(C.byref(shape), mm1.data_ptr(), mm0.data_ptr(),
                                           self._stream()), "w2v_init_model")
                 self.modelmats = [mm0, mm1]
+                self._updater, self._adam_steps = None, 0
+            self._firstPos = None
             ctx = C.c_void_p()
             err = lib.w2v_create(C.byref(self._copts), self.ncols, C.byref(ctx))
             if err:
@@ -174,6 +197,9 @@ class Word2Vec:
         toks = gmats[0]
         if toks.shape[0] != self.ncols:
             return
+        if self.opts.fullSoftmax:
+            self._softmaxBatch(toks, pos, uniforms)
+            return
         self._batches += 1
         with torch.cuda.device(self.device):
             _check(_lib.load().w2v_dobatch(self._ctx, toks.data_ptr(), self._uniforms(uniforms),
@@ -188,6 +214,8 @@ class Word2Vec:
         if toks.shape[0] != self.ncols:
             return 0.0
         self.finishMerge()        # scores are taken on a model no exchange is writing to
+        if self.opts.fullSoftmax:
+            return self._softmaxScore(toks, uniforms)
         self._batches += 1
         score = C.c_double(0.0)
         with torch.cuda.device(self.device):
@@ -204,6 +232,8 @@ class Word2Vec:
         host = _host_i32(mats[0])
         if host.shape[0] != self.ncols:
             return 0
+        if self.opts.fullSoftmax:
+            return self._softmaxBatch(torch.from_numpy(host).to(self.device), pos)
         self._batches += 1
         npairs = C.c_int64(0)
         with torch.cuda.device(self.device):
@@ -221,6 +251,8 @@ class Word2Vec:
         if host.shape[0] != self.ncols:
             return 0.0
         self.finishMerge()
+        if self.opts.fullSoftmax:
+            return self._softmaxScore(torch.from_numpy(host).to(self.device))
         self._batches += 1
         score = C.c_double(0.0)
         with torch.cuda.device(self.device):
@@ -229,6 +261,65 @@ class Word2Vec:
                                                   self._batches, C.byref(score), self._stream()),
                    "w2v_evalbatch_host")
         return score.value
+
+    # -- the softmax over the whole vocabulary -------------------------------
+    def windowRows(self, words, lbound, ubound):
+        """The positive pairs of a minibatch grouped by context word: ``(ids, targets)``, int32 ``[rows]``
+        and ``[rows, 2 * nskip]``; row by row, in the order of the text, a word and the centre words that
+        have it in their window, -1 behind the last.  Positions without a pair have no row."""
+        n, width = words.numel(), 2 * self.opts.nskip
+        ids = torch.empty(n, dtype=torch.int32, device=words.device)
+        targets = torch.empty(n, width, dtype=torch.int32, device=words.device)
+        lib = _lib.load()
+        size = lib.w2v_window_rows_workspace(n)
+        work = torch.empty(size // 4 + 1, dtype=torch.int32, device=words.device)
+        with torch.cuda.device(words.device):
+            _check(lib.w2v_window_rows(words.data_ptr(), lbound.data_ptr(), ubound.data_ptr(), n, self.opts.nskip,
+                                       ids.data_ptr(), targets.data_ptr(), work[size // 4:].data_ptr(),
+                                       work.data_ptr(), size, self._stream()), "w2v_window_rows")
+        rows = int(work[size // 4].item())
+        return ids[:rows], targets[:rows]
+
+    def _softmaxRows(self, toks, uniforms=None):
+        """Word ids, targets and the number of pairs of the minibatch."""
+        self._batches += 1
+        words, lb, ub, _, _ = self.wordMats([toks], uniforms=uniforms, batch_id=self._batches)
+        ids, targets = self.windowRows(words, lb, ub)
+        return ids, targets, self.last_contexts.numel()
+
+    def _softmaxBatch(self, toks, pos: int, uniforms=None) -> int:
+        """One minibatch of ``fullSoftmax``; returns the number of positive pairs."""
+        o = self.opts
+        if self._firstPos is None:
+            self._firstPos = max(1, int(pos))
+        ids, targets, pairs = self._softmaxRows(toks, uniforms)
+        if pairs == 0:
+            return 0
+        context, centre = self.modelmats
+        hidden = EmbedRows.forward(ids, context)
+        _, lse = Softmax.loss(hidden, centre, targets)
+        mean = torch.full((1,), 1.0 / pairs, dtype=torch.float32, device=self.device)
+        dhidden, dcentre = Softmax.grad(hidden, centre, targets, lse, mean)
+        dcontext = EmbedRows.backward(ids, dhidden, context.shape[0])
+        up = self._updater
+        if up is None or any(p is not m for p, m in zip(up.params, self.modelmats)):
+            # the matrices may have moved (symmetric memory): the moments go along
+            state = None if up is None else {"t": self._adam_steps, "m": up.m, "v": up.v, "mscale": up.mscale,
+                                             "vscale": up.vscale}
+            up = self._updater = AdamW(self.modelmats, AdamW.Opts(lrate=o.lrate, beta1=o.beta1, beta2=o.beta2,
+                                                                  eps=o.adamEps, wdecay=o.wdecay, bits=o.momentBits),
+                                       state=state)
+        up.step([dcontext, dcentre], o.lrate * (max(1, int(pos)) / self._firstPos) ** -o.texp)
+        self._adam_steps += 1
+        return pairs
+
+    def _softmaxScore(self, toks, uniforms=None) -> float:
+        """Mean of ``log p(centre | context)`` over the minibatch's positive pairs (0 without any)."""
+        ids, targets, pairs = self._softmaxRows(toks, uniforms)
+        if pairs == 0:
+            return 0.0
+        loss, _ = Softmax.loss(EmbedRows.forward(ids, self.modelmats[0]), self.modelmats[1], targets)
+        return -float(loss.cpu().numpy().sum(dtype=np.float64)) / pairs
 
     # -- the pieces, one reference method each ------------------------------
     def wordMats(self, gmats, ipass: int = 0, pos: int = 0, uniforms=None, batch_id: int = 0):
@@ -504,6 +595,9 @@ class Word2Vec:
         if not dist.is_initialized() or dist.get_world_size(group) == 1:
             return
         self.finishMerge()
+        if self.opts.fullSoftmax:      # its minibatches have no negative update to run beside
+            self.mergeModelFn(group)
+            return
         world = dist.get_world_size(group)
         if getattr(self, "_mc", 0):
             blocks = self.EXCHANGE_BLOCKS.get(world, 24)
@@ -638,6 +732,7 @@ class Word2Vec:
                              ([m.shape for m in mats], self.opts.vocabSize, self.opts.dim))
         if not getattr(self, "modelmats", None) or tuple(self.modelmats[0].shape) != mats[0].shape:
             self.init(getattr(self, "ncols", 0) or 1)
+        self._updater, self._adam_steps = None, 0
         for dst, src in zip(self.modelmats, mats):
             dst.copy_(torch.from_numpy(np.array(src, dtype=np.float32, order="C")))
         return self

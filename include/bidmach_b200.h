@@ -419,7 +419,8 @@ int64_t bidmach_lz4_decompress(const void *src, int64_t n, void *dst, int64_t ca
 /* -------------------------------------------------------------------------
  * Part 5 -- training operators over whole matrices (no counterpart among the
  * reference's native functions): softmax cross entropy over the vocabulary with
- * its gradients, rows by ids with their gradient, and AdamW.
+ * its gradients (and the rows of a minibatch for it), rows by ids with their
+ * gradient, and AdamW.
  *
  * Common to all of them: device pointers; work is enqueued on `stream` and
  * nothing waits for it; the calls can be captured into a CUDA graph; scratch
@@ -443,6 +444,15 @@ int64_t w2v_embed_grad_workspace(int64_t n, int64_t vocab, int dim, int type);  
 int w2v_embed_grad(const int *ids, int64_t n, const void *grad, int64_t ldg, int64_t vocab, int dim,
                    int type, void *out, int64_t ldo, void *workspace, int64_t workspace_bytes,
                    void *stream);
+
+/* The positive pairs of a minibatch (words, lb, ub as w2v_wordmats leaves them) grouped by context:
+ * for each position k, in order, whose word is in the window of at least one centre i (words[i] >= 0,
+ * i != k, lb[i] <= k - i <= ub[i]), ids[row] = words[k] and targets[row] = the words of those centres,
+ * 2 * nskip places, -1 behind the last.  ids holds up to n, targets up to n x 2 nskip; *nrows (device)
+ * receives the number of rows.  1 <= nskip <= 512; workspace 4-byte aligned. */
+int64_t w2v_window_rows_workspace(int n);
+int w2v_window_rows(const int *words, const int *lb, const int *ub, int n, int nskip, int *ids,
+                    int *targets, int *nrows, void *workspace, int64_t workspace_bytes, void *stream);
 
 /* Softmax cross entropy of n rows of hidden vectors against all words, in pieces of the vocabulary
  * (no logits are kept).  With l = hidden weight^T, `labels` targets a row (targets is n x labels; one

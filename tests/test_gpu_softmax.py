@@ -50,22 +50,23 @@ def hold(got, hidden, weight, targets, gloss, t):
     vocab = w.shape[0]
     e = (dim * U + 2.0 ** -20) * (h @ w.T).amax(1)
     lse_off = e + 2.0 ** -20 * (1 + f["lse"].abs())
-    loss, lse, dh, dw = (x.double().cpu() for x in got)
+    loss, lse, dh, dw = (x.double().to(h.device) for x in got)
     assert torch.all((lse - f["lse"]).abs() <= lse_off)
     assert torch.all((loss - f["loss"]).abs() <= f["k"] * (lse_off + e) + f["k"] * U * f["loss"].abs())
     # what d may be off by: its probabilities, then its rounding (fp32 keeps 22 bits of it)
     half = torch.finfo(TYPES[t]).eps / 2
     rel = (e + lse_off + 2.0 ** -20)[:, None]
-    off = 1.001 * rel * f["prob"] + (half if t != "f32" else 2.0 ** -21) * f["d"].abs() + U * f["hit"]
+    off = 1.001 * rel * f["prob"].abs() + (half if t != "f32" else 2.0 ** -21) * f["d"].abs() + U * f["hit"].abs()
+    top = (gloss.double().abs() * f["k"]).amax()
+    off = off + 2.0 ** -126 * top     # an exponential below the smallest normal number is zero
     if t != "bf16":    # fp16 parts of d: steps of 2^-25 where the largest row's is 2^14 to 2^15
-        top = (gloss.double() * f["k"]).amax()
         off = off + 2.0 ** (-38 if t == "f16" else -48) * top
     grow = 2 * U       # truncated accumulation, and the joining of pieces
     for got_g, want, other, terms, count in ((dh, f["dh"], w, f["d"].abs(), vocab), (dw, f["dw"], h, f["d"].abs().T, n)):
         o = off if other is w else off.T
         size = terms @ other
         bound = o @ other + (grow * (count + 64) + 2.0 ** -20) * size
-        bound = bound + (half + U) * (want.abs() + bound) + (2.0 ** -25 if t == "f16" else 0)
+        bound = bound + (half + U) * (want.abs() + bound) + (2.0 ** -25 if t == "f16" else 2.0 ** -126)
         assert torch.all((got_g - want).abs() <= bound)
 
 
@@ -87,3 +88,186 @@ SIZES = [(1, 1, 1), (1, 1000, 256), (2, 33, 7), (3, 257, 300), (5, 1001, 64), (8
 def test_against_64_bits(n, vocab, dim, labels, t):
     x = inputs(n, vocab, dim, labels, t)
     hold(run(*x), *x, t)
+
+
+@pytest.mark.parametrize("n,vocab,dim,t", [(8500, 12000, 24, "f32"), (8500, 21000, 24, "bf16"), (16600, 300, 16, "f16"),
+                                           (8193, 1000, 300, "f32"), (700, 40000, 40, "f16")])
+def test_several_pieces(n, vocab, dim, t):
+    """More rows or words than one piece holds: sums go on over pieces, the last one smaller."""
+    x = inputs(n, vocab, dim, 2, t)
+    got = run(*x)
+    hold([g.cuda() for g in got], *[v.cuda() for v in x], t)
+
+
+@pytest.mark.parametrize("n", [5, 100])
+@pytest.mark.parametrize("t", list(TYPES))
+def test_one_factor_for_all_rows(n, t):
+    hidden, weight, targets, _ = inputs(n, 700, 48, 3, t)
+    for g in (1.0, -0.375, 1e-6, 3e4):
+        if t == "f16" and g == 3e4:
+            continue     # the gradients themselves leave the type's range
+        one = torch.tensor([g])
+        got = run(hidden, weight, targets, one)
+        f = formula(hidden, weight, targets, one.expand(n))
+        for have, want in ((got[2], f["dh"]), (got[3], f["dw"])):
+            half = torch.finfo(TYPES[t]).eps / 2
+            terms = (f["d"].abs() @ weight.double().abs()).amax() if want is f["dh"] else \
+                (f["d"].abs().T @ hidden.double().abs()).amax()
+            # d and the result are rounded, the rest is fp32: four half steps of the largest sum of terms
+            bound = 4 * max(half, 2.0 ** -18) * terms + (2.0 ** -25 if t == "f16" else 0)
+            assert (have.double().cpu() - want).abs().amax() <= bound
+
+
+@pytest.mark.parametrize("n", [4, 60])
+@pytest.mark.parametrize("t", list(TYPES))
+def test_weights_of_rows_over_decades(n, t):
+    """Zero, negative and tiny factors of single rows beside large ones."""
+    hidden, weight, targets, gloss = inputs(n, 333, 40, 2, t)
+    gloss = gloss * torch.logspace(0, -5, n)
+    gloss[1] = 0.0
+    gloss[2] = -gloss[2]
+    got = run(hidden, weight, targets, gloss)
+    hold(got, hidden, weight, targets, gloss, t)
+    assert not got[2][1].any()
+
+
+@pytest.mark.parametrize("n", [3, 200])
+@pytest.mark.parametrize("t", list(TYPES))
+def test_rows_inside_wider_matrices(n, t):
+    """Any leading dimension and alignment, of the operands and of the results; what lies between stays."""
+    from bidmach_b200 import Softmax
+    for off, dim in ((0, 64), (8, 56), (3, 61), (1, 16)):
+        hidden, weight, targets, gloss = inputs(n, 515, dim, 1, t)
+        base_h, base_w = torch.zeros(n, 80, dtype=TYPES[t], device="cuda"), torch.zeros(515, 88, dtype=TYPES[t], device="cuda")
+        h, w = base_h[:, off:off + dim], base_w[:, off:off + dim]
+        h.copy_(hidden)
+        w.copy_(weight)
+        y, g = targets[:, 0].contiguous().cuda(), gloss.cuda()
+        loss, lse = Softmax.loss(h, w, y)
+        dbase_h, dbase_w = torch.full_like(base_h, 9.0), torch.full_like(base_w, 9.0)
+        dh, dw = Softmax.grad(h, w, y, lse, g, dhidden=dbase_h[:, off:off + dim], dweight=dbase_w[:, off:off + dim])
+        hold((loss, lse, dh, dw), hidden, weight, targets, gloss, t)
+        for base in (dbase_h, dbase_w):
+            keep = torch.ones(base.shape[1], dtype=torch.bool)
+            keep[off:off + dim] = False
+            assert (base[:, keep] == 9.0).all()
+
+
+@pytest.mark.parametrize("n", [6, 150])
+@pytest.mark.parametrize("t", list(TYPES))
+def test_large_and_small_logits(n, t):
+    """Logits up to a few hundred (all but one word at probability zero) and logits of nearly zero."""
+    for size in (30.0, 2.0 ** -12):
+        x = inputs(n, 400, 64, 2, t, size=size)
+        hold(run(*x), *x, t)
+
+
+@pytest.mark.parametrize("n", [5, 90])
+@pytest.mark.parametrize("t", list(TYPES))
+def test_not_finite_rows(n, t):
+    """An infinity or a NaN in a row of hidden spoils that row's lse and loss, no other's."""
+    from bidmach_b200 import Softmax
+    hidden, weight, targets, _ = inputs(n, 300, 32, 1, t)
+    targets[:] = 7
+    want = formula(hidden, weight, targets, torch.ones(n))
+    hidden[1, 3], hidden[3, 5] = float("nan"), float("inf")
+    loss, lse = Softmax.loss(hidden.cuda(), weight.cuda(), targets.cuda())
+    bad = torch.zeros(n, dtype=torch.bool)
+    bad[1] = bad[3] = True
+    assert torch.isnan(lse.cpu()[bad]).all() and torch.isnan(loss.cpu()[bad]).all()
+    assert (lse.cpu().double() - want["lse"])[~bad].abs().max() <= 2.0 ** -14
+    assert torch.isfinite(loss.cpu()[~bad]).all()
+
+
+def test_no_rows_and_no_targets():
+    from bidmach_b200 import Softmax
+    w = torch.randn(50, 12, device="cuda")
+    h, y = torch.empty(0, 12, device="cuda"), torch.empty(0, 3, dtype=torch.int32, device="cuda")
+    loss, lse = Softmax.loss(h, w, y)
+    assert loss.shape == lse.shape == (0,)
+    dh, dw = Softmax.grad(h, w, y, lse, torch.ones(1, device="cuda"))
+    assert dh.shape == (0, 12) and not dw.any()
+    for n in (3, 70):
+        h, y = torch.randn(n, 12, device="cuda"), torch.full((n, 2), -1, dtype=torch.int32, device="cuda")
+        loss, lse = Softmax.loss(h, w, y)
+        dh, dw = Softmax.grad(h, w, y, lse, torch.ones(n, device="cuda"))
+        assert not loss.any() and not dh.any() and not dw.any() and torch.isfinite(lse).all()
+
+
+@pytest.mark.parametrize("n,vocab,dim,t", [(7, 500, 20, "f32"), (130, 900, 33, "f32")])
+def test_gradient_against_differences(n, vocab, dim, t):
+    """Along a direction, the difference of the kernel's losses over a step and the kernel's gradient.  The
+    difference has the formula's own curvature error, taken from the same difference in 64 bits, and
+    the losses' rounding over the step."""
+    from bidmach_b200 import Softmax
+    hidden, weight, targets, gloss = inputs(n, vocab, dim, 2, t)
+    gen = torch.Generator().manual_seed(3)
+    u, z, e = torch.randn(n, dim, generator=gen), torch.randn(vocab, dim, generator=gen) / dim ** 0.5, 2.0 ** -6
+
+    def total(s):
+        loss, _ = Softmax.loss((hidden + s * u).cuda(), (weight + s * z).cuda(), targets.cuda())
+        return float((loss.double().cpu() * gloss.double()).sum())
+
+    def total64(s):
+        return float((formula(hidden.double() + s * u, weight.double() + s * z, targets, gloss)["loss"] * gloss.double()).sum())
+
+    _, _, dh, dw = run(hidden, weight, targets, gloss)
+    along = float((dh.double().cpu() * u).sum() + (dw.double().cpu() * z).sum())
+    f = formula(hidden, weight, targets, gloss)
+    exact = float((f["dh"] * u).sum() + (f["dw"] * z).sum())
+    curved = abs((total64(e) - total64(-e)) / (2 * e) - exact)
+    size = (hidden.abs() + e * u.abs()).double() @ (weight.abs() + e * z.abs()).double().T
+    noise = float((gloss.double() * f["k"] * (2 * (dim + 64) * U * size.amax(1) + 2.0 ** -19 * (1 + f["lse"].abs()))).sum()) / e
+    assert abs((total(e) - total(-e)) / (2 * e) - along) <= curved + noise + 2.0 ** -16 * abs(exact)
+
+
+def test_equal_calls_streams_and_graphs():
+    """Two calls at once on two streams, and two captured graphs replayed side by side, give the bits of
+    the call alone."""
+    from bidmach_b200 import Softmax
+    sets = []
+    for n, vocab, dim, t in ((300, 3000, 100, "bf16"), (260, 2000, 70, "f32")):
+        x = [v.cuda() for v in inputs(n, vocab, dim, 2, t)]
+        sets.append((x, run(*x)))
+    torch.cuda.synchronize()
+
+    def step(x):
+        loss, lse = Softmax.loss(*x[:3])
+        return (loss, lse, *Softmax.grad(*x[:3], lse, x[3]))
+
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    for _ in range(3):
+        for s, (x, want) in zip(streams, sets):
+            with torch.cuda.stream(s):
+                got.append((step(x), want))
+    torch.cuda.synchronize()
+    graphs = []
+    for x, want in sets:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step(x)
+        graphs.append(graph)
+        got.append((out, want))
+    for _ in range(3):
+        for s, graph in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+    torch.cuda.synchronize()
+    for have, want in got:
+        assert all(torch.equal(a, b) for a, b in zip(have, want))
+
+
+def test_refusals_on_the_device():
+    from bidmach_b200 import Softmax
+    h, w = torch.zeros(4, 8, device="cuda"), torch.zeros(9, 8, device="cuda")
+    y, g = torch.zeros(4, dtype=torch.int32, device="cuda"), torch.ones(4, device="cuda")
+    for args in [(h.half(), w, y), (h, w[:, :7], y), (h, w, y.long()), (h, w, y[:3]), (h, w, y.cpu()), (h.t(), w, y),
+                 (h, w[:0], y), (h, w, y.view(4, 1, 1)), (torch.zeros(4, 5000, device="cuda"), torch.zeros(9, 5000, device="cuda"), y)]:
+        with pytest.raises(ValueError):
+            Softmax.loss(*args)
+    loss, lse = Softmax.loss(h, w, y)
+    for bad in [(lse[:3], g), (lse.double(), g), (lse, g[:3]), (lse, g.cpu()), (lse, g.half())]:
+        with pytest.raises(ValueError):
+            Softmax.grad(h, w, y, *bad)
+    with pytest.raises(ValueError):
+        Softmax.grad(h, w, y, lse, g, dweight=torch.zeros(8, 8, device="cuda"))

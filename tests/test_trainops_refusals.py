@@ -67,3 +67,12 @@ def test_softmax_refuses():
         Softmax.loss(torch.zeros(3, 4), torch.zeros(5, 4), torch.zeros(3, dtype=torch.int32))
     with pytest.raises(ValueError):
         Softmax.loss(torch.zeros(3, 4, dtype=torch.float64), torch.zeros(5, 4), torch.zeros(3, dtype=torch.int32))
+
+
+def test_window_rows_refuses():
+    lib = _lib.load()
+    assert lib.w2v_window_rows_workspace(-1) == -1
+    size = lib.w2v_window_rows_workspace(10)
+    for n, nskip, rows, ws, have in [(-1, 5, 64, 64, 1 << 20), (10, 0, 64, 64, size), (10, 513, 64, 64, size),
+                                     (10, 5, 0, 64, size), (10, 5, 64, 0, size), (10, 5, 64, 64, size - 1)]:
+        assert lib.w2v_window_rows(64, 64, 64, n, nskip, 64, 64, rows, ws, have, None) == 1
