@@ -539,7 +539,6 @@ __device__ __forceinline__ uint32_t pair_begin(Pipe &s) {
   tmem_before_sync();
   cluster_sync();
   tmem_after_sync();
-  chain_wait();
   return s.tmem;
 }
 // Neither CTA leaves while the other's products read its shared memory or its barriers are arrived on.
@@ -1314,6 +1313,10 @@ struct Operand {
   int width;   // offset between parts
 };
 
+// The kernels that work in pairs of CTAs with tensor memory are launched in the ordinary way, each after
+// its predecessor has ended; started early like the others (w2v_chain.cuh), short ones in a row were seen
+// to stop now and then.
+
 // An attribute of the function on the current device, so it is set before every launch.
 template <typename K>
 int allow_smem(K kernel, size_t bytes) {
@@ -1325,7 +1328,9 @@ template <Use USE>
 int launch_product(const Product &p, cudaStream_t s) {
   const int err = allow_smem(product_kernel<USE>, kProductSmem<USE>);
   if (err) return err;
-  return launch_chained(product_kernel<USE>, 2 * std::min(p.mt * p.nt, sm_pairs()), kMmaThreads, kProductSmem<USE>, s, p);
+  product_kernel<USE><<<2 * std::min(p.mt * p.nt, sm_pairs()), kMmaThreads, kProductSmem<USE>, s>>>(p);
+  count_launch(1);
+  return (int)cudaGetLastError();
 }
 
 template <typename T>
@@ -1334,7 +1339,9 @@ int launch_gradients(const Gradients &g, cudaStream_t s) {
   int err = allow_smem(grad_kernel<split>, kGradSmem);
   if (err) return err;
   const bool whole = g.side[0].whole || g.side[1].whole;
-  err = launch_chained(grad_kernel<split>, 2 * (whole ? g.npairs : g.sharers), kMmaThreads, kGradSmem, s, g);
+  grad_kernel<split><<<2 * (whole ? g.npairs : g.sharers), kMmaThreads, kGradSmem, s>>>(g);
+  count_launch(1);
+  err = (int)cudaGetLastError();
   const int rest = g.side[0].rest(g.npairs) + g.side[1].rest(g.npairs);
   if (!err && rest > 0 && g.sharers > 1) err = launch_chained(pieces_kernel<T>, dim3(rest, kPairM / 8), 256, 0, s, g);
   return err;
