@@ -37,7 +37,13 @@ class on_device:
 
 
 def stream_of(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    """Handle of the device's current stream."""
+    return _raw_stream(device.index)
+
+
+# the handle without a Stream object around it, where torch offers that
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 @dataclasses.dataclass
@@ -95,6 +101,7 @@ class AdamW:
         n = len(self.params)
         self._sizes = [p.numel() for p in self.params]
         self._types = [p.dtype for p in self.params]
+        self._pointers = C.c_void_p * n
         self._kinds = (C.c_int * n)(*[TYPES[t] for t in self._types])
         self._table = (_lib.W2VAdamwTensor * n)()
         for i, p in enumerate(self.params):
@@ -103,8 +110,9 @@ class AdamW:
                 self.mscale[i].data_ptr() if self.mscale else 0, self.vscale[i].data_ptr() if self.vscale else 0,
                 p.numel(), TYPES[p.dtype])
         self._clock = torch.zeros(4, dtype=torch.float64, device=self.device)
+        self._clock_at = self._clock.data_ptr()
         with on_device(self.device):
-            check(_lib.load().w2v_adamw_clock(self._clock.data_ptr(), o.beta1, o.beta2, t, stream_of(self.device)),
+            check(_lib.load().w2v_adamw_clock(self._clock_at, o.beta1, o.beta2, t, stream_of(self.device)),
                   "w2v_adamw_clock")
 
     def _state(self, state):
@@ -169,9 +177,9 @@ class AdamW:
             rate = float(lrate)
         opts = _lib.W2VAdamwOpts(rate, o.beta1, o.beta2, o.eps, o.wdecay)
         with on_device(dev):
-            check(_lib.load().w2v_adamw_step(self._table, (C.c_void_p * n)(*[g.data_ptr() for g in grads]),
+            check(_lib.load().w2v_adamw_step(self._table, self._pointers(*map(torch.Tensor.data_ptr, grads)),
                                              kinds, n, o.bits, C.byref(opts), rate_ptr,
-                                             self._clock.data_ptr(), stream_of(dev)), "w2v_adamw_step")
+                                             self._clock_at, stream_of(dev)), "w2v_adamw_step")
 
     def moments(self, mout=None, vout=None):
         """Both moments as fp32 values: lists (m, v).  With 32 bits these are the state itself; with 8
@@ -194,7 +202,7 @@ class AdamW:
         if any(x.dtype is not torch.float32 for x in both):
             raise ValueError(what)
         with on_device(dev):
-            check(_lib.load().w2v_adamw_moments(self._table, (C.c_void_p * n)(*[x.data_ptr() for x in mout]),
-                                                (C.c_void_p * n)(*[x.data_ptr() for x in vout]), n,
+            check(_lib.load().w2v_adamw_moments(self._table, self._pointers(*map(torch.Tensor.data_ptr, mout)),
+                                                self._pointers(*map(torch.Tensor.data_ptr, vout)), n,
                                                 stream_of(dev)), "w2v_adamw_moments")
         return mout, vout

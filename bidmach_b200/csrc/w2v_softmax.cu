@@ -7,7 +7,7 @@
 // and gradient are zero).  For N rows, V words and D columns the loss costs 2 N V D operations, the
 // gradients 4 N V D and, since no logits are kept, the logits' 2 N V D again.
 //
-// More than kFewRows rows: the tensor cores.  One kernel computes tiles of 128 x 256 of a product
+// More than a few rows (few_rows): the tensor cores.  One kernel computes tiles of 128 x 256 of a product
 // whose operands TMA brings into shared memory (a producer warp, a warp that issues tcgen05.mma, eight
 // warps that read the finished tile from tensor memory while the next one is computed in the other
 // half of it).  What the eight warps do with a tile is the difference between its three uses:
@@ -20,12 +20,17 @@
 // the fp32 accumulators.  d is rounded once to the operands' type (fp32: to hi + lo with lo scaled by
 // 2^11, so that small probabilities keep their bits; the operand it meets carries the 2^-11).
 //
-// Up to kFewRows rows the bound is reading W once: a kernel with the rows in shared memory, W straight
-// from memory in its own type, plain fp32 arithmetic.
+// For few rows the bound is reading W once: a kernel with eight rows in shared memory, W straight from
+// memory in its own type, plain fp32 arithmetic.  fp32 goes that way up to 16 rows, in two passes: the
+// tensor cores would need W in two parts, three more passes over it (100000 x 256, loss / gradients: 8 rows
+// 30 / 78 us, 16 rows 60 / 156, against 107 / 223 for 9 or more).  16-bit types need no such parts, so
+// four rows are the border (4 rows 24 / 97 us, 8 rows 30 / 110, against 27 / 86).
 #include <cuda.h>
 #include <math.h>
 
 #include <algorithm>
+#include <atomic>
+#include <type_traits>
 
 #include "../../include/bidmach_b200.h"
 #include "w2v_chain.cuh"
@@ -39,7 +44,7 @@ namespace {
 using namespace w2v;
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kFewRows = 8;
+constexpr int kFewRows = 8;   // of a pass
 constexpr int kMaxDim = 4096;
 
 // A row's sum of exponentials as 2^m * s, with exponents in units of log2 e.
@@ -189,7 +194,7 @@ template <typename T, int RB>
 __global__ void __launch_bounds__(kFewThreads) few_grad_kernel(const T *h, int64_t ldh, int rows, const T *w, int64_t ldw,
                                                                int64_t vocab, int dim, bool wide, const int *targets,
                                                                int labels, const float *lse, const float *gloss,
-                                                               int64_t ldg, T *dw, int64_t lddw, bool wide_out,
+                                                               int64_t ldg, T *dw, int64_t lddw, bool wide_out, bool add,
                                                                float *d) {
   extern __shared__ __align__(16) float sh[];
   __shared__ float lse_s[RB], g_s[RB], k_s[RB];
@@ -244,6 +249,12 @@ __global__ void __launch_bounds__(kFewThreads) few_grad_kernel(const T *h, int64
       for (int q = 0; q < kFewWords; q++) {
         if (v + q >= vocab) break;
         T *p = dw + (v + q) * lddw + col;
+        if (add) {   // fp32 only: a second pass
+          float old[8];
+          load_some(p, have, old);
+#pragma unroll
+          for (int e = 0; e < 8; e++) acc[q][e] += old[e];
+        }
         if (wide_out && have == 8) store8(p, acc[q]);
         else store_some(p, have, acc[q]);
       }
@@ -252,32 +263,50 @@ __global__ void __launch_bounds__(kFewThreads) few_grad_kernel(const T *h, int64
   }
 }
 
-// dH of few rows: a block sums d_nv w_v over a range of words, a thread a column.
+// dH of few rows: a warp sums d_nv w_v over a range of words, 256 columns (8 a lane) of all rows at a
+// time, four words in flight; the block adds its warps' sums.  parts is [block][RB][dim].
 template <typename T, int RB>
-__global__ void __launch_bounds__(kFewThreads) few_dh_kernel(const T *w, int64_t ldw, int64_t vocab, int dim,
+__global__ void __launch_bounds__(kFewThreads) few_dh_kernel(const T *w, int64_t ldw, int64_t vocab, int dim, bool wide,
                                                              const float *d, float *parts) {
+  constexpr int warps = kFewThreads / 32;
+  __shared__ __align__(16) float sums[warps][256];
   chain_wait();
-  const int64_t each = (vocab + gridDim.x - 1) / gridDim.x;
-  const int64_t lo = blockIdx.x * each, hi = min(vocab, lo + each);
-  for (int c = blockIdx.y * kFewThreads + threadIdx.x; c < dim; c += gridDim.y * kFewThreads) {
-    float acc[RB] = {};
-    int64_t v = lo;
-    for (; v + 4 <= hi; v += 4) {
-      float x[4];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+  const int64_t all = (int64_t)gridDim.x * warps, me = (int64_t)blockIdx.x * warps + warp;
+  const int64_t lo = me * vocab / all, hi = (me + 1) * vocab / all;
+  const int col = blockIdx.y * 256 + lane * 8, have = min(8, max(0, dim - col));
+  float acc[RB][8] = {};
+  for (int64_t v = lo; v < hi; v += 4) {
+    float x[4][8], dv[4][RB];
 #pragma unroll
-      for (int q = 0; q < 4; q++) x[q] = to_float(w[(v + q) * ldw + c]);
+    for (int q = 0; q < 4; q++) {
+      const bool there = v + q < hi;
+      const T *p = w + (v + q) * ldw + col;
+      if (wide && there && have == 8) load8(p, x[q]);
+      else load_some(p, there ? have : 0, x[q]);
 #pragma unroll
-      for (int q = 0; q < 4; q++)
-#pragma unroll
-        for (int r = 0; r < RB; r++) acc[r] = fmaf(d[(v + q) * RB + r], x[q], acc[r]);
-    }
-    for (; v < hi; v++) {
-      const float x = to_float(w[v * ldw + c]);
-#pragma unroll
-      for (int r = 0; r < RB; r++) acc[r] = fmaf(d[v * RB + r], x, acc[r]);
+      for (int r = 0; r < RB; r++) dv[q][r] = there ? d[(v + q) * RB + r] : 0.f;
     }
 #pragma unroll
-    for (int r = 0; r < RB; r++) parts[((int64_t)blockIdx.x * RB + r) * dim + c] = acc[r];
+    for (int q = 0; q < 4; q++)
+#pragma unroll
+      for (int r = 0; r < RB; r++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) acc[r][e] = fmaf(dv[q][r], x[q][e], acc[r][e]);
+  }
+  const int c = blockIdx.y * 256 + threadIdx.x;
+#pragma unroll
+  for (int r = 0; r < RB; r++) {
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 8; e += 4)
+      *reinterpret_cast<float4 *>(&sums[warp][lane * 8 + e]) =
+          make_float4(acc[r][e], acc[r][e + 1], acc[r][e + 2], acc[r][e + 3]);
+    __syncthreads();
+    float x = 0.f;
+#pragma unroll
+    for (int k = 0; k < warps; k++) x += sums[k][threadIdx.x];
+    if (c < dim) parts[((int64_t)blockIdx.x * RB + r) * dim + c] = x;
   }
 }
 
@@ -301,27 +330,30 @@ __device__ __forceinline__ float rescale_of(const Rescale &r) {
   return r.operand ? x * pow2(-scale_exp(r.operand == 1 ? r.sc->w : r.sc->h, kOperandTop)) : x;
 }
 
-// out[r][c] = sum over slabs, in their order; a warp a row.
+// out[r][c] = sum over slabs: eight warps take an eighth of them each, for 32 columns of a row.
 template <typename T>
-__global__ void __launch_bounds__(256) slabs_kernel(const float *slabs, int count, int64_t slab, int64_t rows, int dim,
-                                                    T *out, int64_t ldo) {
+__global__ void __launch_bounds__(256) slabs_kernel(const float *slabs, int count, int64_t slab, int dim, T *out,
+                                                    int64_t ldo) {
+  __shared__ float sums[8][32];
   chain_wait();
-  const int lane = threadIdx.x & 31;
-  const int64_t cols = (dim + 31) / 32, i = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
-  if (i >= rows * cols) return;
-  const int64_t r = i / cols;
-  const int c = (int)(i % cols) * 32 + lane;
-  if (c >= dim) return;
-  const float *p = slabs + r * dim + c;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+  const int c = blockIdx.x * 32 + lane;
+  const int each = (count + 7) / 8, a = min(count, warp * each), b = min(count, a + each);
+  const float *p = slabs + (int64_t)blockIdx.y * dim + c;
   float x = 0.f;
-  for (int k = 0; k < count; k += 8) {
+  for (int k = a; k < b; k += 8) {
     float y[8];
 #pragma unroll
-    for (int j = 0; j < 8; j++) y[j] = k + j < count ? p[(k + j) * slab] : 0.f;
+    for (int j = 0; j < 8; j++) y[j] = k + j < b && c < dim ? p[(k + j) * slab] : 0.f;
 #pragma unroll
     for (int j = 0; j < 8; j++) x += y[j];
   }
-  out[r * ldo + c] = from_float<T>(x);
+  sums[warp][lane] = x;
+  __syncthreads();
+  if (warp > 0 || c >= dim) return;
+#pragma unroll
+  for (int k = 1; k < 8; k++) x += sums[k][lane];
+  out[(int64_t)blockIdx.y * ldo + c] = from_float<T>(x);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -1317,16 +1349,24 @@ struct Operand {
 // its predecessor has ended; started early like the others (w2v_chain.cuh), short ones in a row were seen
 // to stop now and then.
 
-// An attribute of the function on the current device, so it is set before every launch.
-template <typename K>
-int allow_smem(K kernel, size_t bytes) {
-  return (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+// An attribute of the function on the current device, set once for each (a call costs a microsecond).
+template <auto KERNEL>
+int allow_smem(size_t bytes) {
+  constexpr int kDevices = 64;
+  static std::atomic<size_t> allowed[kDevices];
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return (int)e;
+  if (device < kDevices && allowed[device].load() >= bytes) return 0;
+  e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e == cudaSuccess && device < kDevices) allowed[device].store(bytes);
+  return (int)e;
 }
 int sm_pairs() { return std::max(1, device_sm_count() / 2); }
 
 template <Use USE>
 int launch_product(const Product &p, cudaStream_t s) {
-  const int err = allow_smem(product_kernel<USE>, kProductSmem<USE>);
+  const int err = allow_smem<product_kernel<USE>>(kProductSmem<USE>);
   if (err) return err;
   product_kernel<USE><<<2 * std::min(p.mt * p.nt, sm_pairs()), kMmaThreads, kProductSmem<USE>, s>>>(p);
   count_launch(1);
@@ -1336,7 +1376,7 @@ int launch_product(const Product &p, cudaStream_t s) {
 template <typename T>
 int launch_gradients(const Gradients &g, cudaStream_t s) {
   constexpr bool split = sizeof(T) == 4;
-  int err = allow_smem(grad_kernel<split>, kGradSmem);
+  int err = allow_smem<grad_kernel<split>>(kGradSmem);
   if (err) return err;
   const bool whole = g.side[0].whole || g.side[1].whole;
   grad_kernel<split><<<2 * (whole ? g.npairs : g.sharers), kMmaThreads, kGradSmem, s>>>(g);
@@ -1368,9 +1408,10 @@ int few_blocks(int64_t vocab) {
   return (int)std::min<int64_t>(need, (int64_t)device_sm_count() * 2);
 }
 int few_dh_blocks(int64_t vocab) {
-  return (int)std::min<int64_t>((vocab + 31) / 32, (int64_t)device_sm_count() * 4);
+  return (int)std::min<int64_t>((vocab + 31) / 32, (int64_t)device_sm_count());
 }
 int few_rows_of(int64_t n) { return n <= 1 ? 1 : n <= 2 ? 2 : n <= 4 ? 4 : 8; }
+bool few_rows(const Shape &x) { return x.n <= (x.type == W2V_F32 ? 2 * kFewRows : 4); }
 
 struct Layout {
   int64_t scalars, hs, ws, parts, probs, scratch, pieces, acc_h, acc_w, total;
@@ -1394,10 +1435,10 @@ Layout plan(const Shape &x, bool grad) {
     return here;
   };
   l.scalars = take(sizeof(Scalars));
-  if (x.n <= kFewRows) {
+  if (few_rows(x)) {
     const int rb = few_rows_of(x.n);
     if (!grad) {
-      l.parts = take((int64_t)few_blocks(x.vocab) * x.n * sizeof(Part));
+      l.parts = take((int64_t)few_blocks(x.vocab) * rb * sizeof(Part));
     } else {
       l.probs = take(x.vocab * rb * 4);
       l.acc_h = take((int64_t)few_dh_blocks(x.vocab) * rb * x.dim * 4);
@@ -1484,15 +1525,15 @@ int logits_product(const Shape &x, const Operand &oh, const Operand &ow, const S
 }
 
 template <typename T, int RB>
-int few_loss(const Shape &x, const Layout &l, const void *h, int64_t ldh, const void *w, int64_t ldw, char *ws,
+int few_loss(const Shape &x, const Layout &l, const T *h, int64_t ldh, int rows, const void *w, int64_t ldw, char *ws,
              int *count, cudaStream_t s) {
   const size_t smem = (size_t)RB * few_steps(x.dim) * 1024;
-  auto k = few_loss_kernel<T, RB>;
-  const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e != cudaSuccess) return (int)e;
+  const auto k = few_loss_kernel<T, RB>;
+  const int refused = allow_smem<few_loss_kernel<T, RB>>((size_t)RB * few_steps(kMaxDim) * 1024);
+  if (refused) return refused;
   const bool wide = aligned(w, 8 * sizeof(T)) && ldw % 8 == 0;
   *count = few_blocks(x.vocab);
-  return launch_chained(k, *count, kFewThreads, smem, s, static_cast<const T *>(h), ldh, (int)x.n,
+  return launch_chained(k, *count, kFewThreads, smem, s, h, ldh, rows,
                         static_cast<const T *>(w), ldw, x.vocab, x.dim, wide, reinterpret_cast<Part *>(ws + l.parts));
 }
 
@@ -1506,15 +1547,21 @@ int run_loss(const Shape &x, const Layout &l, const void *h, int64_t ldh, const 
                           rows, static_cast<const T *>(h) + r0 * ldh, ldh, static_cast<const T *>(w), ldw, x.vocab, x.dim,
                           wide, targets + r0 * x.labels, x.labels, loss + r0, lse + r0);
   };
-  if (x.n <= kFewRows) {
-    int count = 0, err = 0;
-    switch (few_rows_of(x.n)) {
-      case 1: err = few_loss<T, 1>(x, l, h, ldh, w, ldw, ws, &count, s); break;
-      case 2: err = few_loss<T, 2>(x, l, h, ldh, w, ldw, ws, &count, s); break;
-      case 4: err = few_loss<T, 4>(x, l, h, ldh, w, ldw, ws, &count, s); break;
-      default: err = few_loss<T, 8>(x, l, h, ldh, w, ldw, ws, &count, s);
+  if (few_rows(x)) {
+    int err = 0;
+    for (int64_t r0 = 0; r0 < x.n && !err; r0 += kFewRows) {
+      const int rows = (int)std::min<int64_t>(kFewRows, x.n - r0);
+      const T *hr = static_cast<const T *>(h) + r0 * ldh;
+      int count = 0;
+      switch (few_rows_of(rows)) {
+        case 1: err = few_loss<T, 1>(x, l, hr, ldh, rows, w, ldw, ws, &count, s); break;
+        case 2: err = few_loss<T, 2>(x, l, hr, ldh, rows, w, ldw, ws, &count, s); break;
+        case 4: err = few_loss<T, 4>(x, l, hr, ldh, rows, w, ldw, ws, &count, s); break;
+        default: err = few_loss<T, 8>(x, l, hr, ldh, rows, w, ldw, ws, &count, s);
+      }
+      if (!err) err = join_rows(count, rows, r0, rows);
     }
-    return err ? err : join_rows(count, x.n, 0, (int)x.n);
+    return err;
   }
   Operand oh, ow;
   int err = stage<T>(x, l, h, ldh, w, ldw, nullptr, nullptr, ws, &oh, &ow, s);
@@ -1537,25 +1584,26 @@ int run_loss(const Shape &x, const Layout &l, const void *h, int64_t ldh, const 
 }
 
 template <typename T, int RB>
-int few_grad(const Shape &x, const Layout &l, const void *h, int64_t ldh, const void *w, int64_t ldw, const int *targets,
-             const float *lse, const float *gloss, int64_t ldg, void *dh, int64_t lddh, void *dw, int64_t lddw, char *ws,
-             cudaStream_t s) {
+int few_grad(const Shape &x, const Layout &l, const void *h, int64_t ldh, int64_t r0, int rows, const void *w, int64_t ldw,
+             const int *targets, const float *lse, const float *gloss, int64_t ldg, void *dh, int64_t lddh, void *dw,
+             int64_t lddw, char *ws, cudaStream_t s) {
   const size_t smem = (size_t)RB * few_steps(x.dim) * 1024;
-  auto k = few_grad_kernel<T, RB>;
-  const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e != cudaSuccess) return (int)e;
+  const auto k = few_grad_kernel<T, RB>;
+  const int refused = allow_smem<few_grad_kernel<T, RB>>((size_t)RB * few_steps(kMaxDim) * 1024);
+  if (refused) return refused;
   const bool wide = aligned(w, 8 * sizeof(T)) && ldw % 8 == 0, wout = aligned(dw, 8 * sizeof(T)) && lddw % 8 == 0;
   float *d = reinterpret_cast<float *>(ws + l.probs), *acc = reinterpret_cast<float *>(ws + l.acc_h);
   const T *wt = static_cast<const T *>(w);
-  int err = launch_chained(k, few_blocks(x.vocab), kFewThreads, smem, s, static_cast<const T *>(h), ldh, (int)x.n, wt, ldw,
-                           x.vocab, x.dim, wide, targets, x.labels, lse, gloss, ldg, static_cast<T *>(dw), lddw, wout, d);
+  int err = launch_chained(k, few_blocks(x.vocab), kFewThreads, smem, s, static_cast<const T *>(h) + r0 * ldh, ldh, rows,
+                           wt, ldw, x.vocab, x.dim, wide, targets + r0 * x.labels, x.labels, lse + r0, gloss + r0 * ldg, ldg,
+                           static_cast<T *>(dw), lddw, wout, r0 > 0, d);
   const int blocks = few_dh_blocks(x.vocab);
   if (!err)
-    err = launch_chained(few_dh_kernel<T, RB>, dim3(blocks, (x.dim + kFewThreads - 1) / kFewThreads), kFewThreads, 0, s, wt,
-                         ldw, x.vocab, x.dim, d, acc);
+    err = launch_chained(few_dh_kernel<T, RB>, dim3(blocks, (x.dim + 255) / 256), kFewThreads, 0, s, wt, ldw, x.vocab, x.dim,
+                         wide, d, acc);
   if (!err)
-    err = launch_chained(slabs_kernel<T>, (unsigned)((x.n * ((x.dim + 31) / 32) + 7) / 8), 256, 0, s, acc, blocks,
-                         (int64_t)RB * x.dim, x.n, x.dim, static_cast<T *>(dh), lddh);
+    err = launch_chained(slabs_kernel<T>, dim3((x.dim + 31) / 32, rows), 256, 0, s, acc, blocks, (int64_t)RB * x.dim, x.dim,
+                         static_cast<T *>(dh) + r0 * lddh, lddh);
   return err;
 }
 
@@ -1564,13 +1612,22 @@ int run_grad(const Shape &x, const Layout &l, const void *h, int64_t ldh, const 
              const float *lse, const float *gloss, int64_t ldg, void *dh, int64_t lddh, void *dw, int64_t lddw, char *ws,
              cudaStream_t s) {
   if (x.n == 0) return (int)cudaMemset2DAsync(dw, lddw * sizeof(T), 0, x.dim * sizeof(T), x.vocab, s);
-  if (x.n <= kFewRows) {
-    switch (few_rows_of(x.n)) {
-      case 1: return few_grad<T, 1>(x, l, h, ldh, w, ldw, targets, lse, gloss, ldg, dh, lddh, dw, lddw, ws, s);
-      case 2: return few_grad<T, 2>(x, l, h, ldh, w, ldw, targets, lse, gloss, ldg, dh, lddh, dw, lddw, ws, s);
-      case 4: return few_grad<T, 4>(x, l, h, ldh, w, ldw, targets, lse, gloss, ldg, dh, lddh, dw, lddw, ws, s);
-      default: return few_grad<T, 8>(x, l, h, ldh, w, ldw, targets, lse, gloss, ldg, dh, lddh, dw, lddw, ws, s);
+  if (few_rows(x)) {
+    int err = 0;
+    for (int64_t r0 = 0; r0 < x.n && !err; r0 += kFewRows) {
+      const int rows = (int)std::min<int64_t>(kFewRows, x.n - r0);
+      auto go = [&](auto rb) {
+        return few_grad<T, decltype(rb)::value>(x, l, h, ldh, r0, rows, w, ldw, targets, lse, gloss, ldg, dh, lddh, dw, lddw,
+                                                ws, s);
+      };
+      switch (few_rows_of(rows)) {
+        case 1: err = go(std::integral_constant<int, 1>()); break;
+        case 2: err = go(std::integral_constant<int, 2>()); break;
+        case 4: err = go(std::integral_constant<int, 4>()); break;
+        default: err = go(std::integral_constant<int, 8>());
+      }
     }
+    return err;
   }
   constexpr bool split = sizeof(T) == 4;
   const float *each_gloss = ldg ? gloss : nullptr, *one_gloss = ldg ? nullptr : gloss;

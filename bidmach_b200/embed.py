@@ -11,22 +11,25 @@ def check_matrix(x, name: str, device=None, dtype=None):
     """A CUDA matrix whose rows are contiguous; returns its leading dimension."""
     if not isinstance(x, torch.Tensor) or x.dim() != 2 or x.dtype not in TYPES:
         raise ValueError(f"{name} is a matrix of fp32, bf16 or fp16")
-    if dtype is not None and x.dtype != dtype:
+    if dtype is not None and x.dtype is not dtype:
         raise ValueError(f"{name} has type {x.dtype}, expected {dtype}")
     if not x.is_cuda:
         raise ValueError(f"{name} is not on a CUDA device")
-    if device is not None and x.device != device:
+    if device is not None and x.get_device() != device.index:
         raise ValueError(f"{name} is on {x.device}, expected {device}")
-    if x.shape[1] < 1:
+    rows, cols = x.shape
+    if cols < 1:
         raise ValueError(f"{name} has no columns")
-    ld = x.stride(0) if x.shape[0] > 1 else x.shape[1]
-    if (x.stride(1) != 1 and x.shape[1] > 1) or ld < x.shape[1]:
+    if rows <= 1 and (cols == 1 or x.stride(1) == 1):
+        return cols
+    ld, step = x.stride()
+    if (step != 1 and cols > 1) or ld < cols:
         raise ValueError(f"{name}: rows have to be contiguous and must not overlap")
     return ld
 
 
 def check_ids(x, name: str, dim: int):
-    if not isinstance(x, torch.Tensor) or x.dim() != dim or x.dtype != torch.int32:
+    if not isinstance(x, torch.Tensor) or x.dim() != dim or x.dtype is not torch.int32:
         raise ValueError(f"{name} is int32 with {dim} dimension" + ("s" if dim > 1 else ""))
     if not x.is_cuda:
         raise ValueError(f"{name} is not on a CUDA device")
@@ -47,10 +50,11 @@ class EmbedRows:
         if vocab < 1:
             raise ValueError("matrix has no rows")
         if out is None:
-            out = torch.empty(n, dim, dtype=matrix.dtype, device=ids.device)
-        ldo = check_matrix(out, "out", ids.device, matrix.dtype)
-        if tuple(out.shape) != (n, dim):
-            raise ValueError(f"out has shape {tuple(out.shape)}, expected {(n, dim)}")
+            out, ldo = torch.empty(n, dim, dtype=matrix.dtype, device=ids.device), dim
+        else:
+            ldo = check_matrix(out, "out", ids.device, matrix.dtype)
+            if tuple(out.shape) != (n, dim):
+                raise ValueError(f"out has shape {tuple(out.shape)}, expected {(n, dim)}")
         with on_device(ids.device):
             check(_lib.load().w2v_embed_rows(ids.data_ptr(), n, matrix.data_ptr(), ldm, vocab, dim,
                                              TYPES[matrix.dtype], out.data_ptr(), ldo, stream_of(ids.device)),
@@ -70,10 +74,11 @@ class EmbedRows:
         if not 1 <= nrows < 2 ** 31 - 1 or n >= 2 ** 30 or dim > 65536:
             raise ValueError("need 1 <= nrows < 2^31 - 1, fewer than 2^30 ids, at most 65536 columns")
         if out is None:
-            out = torch.empty(nrows, dim, dtype=grad.dtype, device=ids.device)
-        ldo = check_matrix(out, "out", ids.device, grad.dtype)
-        if tuple(out.shape) != (nrows, dim):
-            raise ValueError(f"out has shape {tuple(out.shape)}, expected {(nrows, dim)}")
+            out, ldo = torch.empty(nrows, dim, dtype=grad.dtype, device=ids.device), dim
+        else:
+            ldo = check_matrix(out, "out", ids.device, grad.dtype)
+            if tuple(out.shape) != (nrows, dim):
+                raise ValueError(f"out has shape {tuple(out.shape)}, expected {(nrows, dim)}")
         lib, t = _lib.load(), TYPES[grad.dtype]
         with on_device(ids.device):
             size = lib.w2v_embed_grad_workspace(n, nrows, dim, t)

@@ -9,8 +9,8 @@ from .embed import check_ids, check_matrix
 
 
 def _vector(x, name: str, n: int, device):
-    if not isinstance(x, torch.Tensor) or x.dtype != torch.float32 or tuple(x.shape) != (n,) or x.device != device \
-            or not x.is_contiguous():
+    if not isinstance(x, torch.Tensor) or x.dtype is not torch.float32 or x.dim() != 1 or x.shape[0] != n \
+            or x.get_device() != device.index or not x.is_contiguous():
         raise ValueError(f"{name}: contiguous fp32 [{n}] on {device}")
 
 
@@ -35,7 +35,7 @@ class Softmax:
         check_ids(targets, "targets", targets.dim())
         n, dim = hidden.shape
         labels = 1 if targets.dim() == 1 else targets.shape[1]
-        if targets.shape[0] != n or targets.device != hidden.device:
+        if targets.shape[0] != n or targets.get_device() != hidden.get_device():
             raise ValueError(f"targets has {targets.shape[0]} rows on {targets.device}, hidden {n} on {hidden.device}")
         if weight.shape[1] != dim:
             raise ValueError(f"weight has {weight.shape[1]} columns, hidden {dim}")
@@ -55,10 +55,14 @@ class Softmax:
         """Returns ``(loss, lse)``, fp32 ``[n]`` each, new or in the given tensors."""
         ldh, ldw, n, vocab, dim, labels = Softmax._operands(hidden, weight, targets)
         dev, kind = hidden.device, TYPES[hidden.dtype]
-        loss = torch.empty(n, dtype=torch.float32, device=dev) if loss is None else loss
-        lse = torch.empty(n, dtype=torch.float32, device=dev) if lse is None else lse
-        _vector(loss, "loss", n, dev)
-        _vector(lse, "lse", n, dev)
+        if loss is None:
+            loss = torch.empty(n, dtype=torch.float32, device=dev)
+        else:
+            _vector(loss, "loss", n, dev)
+        if lse is None:
+            lse = torch.empty(n, dtype=torch.float32, device=dev)
+        else:
+            _vector(lse, "lse", n, dev)
         with on_device(dev):
             work, size = Softmax._workspace(n, vocab, dim, labels, kind, False, dev)
             check(_lib.load().w2v_softmax_loss(hidden.data_ptr(), ldh, weight.data_ptr(), ldw, targets.data_ptr(), n,
@@ -74,15 +78,21 @@ class Softmax:
         ldh, ldw, n, vocab, dim, labels = Softmax._operands(hidden, weight, targets)
         dev, kind = hidden.device, TYPES[hidden.dtype]
         _vector(lse, "lse", n, dev)
-        if not isinstance(gloss, torch.Tensor) or gloss.dtype != torch.float32 or gloss.device != dev:
+        if not isinstance(gloss, torch.Tensor) or gloss.dtype is not torch.float32 \
+                or gloss.get_device() != dev.index:
             raise ValueError(f"gloss is an fp32 tensor on {dev}")
         one = gloss.numel() == 1
         if not one:
             _vector(gloss, "gloss", n, dev)
-        dhidden = torch.empty(n, dim, dtype=hidden.dtype, device=dev) if dhidden is None else dhidden
-        dweight = torch.empty(vocab, dim, dtype=hidden.dtype, device=dev) if dweight is None else dweight
-        lddh = check_matrix(dhidden, "dhidden", dev, hidden.dtype)
-        lddw = check_matrix(dweight, "dweight", dev, hidden.dtype)
+        lddh = lddw = dim
+        if dhidden is None:
+            dhidden = torch.empty(n, dim, dtype=hidden.dtype, device=dev)
+        else:
+            lddh = check_matrix(dhidden, "dhidden", dev, hidden.dtype)
+        if dweight is None:
+            dweight = torch.empty(vocab, dim, dtype=hidden.dtype, device=dev)
+        else:
+            lddw = check_matrix(dweight, "dweight", dev, hidden.dtype)
         if tuple(dhidden.shape) != (n, dim) or tuple(dweight.shape) != (vocab, dim):
             raise ValueError(f"dhidden is {(n, dim)} and dweight {(vocab, dim)}")
         with on_device(dev):

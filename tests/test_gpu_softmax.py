@@ -78,7 +78,7 @@ def run(hidden, weight, targets, gloss):
 
 
 SIZES = [(1, 1, 1), (1, 1000, 256), (2, 33, 7), (3, 257, 300), (5, 1001, 64), (8, 4097, 100), (9, 1, 1), (9, 255, 64),
-         (16, 300, 301), (127, 256, 128), (128, 513, 37), (129, 1000, 16), (200, 5003, 300), (300, 777, 1000),
+         (16, 300, 301), (17, 300, 100), (4, 999, 96), (12, 60, 513), (127, 256, 128), (128, 513, 37), (129, 1000, 16), (200, 5003, 300), (300, 777, 1000),
          (515, 2049, 520), (64, 40, 4096)]
 
 
