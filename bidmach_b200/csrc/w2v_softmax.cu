@@ -1042,9 +1042,9 @@ struct Walk {
 };
 
 template <typename T>
-__device__ __forceinline__ void put16(T *to, const float (&v)[16]) {
+__device__ __forceinline__ void put32(T *to, const float (&v)[32]) {
 #pragma unroll
-  for (int b = 0; b < 2; b++) {
+  for (int b = 0; b < 4; b++) {
     float x[8];
 #pragma unroll
     for (int e = 0; e < 8; e++) x[e] = v[b * 8 + e];
@@ -1052,31 +1052,34 @@ __device__ __forceinline__ void put16(T *to, const float (&v)[16]) {
   }
 }
 
-// A column of every other row, from row `first`, of the `rows` that exist.
+// A column of the `rows` rows that exist.
 template <typename T>
-__device__ __forceinline__ void put_rows(T *to, int64_t step, const float *from, int first, int rows) {
-  float x[16];
+__device__ __forceinline__ void put_column(T *to, int64_t step, const float *from, int rows) {
 #pragma unroll
-  for (int i = 0; i < 16; i++) x[i] = from[i * 34];
+  for (int i0 = 0; i0 < 32; i0 += 16) {
+    float x[16];
 #pragma unroll
-  for (int i = 0; i < 16; i++)
-    if (first + 2 * i < rows) to[i * step] = from_float<T>(x[i]);
+    for (int i = 0; i < 16; i++) x[i] = from[(i0 + i) * 33];
+#pragma unroll
+    for (int i = 0; i < 16; i++)
+      if (i0 + i < rows) to[(i0 + i) * step] = from_float<T>(x[i]);
+  }
 }
 
-// 32 rows x 16 columns of a finished tile, a row a lane (row0: lane 0's).  Rows that no wide store fits
-// go through `stage`, 32 x 17 floats of this warp's, so that half a warp writes a row's 16 in one piece.
-__device__ __forceinline__ void put_tile(const Gradients &g, const Side &s, int64_t row0, int at, const float *x, float factor,
-                                         float *stage) {
+// 32 rows x 32 columns of a finished tile, a row a lane (row0: lane 0's).  Rows that no wide store fits
+// go through `stage`, 32 x 33 floats of this warp's, so that the warp writes 32 of a row in one piece.
+__device__ __forceinline__ void put_tile(const Gradients &g, const Side &s, int64_t row0, int at, const float (&x)[32],
+                                         float factor, float *stage) {
   if (at >= g.dim) return;
   const int lane = threadIdx.x & 31;
   const int64_t r = row0 + lane;
-  float v[16];
+  float v[32];
 #pragma unroll
-  for (int e = 0; e < 16; e++) v[e] = x[e];
+  for (int e = 0; e < 32; e++) v[e] = x[e];
   float *acc = s.acc + r * g.ldacc + at;
   if (s.add && r < s.rows) {
 #pragma unroll
-    for (int b = 0; b < 2; b++) {
+    for (int b = 0; b < 4; b++) {
       float old[8];
       load8(acc + b * 8, old);
 #pragma unroll
@@ -1084,40 +1087,38 @@ __device__ __forceinline__ void put_tile(const Gradients &g, const Side &s, int6
     }
   }
   if (!s.last) {
-    if (r < s.rows) put16(acc, v);
+    if (r < s.rows) put32(acc, v);
     return;
   }
 #pragma unroll
-  for (int e = 0; e < 16; e++) v[e] *= factor;
-  if (s.out_wide && at + 16 <= g.dim) {
+  for (int e = 0; e < 32; e++) v[e] *= factor;
+  if (s.out_wide && at + 32 <= g.dim) {
     if (r >= s.rows) return;
     const int64_t to = r * s.ldout + at;
-    if (g.out_type == W2V_F32) put16(static_cast<float *>(s.out) + to, v);
-    else if (g.out_type == W2V_BF16) put16(static_cast<__nv_bfloat16 *>(s.out) + to, v);
-    else put16(static_cast<__half *>(s.out) + to, v);
+    if (g.out_type == W2V_F32) put32(static_cast<float *>(s.out) + to, v);
+    else if (g.out_type == W2V_BF16) put32(static_cast<__nv_bfloat16 *>(s.out) + to, v);
+    else put32(static_cast<__half *>(s.out) + to, v);
     return;
   }
 #pragma unroll
-  for (int e = 0; e < 16; e++) stage[lane * 17 + e] = v[e];
+  for (int e = 0; e < 32; e++) stage[lane * 33 + e] = v[e];
   __syncwarp();
-  const int c = lane % 16, first = lane / 16;
-  const int rows = at + c < g.dim ? (int)min((int64_t)32, s.rows - row0) : 0;
-  const int64_t to = (row0 + first) * s.ldout + at + c;
-  if (g.out_type == W2V_F32) put_rows(static_cast<float *>(s.out) + to, 2 * s.ldout, stage + first * 17 + c, first, rows);
-  else if (g.out_type == W2V_BF16)
-    put_rows(static_cast<__nv_bfloat16 *>(s.out) + to, 2 * s.ldout, stage + first * 17 + c, first, rows);
-  else put_rows(static_cast<__half *>(s.out) + to, 2 * s.ldout, stage + first * 17 + c, first, rows);
+  const int rows = at + lane < g.dim ? (int)max((int64_t)0, min((int64_t)32, s.rows - row0)) : 0;
+  const int64_t to = row0 * s.ldout + at + lane;
+  if (g.out_type == W2V_F32) put_column(static_cast<float *>(s.out) + to, s.ldout, stage + lane, rows);
+  else if (g.out_type == W2V_BF16) put_column(static_cast<__nv_bfloat16 *>(s.out) + to, s.ldout, stage + lane, rows);
+  else put_column(static_cast<__half *>(s.out) + to, s.ldout, stage + lane, rows);
   __syncwarp();
 }
 
-constexpr int kGradSmem = smem_bytes(kMostStages, 0);
+constexpr int kGradStages = 5, kGradSmem = smem_bytes(kGradStages, 0);
 
 template <bool SEGMENTS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) grad_kernel(const __grid_constant__ Gradients g) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char *smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
   __shared__ Pipe pipe;
-  __shared__ float stage_s[8][32 * 17];
+  __shared__ float stage_s[8][32 * 33];
   volatile int *gave_up = &pipe.gave_up;
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
   const uint32_t tmem = pair_begin(pipe);
@@ -1127,7 +1128,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) grad
 
   if (warp == 0) {
     if (elected()) {
-      Ring<kMostStages> ring{pipe, smem, gave_up};
+      Ring<kGradStages> ring{pipe, smem, gave_up};
       bool ok = true;
       // each CTA brings its own rows of d and half of the operand's columns
       const int half_n = g.ntile / 2, groups = (half_n + 63) / 64;
@@ -1156,7 +1157,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) grad
     __syncwarp();
   } else if (warp == 1) {
     if (rank == 0 && elected()) {
-      Issue<kMostStages> issue{pipe, gave_up, tmem, smem_addr(smem)};
+      Issue<kGradStages> issue{pipe, gave_up, tmem, smem_addr(smem)};
       bool ok = true;
       while (ok && walk.next(p)) {
         const bool mn = g.side[p.side].a_mn;
@@ -1189,7 +1190,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) grad
       auto finish = [&](int ch, const float (&x)[32]) {
         if (p.slot < 0) {
           put_tile(g, s, row0, n * g.ntile + ch * 32, x, factor[p.side], stage);
-          put_tile(g, s, row0, n * g.ntile + ch * 32 + 16, x + 16, factor[p.side], stage);
         } else {
 #pragma unroll
           for (int b = 0; b < 4; b++) {
