@@ -981,7 +981,7 @@ struct Side {
 
 struct Gradients {
   Side side[2];             // dW, dH
-  int nt, ntile;            // column tiles, and their width (a multiple of 32)
+  int nt, ntile, nlast;     // column tiles, their width and the last one's (multiples of 32)
   int npairs, sharers;      // pairs of CTAs; how many of them share what is left
   int64_t left;             // its blocks of K
   int pairs, segment;       // pairs of parts; blocks of K that are accumulated in tensor memory at a time
@@ -989,6 +989,7 @@ struct Gradients {
   int64_t ldacc;
   float *scratch;           // kM x kN for each CTA
   float *pieces;            // [pair][2][kPairM][ntile]
+  __device__ __forceinline__ int width(int n) const { return n == nt - 1 ? nlast : ntile; }
 };
 
 struct Piece {
@@ -1131,10 +1132,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) grad
       Ring<kGradStages> ring{pipe, smem, gave_up};
       bool ok = true;
       // each CTA brings its own rows of d and half of the operand's columns
-      const int half_n = g.ntile / 2, groups = (half_n + 63) / 64;
-      const unsigned bytes = 2 * (kBytesA + groups * 8192);
       while (ok && walk.next(p)) {
         const Side &s = g.side[p.side];
+        const int half_n = g.width(p.tile % g.nt) / 2, groups = (half_n + 63) / 64;
+        const unsigned bytes = 2 * (kBytesA + groups * 8192);
         const int row = p.tile / g.nt * kPairM + rank * kM, col = p.tile % g.nt * g.ntile + rank * half_n;
         for (int k0 = p.k0; ok && k0 < p.k1; k0 += g.segment)
           for (int q = 0; ok && q < g.pairs; q++)
@@ -1161,7 +1162,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) grad
       bool ok = true;
       while (ok && walk.next(p)) {
         const bool mn = g.side[p.side].a_mn;
-        const uint32_t idesc = mma_desc(g.bf16, mn, true, kPairM, g.ntile);
+        const uint32_t idesc = mma_desc(g.bf16, mn, true, kPairM, g.width(p.tile % g.nt));
         const uint64_t da = issue.desc(0, mn), db = issue.desc(kBytesA, true);
         const uint32_t step_a = mn ? 2048 >> 4 : 32 >> 4;
         for (int k0 = p.k0; ok && k0 < p.k1; k0 += g.segment) {
@@ -1177,13 +1178,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) grad
     __syncwarp();
   } else if (warp >= 4) {
     const int half = (warp - 4) / 4, row = (warp & 3) * 32;
-    const int chunks = g.ntile / 32;
     float *stage = stage_s[warp - 4];
     const float factor[2] = {rescale_of(g.side[0].rescale), rescale_of(g.side[1].rescale)};
     Reader reader(pipe, gave_up, tmem);
     while (walk.next(p)) {
       const Side &s = g.side[p.side];
-      const int n = p.tile % g.nt;
+      const int n = p.tile % g.nt, chunks = g.width(n) / 32;
       const int64_t row0 = (int64_t)(p.tile / g.nt) * kPairM + rank * kM + row;
       float *piece = g.pieces + ((int64_t)(walk.pair * 2 + max(p.slot, 0)) * kPairM + rank * kM + row + lane) * g.ntile;
       // 32 columns of the sum over the piece
@@ -1266,7 +1266,7 @@ __global__ void __launch_bounds__(256) pieces_kernel(const __grid_constant__ Gra
   if (r >= s.rows) return;
   const float factor = rescale_of(s.rescale);
   const int col = lane * 8, at = tile % g.nt * g.ntile + col;
-  if (col >= g.ntile || at >= g.dim) return;
+  if (col >= g.width(tile % g.nt) || at >= g.dim) return;
   float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
   for (int q = first; q <= last; q += 4) {
     float x[4][8];
@@ -1417,13 +1417,16 @@ struct Layout {
   int64_t scalars, hs, ws, parts, probs, scratch, pieces, acc_h, acc_w, total;
   int width, nparts;         // staged operands
   int64_t rows, words;       // of a piece of d
-  int nt, ntile;
+  int nt, ntile, nlast;
 };
 
-// Column tiles of a gradient: as few as hold dim, equally wide.
-void column_tiles(int dim, int *nt, int *ntile) {
+// Column tiles of a gradient: as wide as they can be, the rest in a last one.  A block of K of any width up
+// to 128 + 128 columns costs at least the time that d's part of it takes to arrive, so two of 160 take
+// as long as two of 256 (301 columns at 1023 x 50021: 94 us as 160 + 160, 87 as 256 + 64).
+void column_tiles(int dim, int *nt, int *ntile, int *nlast) {
   *nt = (dim + kN - 1) / kN;
-  *ntile = (int)up((dim + *nt - 1) / *nt, 32);
+  *nlast = (int)up(dim - (*nt - 1) * kN, 32);
+  *ntile = *nt > 1 ? kN : *nlast;
 }
 
 Layout plan(const Shape &x, bool grad) {
@@ -1459,7 +1462,7 @@ Layout plan(const Shape &x, bool grad) {
     const int64_t most = std::max<int64_t>(kN, kProbBytes / (l.rows * bytes));
     const int64_t pieces = std::max<int64_t>(1, (x.vocab + most * 5 / 4 - 1) / (most * 5 / 4));
     l.words = up((x.vocab + pieces - 1) / pieces, kN);
-    column_tiles(x.dim, &l.nt, &l.ntile);
+    column_tiles(x.dim, &l.nt, &l.ntile, &l.nlast);
     const int64_t cols = (int64_t)l.nt * l.ntile * 4;
     l.probs = take(l.rows * l.words * bytes);
     if (x.type == W2V_F32) l.scratch = take((int64_t)sm_pairs() * kPairM * kN * 4);
@@ -1653,6 +1656,7 @@ int run_grad(const Shape &x, const Layout &l, const void *h, int64_t ldh, const 
   Gradients g{};
   g.nt = l.nt;
   g.ntile = l.ntile;
+  g.nlast = l.nlast;
   g.npairs = sm_pairs();
   g.pairs = split ? 3 : 1;
   g.segment = split ? kSegment : 1 << 30;

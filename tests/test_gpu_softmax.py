@@ -222,11 +222,11 @@ def test_gradient_against_differences(n, vocab, dim, t):
 
 
 def test_equal_calls_streams_and_graphs():
-    """Two calls at once on two streams, and two captured graphs replayed side by side, give the bits of
-    the call alone."""
+    """Calls at once on several streams, and captured graphs replayed side by side, give the bits of the call
+    alone."""
     from bidmach_b200 import Softmax
     sets = []
-    for n, vocab, dim, t in ((300, 3000, 100, "bf16"), (260, 2000, 70, "f32")):
+    for n, vocab, dim, t in ((300, 3000, 100, "bf16"), (260, 2000, 70, "f32"), (12, 3000, 50, "f32"), (3, 900, 64, "f16")):
         x = [v.cuda() for v in inputs(n, vocab, dim, 2, t)]
         sets.append((x, run(*x)))
     torch.cuda.synchronize()
@@ -235,7 +235,7 @@ def test_equal_calls_streams_and_graphs():
         loss, lse = Softmax.loss(*x[:3])
         return (loss, lse, *Softmax.grad(*x[:3], lse, x[3]))
 
-    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    streams, got = [torch.cuda.Stream() for _ in sets], []
     for _ in range(3):
         for s, (x, want) in zip(streams, sets):
             with torch.cuda.stream(s):
