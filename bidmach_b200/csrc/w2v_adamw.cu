@@ -10,6 +10,9 @@
 // table in device memory: nothing has to be uploaded before a step, and a captured step holds
 // its own.
 //
+// Measured: 51 million elements with fp32 moments 217 us (6.6 TB/s); 300 million with 8-bit moments 880 us
+// (5.5 TB/s; the codes cost about 40 of 70 instructions an element), their values as fp32 491 us.
+//
 // Each operation on the moments is rounded on its own (no contraction to fused multiply-adds), so the
 // result does not depend on how a compiler groups them: next to the border of two 8-bit codes that
 // would change a stored moment by a whole step.
