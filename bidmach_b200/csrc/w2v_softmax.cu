@@ -552,8 +552,8 @@ struct Pipe {
   int gave_up;
 };
 
-// Returns the address of the pair's tensor memory.
-__device__ __forceinline__ uint32_t pair_begin(Pipe &s) {
+// Returns the address of the pair's tensor memory, which `readers` warps of each CTA read.
+__device__ __forceinline__ uint32_t pair_begin(Pipe &s, int readers) {
   if (threadIdx.x == 0) {
     for (int i = 0; i < kMostStages; i++) {
       mbar_init(&s.full[i], 1);
@@ -561,7 +561,7 @@ __device__ __forceinline__ uint32_t pair_begin(Pipe &s) {
     }
     for (int i = 0; i < 2; i++) {
       mbar_init(&s.tfull[i], 1);
-      mbar_init(&s.tempty[i], 16);
+      mbar_init(&s.tempty[i], 2 * readers);
       mbar_init(&s.hfull[i], 2);
       mbar_init(&s.hempty[i], 8);
     }
@@ -686,13 +686,15 @@ struct Reader {
     tmem_after_sync();
   }
   // A warp that gave up reads NaN: nothing that was not computed passes for a result.
-  __device__ __forceinline__ void fetch(int col, float (&x)[32]) const {
+  template <int N>
+  __device__ __forceinline__ void fetch(int col, float (&x)[N]) const {
     if (ok) {
-      tmem_load32(lanes + (local & 1) * 256 + col, x);
+      if constexpr (N == 32) tmem_load32(lanes + (local & 1) * 256 + col, x);
+      else tmem_load16(lanes + (local & 1) * 256 + col, x);
       tmem_wait_load();
     } else {
 #pragma unroll
-      for (int i = 0; i < 32; i++) x[i] = __int_as_float(0x7fffffff);
+      for (int i = 0; i < N; i++) x[i] = __int_as_float(0x7fffffff);
     }
   }
   __device__ __forceinline__ void end() {
@@ -788,7 +790,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) prod
   volatile int *gave_up = &pipe.gave_up;
   constexpr int STAGES = kProductStages<USE>;
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
-  const uint32_t tmem = pair_begin(pipe);
+  const uint32_t tmem = pair_begin(pipe, 8);
   const int rank = (int)cluster_rank(), pair = blockIdx.x / 2, npairs = gridDim.x / 2;
   const int tiles = p.mt * p.nt;
   // pairs that run together share a few tiles of W, against all rows
@@ -990,7 +992,6 @@ struct Gradients {
   int pairs, segment;       // pairs of parts; blocks of K that are accumulated in tensor memory at a time
   int bf16, strip, dim, out_type;
   int64_t ldacc;
-  float *scratch;           // kM x kN for each CTA
   float *pieces;            // [pair][2][kPairM][ntile]
   __device__ __forceinline__ int width(int n) const { return n == nt - 1 ? nlast : ntile; }
 };
@@ -1046,9 +1047,9 @@ struct Walk {
 };
 
 template <typename T>
-__device__ __forceinline__ void put32(T *to, const float (&v)[32]) {
+__device__ __forceinline__ void put16(T *to, const float (&v)[16]) {
 #pragma unroll
-  for (int b = 0; b < 4; b++) {
+  for (int b = 0; b < 2; b++) {
     float x[8];
 #pragma unroll
     for (int e = 0; e < 8; e++) x[e] = v[b * 8 + e];
@@ -1056,34 +1057,31 @@ __device__ __forceinline__ void put32(T *to, const float (&v)[32]) {
   }
 }
 
-// A column of the `rows` rows that exist.
+// A column of every other row, from row `first`, of the `rows` that exist.
 template <typename T>
-__device__ __forceinline__ void put_column(T *to, int64_t step, const float *from, int rows) {
+__device__ __forceinline__ void put_rows(T *to, int64_t step, const float *from, int first, int rows) {
+  float x[16];
 #pragma unroll
-  for (int i0 = 0; i0 < 32; i0 += 16) {
-    float x[16];
+  for (int i = 0; i < 16; i++) x[i] = from[i * 34];
 #pragma unroll
-    for (int i = 0; i < 16; i++) x[i] = from[(i0 + i) * 33];
-#pragma unroll
-    for (int i = 0; i < 16; i++)
-      if (i0 + i < rows) to[(i0 + i) * step] = from_float<T>(x[i]);
-  }
+  for (int i = 0; i < 16; i++)
+    if (first + 2 * i < rows) to[i * step] = from_float<T>(x[i]);
 }
 
-// 32 rows x 32 columns of a finished tile, a row a lane (row0: lane 0's).  Rows that no wide store fits
-// go through `stage`, 32 x 33 floats of this warp's, so that the warp writes 32 of a row in one piece.
-__device__ __forceinline__ void put_tile(const Gradients &g, const Side &s, int64_t row0, int at, const float (&x)[32],
-                                         float factor, float *stage) {
+// 32 rows x 16 columns of a finished tile, a row a lane (row0: lane 0's).  Rows that no wide store fits
+// go through `stage`, 32 x 17 floats of this warp's, so that half a warp writes a row's 16 in one piece.
+__device__ __forceinline__ void put_tile(const Gradients &g, const Side &s, int64_t row0, int at, const float *x, float factor,
+                                         float *stage) {
   if (at >= g.dim) return;
   const int lane = threadIdx.x & 31;
   const int64_t r = row0 + lane;
-  float v[32];
+  float v[16];
 #pragma unroll
-  for (int e = 0; e < 32; e++) v[e] = x[e];
+  for (int e = 0; e < 16; e++) v[e] = x[e];
   float *acc = s.acc + r * g.ldacc + at;
   if (s.add && r < s.rows) {
 #pragma unroll
-    for (int b = 0; b < 4; b++) {
+    for (int b = 0; b < 2; b++) {
       float old[8];
       load8(acc + b * 8, old);
 #pragma unroll
@@ -1091,41 +1089,52 @@ __device__ __forceinline__ void put_tile(const Gradients &g, const Side &s, int6
     }
   }
   if (!s.last) {
-    if (r < s.rows) put32(acc, v);
+    if (r < s.rows) put16(acc, v);
     return;
   }
 #pragma unroll
-  for (int e = 0; e < 32; e++) v[e] *= factor;
-  if (s.out_wide && at + 32 <= g.dim) {
+  for (int e = 0; e < 16; e++) v[e] *= factor;
+  if (s.out_wide && at + 16 <= g.dim) {
     if (r >= s.rows) return;
     const int64_t to = r * s.ldout + at;
-    if (g.out_type == W2V_F32) put32(static_cast<float *>(s.out) + to, v);
-    else if (g.out_type == W2V_BF16) put32(static_cast<__nv_bfloat16 *>(s.out) + to, v);
-    else put32(static_cast<__half *>(s.out) + to, v);
+    if (g.out_type == W2V_F32) put16(static_cast<float *>(s.out) + to, v);
+    else if (g.out_type == W2V_BF16) put16(static_cast<__nv_bfloat16 *>(s.out) + to, v);
+    else put16(static_cast<__half *>(s.out) + to, v);
     return;
   }
 #pragma unroll
-  for (int e = 0; e < 32; e++) stage[lane * 33 + e] = v[e];
+  for (int e = 0; e < 16; e++) stage[lane * 17 + e] = v[e];
   __syncwarp();
-  const int rows = at + lane < g.dim ? (int)max((int64_t)0, min((int64_t)32, s.rows - row0)) : 0;
-  const int64_t to = row0 * s.ldout + at + lane;
-  if (g.out_type == W2V_F32) put_column(static_cast<float *>(s.out) + to, s.ldout, stage + lane, rows);
-  else if (g.out_type == W2V_BF16) put_column(static_cast<__nv_bfloat16 *>(s.out) + to, s.ldout, stage + lane, rows);
-  else put_column(static_cast<__half *>(s.out) + to, s.ldout, stage + lane, rows);
+  const int c = lane % 16, first = lane / 16;
+  const int rows = at + c < g.dim ? (int)max((int64_t)0, min((int64_t)32, s.rows - row0)) : 0;
+  const int64_t to = (row0 + first) * s.ldout + at + c;
+  const float *from = stage + first * 17 + c;
+  if (g.out_type == W2V_F32) put_rows(static_cast<float *>(s.out) + to, 2 * s.ldout, from, first, rows);
+  else if (g.out_type == W2V_BF16) put_rows(static_cast<__nv_bfloat16 *>(s.out) + to, 2 * s.ldout, from, first, rows);
+  else put_rows(static_cast<__half *>(s.out) + to, 2 * s.ldout, from, first, rows);
   __syncwarp();
 }
 
 constexpr int kGradStages = 5, kGradSmem = smem_bytes(kGradStages, 0);
 
+// SEGMENTS (fp32): the tensor cores truncate what they accumulate, so after `segment` blocks of K the sum
+// moves to registers, where it is rounded: sixteen warps, 64 columns of a row a lane.  dH of 4096 x 100000
+// x 256 is then 1.2e-6 off in norm (2 blocks; 4: 2.7e-6, 8: 5.8e-6; an fp32 product: 6.5e-6), dW 1.6e-7 (fp32
+// product 5.4e-7), and takes 2.26 ms (4 blocks: 2.20).
 template <bool SEGMENTS>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) grad_kernel(const __grid_constant__ Gradients g) {
+constexpr int kGradReaders = SEGMENTS ? 16 : 8;
+template <bool SEGMENTS>
+constexpr int kGradThreads = 128 + 32 * kGradReaders<SEGMENTS>;
+
+template <bool SEGMENTS>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGradThreads<SEGMENTS>, 1) grad_kernel(const __grid_constant__ Gradients g) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char *smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
   __shared__ Pipe pipe;
-  __shared__ float stage_s[8][32 * 33];
+  __shared__ float stage_s[kGradReaders<SEGMENTS>][32 * 17];
   volatile int *gave_up = &pipe.gave_up;
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
-  const uint32_t tmem = pair_begin(pipe);
+  const uint32_t tmem = pair_begin(pipe, kGradReaders<SEGMENTS>);
   const int rank = (int)cluster_rank();
   Walk walk(g, blockIdx.x / 2);
   Piece p;
@@ -1180,70 +1189,60 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) grad
     }
     __syncwarp();
   } else if (warp >= 4) {
-    const int half = (warp - 4) / 4, row = (warp & 3) * 32;
+    const int part = (warp - 4) / 4, row = (warp & 3) * 32;
     float *stage = stage_s[warp - 4];
     const float factor[2] = {rescale_of(g.side[0].rescale), rescale_of(g.side[1].rescale)};
     Reader reader(pipe, gave_up, tmem);
     while (walk.next(p)) {
       const Side &s = g.side[p.side];
-      const int n = p.tile % g.nt, chunks = g.width(n) / 32;
+      const int n = p.tile % g.nt, width = g.width(n);
       const int64_t row0 = (int64_t)(p.tile / g.nt) * kPairM + rank * kM + row;
       float *piece = g.pieces + ((int64_t)(walk.pair * 2 + max(p.slot, 0)) * kPairM + rank * kM + row + lane) * g.ntile;
-      // 32 columns of the sum over the piece
-      auto finish = [&](int ch, const float (&x)[32]) {
+      // 16 columns of the sum over the piece
+      auto finish = [&](int col, const float *x) {
         if (p.slot < 0) {
-          put_tile(g, s, row0, n * g.ntile + ch * 32, x, factor[p.side], stage);
+          put_tile(g, s, row0, n * g.ntile + col, x, factor[p.side], stage);
         } else {
 #pragma unroll
-          for (int b = 0; b < 4; b++) {
+          for (int b = 0; b < 2; b++) {
             float v[8];
 #pragma unroll
             for (int e = 0; e < 8; e++) v[e] = x[b * 8 + e];
-            store8(piece + ch * 32 + b * 8, v);
+            store8(piece + col + b * 8, v);
           }
         }
       };
       if (!SEGMENTS) {
         reader.begin();
-        for (int ch = half; ch < chunks; ch += 2) {
+        for (int ch = part; ch < width / 32; ch += 2) {
           float x[32];
           reader.fetch(ch * 32, x);
-          finish(ch, x);
+          finish(ch * 32, x);
+          finish(ch * 32 + 16, x + 16);
         }
         reader.end();
       } else {
-        // the tensor cores truncate what they accumulate: after `segment` blocks of K the sum goes on in
-        // fp32 with rounding, in a scratch of the CTA's own that stays in L2 (a thread's eight values
-        // side by side, a warp's in one piece); registers for it would spill
-        float *mine = g.scratch + (int64_t)blockIdx.x * kM * kN + (threadIdx.x - 128) * 8;
+        float acc[4][16];
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+          for (int e = 0; e < 16; e++) acc[i][e] = 0.f;
         for (int k0 = p.k0; k0 < p.k1; k0 += g.segment) {
           reader.begin();
-          for (int ch = half; ch < chunks; ch += 2) {
-            float x[32], old[4][8];
-            float *at = mine + ch / 2 * (4 * 256 * 8);
-            if (k0 > p.k0) {
+          if (part * 64 < width) {
 #pragma unroll
-              for (int b = 0; b < 4; b++) load8(at + b * (256 * 8), old[b]);
-            }
-            reader.fetch(ch * 32, x);
-            if (k0 > p.k0) {
+            for (int i = 0; i < 4; i++) {
+              float x[16];
+              reader.fetch(part * 64 + i * 16, x);
 #pragma unroll
-              for (int i = 0; i < 32; i++) x[i] += old[i / 8][i % 8];
-            }
-            if (k0 + g.segment < p.k1) {
-#pragma unroll
-              for (int b = 0; b < 4; b++) {
-                float v[8];
-#pragma unroll
-                for (int e = 0; e < 8; e++) v[e] = x[b * 8 + e];
-                store8(at + b * (256 * 8), v);
-              }
-            } else {
-              finish(ch, x);
+              for (int e = 0; e < 16; e++) acc[i][e] += x[e];
             }
           }
           reader.end();
         }
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          if (part * 64 + i * 16 < width) finish(part * 64 + i * 16, acc[i]);
       }
     }
   }
@@ -1382,7 +1381,7 @@ int launch_gradients(const Gradients &g, cudaStream_t s) {
   int err = allow_smem<grad_kernel<split>>(kGradSmem);
   if (err) return err;
   const bool whole = g.side[0].whole || g.side[1].whole;
-  grad_kernel<split><<<2 * (whole ? g.npairs : g.sharers), kMmaThreads, kGradSmem, s>>>(g);
+  grad_kernel<split><<<2 * (whole ? g.npairs : g.sharers), kGradThreads<split>, kGradSmem, s>>>(g);
   count_launch(1);
   err = (int)cudaGetLastError();
   const int rest = g.side[0].rest(g.npairs) + g.side[1].rest(g.npairs);
@@ -1404,7 +1403,7 @@ bool good_shape(const Shape &x) {
 constexpr int64_t kLossRows = 16384;            // rows whose parts are kept at a time
 constexpr int64_t kGradRows = 8192;             // rows of a piece of d
 constexpr int64_t kProbBytes = (int64_t)256 << 20;
-constexpr int kSegment = 8;                     // fp32 gradients: blocks of K between two roundings
+constexpr int kSegment = 2;                     // fp32 gradients: blocks of K between two roundings
 
 int few_blocks(int64_t vocab) {
   const int64_t need = (vocab + kFewThreads / 32 * kFewWords - 1) / (kFewThreads / 32 * kFewWords);
@@ -1417,7 +1416,7 @@ int few_rows_of(int64_t n) { return n <= 1 ? 1 : n <= 2 ? 2 : n <= 4 ? 4 : 8; }
 bool few_rows(const Shape &x) { return x.n <= (x.type == W2V_F32 ? 2 * kFewRows : 4); }
 
 struct Layout {
-  int64_t scalars, hs, ws, parts, probs, scratch, pieces, acc_h, acc_w, total;
+  int64_t scalars, hs, ws, parts, probs, pieces, acc_h, acc_w, total;
   int width, nparts;         // staged operands
   int64_t rows, words;       // of a piece of d
   int nt, ntile, nlast;
@@ -1468,7 +1467,6 @@ Layout plan(const Shape &x, bool grad) {
     column_tiles(x.dim, &l.nt, &l.ntile, &l.nlast);
     const int64_t cols = (int64_t)l.nt * l.ntile * 4;
     l.probs = take(l.rows * l.words * bytes);
-    if (x.type == W2V_F32) l.scratch = take((int64_t)sm_pairs() * kPairM * kN * 4);
     l.pieces = take((int64_t)sm_pairs() * 2 * kPairM * l.ntile * 4);
     if (l.words < x.vocab) l.acc_h = take(l.rows * cols);
     if (l.rows < x.n) l.acc_w = take(up(x.vocab, kPairM) * cols);
@@ -1668,7 +1666,6 @@ int run_grad(const Shape &x, const Layout &l, const void *h, int64_t ldh, const 
   g.dim = x.dim;
   g.out_type = x.type;
   g.ldacc = (int64_t)l.nt * l.ntile;
-  g.scratch = reinterpret_cast<float *>(ws + l.scratch);
   g.pieces = reinterpret_cast<float *>(ws + l.pieces);
   for (int i = 0; i < 2 && !err; i++) {
     Side &side = g.side[i];
