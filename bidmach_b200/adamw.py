@@ -66,7 +66,8 @@ class AdamW:
     ``params``: contiguous CUDA tensors of one device, fp32, bf16 or fp16, none overlapping another.
     ``state``, when given, is the state to go on from (its tensors are used in place): ``t`` steps
     done, and lists ``m`` and ``v`` like the parameters: fp32, or for 8 bits uint8 of as many
-    elements, with lists ``mscale`` and ``vscale`` of fp32, one for every 256 elements.  Without it
+    elements, with lists ``mscale`` and ``vscale`` of fp32, one for every 256 elements, none overlapping
+    another or a parameter.  Without it
     the moments start at zero.  The arithmetic is fp32; a 16-bit parameter is rounded to nearest
     once a step, so a step smaller than half of its last place leaves it as it is.
 
@@ -89,15 +90,15 @@ class AdamW:
                 raise ValueError("parameters are fp32, bf16 or fp16 tensors")
             if not p.is_contiguous():
                 raise ValueError("parameters have to be contiguous")
-        spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in self.params if p.numel())
-        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
-            raise ValueError("two parameters overlap")
+        self._apart(self.params, "two parameters overlap")
         if any(not p.is_cuda for p in self.params):
             raise ValueError("AdamW expects CUDA tensors")
         self.device = self.params[0].device
         if any(p.device != self.device for p in self.params):
             raise ValueError("parameters on more than one device")
         self.m, self.v, self.mscale, self.vscale, t = self._state(state)
+        self._apart([*self.params, *self.m, *self.v, *(self.mscale or ()), *(self.vscale or ())],
+                    "a tensor of the state overlaps another or a parameter")
         n = len(self.params)
         self._sizes = [p.numel() for p in self.params]
         self._types = [p.dtype for p in self.params]
@@ -144,6 +145,12 @@ class AdamW:
             else (None, None)
         return given("m", sizes, dtype), given("v", sizes, dtype), *scales, int(state["t"])
 
+    @staticmethod
+    def _apart(tensors, what):
+        spans = sorted((x.data_ptr(), x.data_ptr() + x.numel() * x.element_size()) for x in tensors if x.numel())
+        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise ValueError(what)
+
     def _like(self, tensors, sizes, what):
         """Refuses tensors that are not contiguous ones of this device and these sizes (in few passes:
         a model may have hundreds)."""
@@ -153,8 +160,9 @@ class AdamW:
 
     def step(self, grads, lrate: "float | torch.Tensor | None" = None):
         """One step.  ``grads``: a tensor for each parameter, same number of elements, contiguous, fp32
-        or the parameter's type.  ``lrate`` replaces the option's: a number, or a one-element fp32
-        tensor of the device, read when the step runs."""
+        or the parameter's type, in memory of its own (one tensor may serve several parameters).
+        ``lrate`` replaces the option's: a number, or a one-element fp32 tensor of the device, read when
+        the step runs."""
         n = len(self._sizes)
         if len(grads) != n:
             raise ValueError(f"{len(grads)} gradients for {n} parameters")
@@ -183,7 +191,8 @@ class AdamW:
 
     def moments(self, mout=None, vout=None):
         """Both moments as fp32 values: lists (m, v).  With 32 bits these are the state itself; with 8
-        the codes are decoded into new tensors or into the lists ``mout`` and ``vout``."""
+        the codes are decoded into new tensors or into the lists ``mout`` and ``vout``, whose tensors
+        overlap neither each other nor the state."""
         if self.opts.bits == 32:
             if mout is not None or vout is not None:
                 raise ValueError("32-bit moments are not copied: mout and vout are for 8 bits")

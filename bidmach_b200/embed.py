@@ -37,9 +37,37 @@ def check_ids(x, name: str, dim: int):
         raise ValueError(f"{name} is not contiguous")
 
 
+def _meet(a, b) -> bool:
+    """Whether an element of `a` shares memory with one of `b`: contiguous tensors, or matrices with
+    contiguous rows.  Two sets of columns of one buffer do not; others whose ranges cross count as met."""
+    spans = []
+    for x in (a, b):
+        if x.numel() == 0:
+            return False
+        matrix = x.dim() == 2 and x.shape[0] > 1
+        row = (x.shape[1] if matrix else x.numel()) * x.element_size()
+        ld, rows = (x.stride(0) * x.element_size(), x.shape[0]) if matrix else (row, 1)
+        spans.append((x.data_ptr(), x.data_ptr() + (rows - 1) * ld + row, ld, row))
+    (a0, a1, lda, rowa), (b0, b1, ldb, rowb) = spans
+    if a1 <= b0 or b1 <= a0:
+        return False
+    if lda != ldb:
+        return True
+    off = (b0 - a0) % lda
+    return off < rowa or off + rowb > lda
+
+
+def check_apart(name: str, out, **others):
+    """Refuses an output that shares memory with another tensor of the call."""
+    for other, x in others.items():
+        if _meet(out, x):
+            raise ValueError(f"{name} overlaps {other}")
+
+
 class EmbedRows:
     """Static methods only.  ``ids``: int32, one for each row; an id outside the matrix (-1 marks a
-    dropped word) gives a row of zeros and takes no part in the gradient."""
+    dropped word) gives a row of zeros and takes no part in the gradient.
+    ``out``, where one is given, shares no memory with the inputs."""
 
     @staticmethod
     def forward(ids, matrix, out=None):
@@ -55,6 +83,7 @@ class EmbedRows:
             ldo = check_matrix(out, "out", ids.device, matrix.dtype)
             if tuple(out.shape) != (n, dim):
                 raise ValueError(f"out has shape {tuple(out.shape)}, expected {(n, dim)}")
+            check_apart("out", out, ids=ids, matrix=matrix)
         with on_device(ids.device):
             check(_lib.load().w2v_embed_rows(ids.data_ptr(), n, matrix.data_ptr(), ldm, vocab, dim,
                                              TYPES[matrix.dtype], out.data_ptr(), ldo, stream_of(ids.device)),
@@ -79,6 +108,7 @@ class EmbedRows:
             ldo = check_matrix(out, "out", ids.device, grad.dtype)
             if tuple(out.shape) != (nrows, dim):
                 raise ValueError(f"out has shape {tuple(out.shape)}, expected {(nrows, dim)}")
+            check_apart("out", out, ids=ids, grad=grad)
         lib, t = _lib.load(), TYPES[grad.dtype]
         with on_device(ids.device):
             size = lib.w2v_embed_grad_workspace(n, nrows, dim, t)

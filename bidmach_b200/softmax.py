@@ -5,7 +5,7 @@ import torch
 
 from . import _lib
 from .adamw import TYPES, check, on_device, stream_of
-from .embed import check_ids, check_matrix
+from .embed import check_apart, check_ids, check_matrix
 
 
 def _vector(x, name: str, n: int, device):
@@ -24,7 +24,8 @@ class Softmax:
     ``targets`` int32 ``[n]`` or ``[n, labels]``.  A target outside ``[0, vocab)`` (-1 by convention) stands
     for none; a row may have none (its loss and gradient are zero) or the same word more than once.
     fp32 operands are multiplied to 22 bits and accumulated in fp32; 16-bit ones are multiplied exactly.
-    Every row takes part in the products, so ``hidden`` has to be finite in rows without targets too."""
+    Every row takes part in the products, so ``hidden`` has to be finite in rows without targets too.
+    Outputs that are given share no memory with the inputs or with each other."""
 
     @staticmethod
     def _operands(hidden, weight, targets):
@@ -59,10 +60,12 @@ class Softmax:
             loss = torch.empty(n, dtype=torch.float32, device=dev)
         else:
             _vector(loss, "loss", n, dev)
+            check_apart("loss", loss, hidden=hidden, weight=weight, targets=targets)
         if lse is None:
             lse = torch.empty(n, dtype=torch.float32, device=dev)
         else:
             _vector(lse, "lse", n, dev)
+            check_apart("lse", lse, hidden=hidden, weight=weight, targets=targets, loss=loss)
         with on_device(dev):
             work, size = Softmax._workspace(n, vocab, dim, labels, kind, False, dev)
             check(_lib.load().w2v_softmax_loss(hidden.data_ptr(), ldh, weight.data_ptr(), ldw, targets.data_ptr(), n,
@@ -85,6 +88,7 @@ class Softmax:
         if not one:
             _vector(gloss, "gloss", n, dev)
         lddh = lddw = dim
+        given = dhidden is not None, dweight is not None
         if dhidden is None:
             dhidden = torch.empty(n, dim, dtype=hidden.dtype, device=dev)
         else:
@@ -95,6 +99,11 @@ class Softmax:
             lddw = check_matrix(dweight, "dweight", dev, hidden.dtype)
         if tuple(dhidden.shape) != (n, dim) or tuple(dweight.shape) != (vocab, dim):
             raise ValueError(f"dhidden is {(n, dim)} and dweight {(vocab, dim)}")
+        inputs = dict(hidden=hidden, weight=weight, targets=targets, lse=lse, gloss=gloss)
+        if given[0]:
+            check_apart("dhidden", dhidden, **inputs, dweight=dweight)
+        if given[1]:
+            check_apart("dweight", dweight, **inputs, dhidden=dhidden)
         with on_device(dev):
             work, size = Softmax._workspace(n, vocab, dim, labels, kind, True, dev)
             check(_lib.load().w2v_softmax_grad(hidden.data_ptr(), ldh, weight.data_ptr(), ldw, targets.data_ptr(), n,

@@ -428,7 +428,8 @@ int64_t bidmach_lz4_decompress(const void *src, int64_t n, void *dst, int64_t ca
  * address must be a multiple of 256) and may be reused once the call's work
  * has finished, so calls that can run at the same time need workspaces of
  * their own.  Matrices are rows of contiguous elements, `ld` elements apart
- * (ld >= dim); any alignment works, multiples of 32 bytes are fastest.
+ * (ld >= dim); any alignment works, multiples of 32 bytes are fastest.  Outputs
+ * share no memory with inputs or other outputs (rows of two matrices may alternate).
  * Return value: 0, 1 for arguments that are refused, or a cudaError_t.
  * ---------------------------------------------------------------------- */
 enum { W2V_F32 = 0, W2V_BF16 = 1, W2V_F16 = 2 };   /* element types */

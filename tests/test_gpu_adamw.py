@@ -229,3 +229,12 @@ def test_refusals_on_the_device():
         AdamW([p], state={"t": 0, "m": [torch.zeros(511, device="cuda")], "v": [p.clone()]})
     with pytest.raises(ValueError):
         opt.moments(mout=[p.clone()])
+
+
+def test_moments_that_share_memory_are_refused():
+    from bidmach_b200 import AdamW
+    p = torch.zeros(300, device="cuda")
+    x = torch.zeros(300, device="cuda")
+    for m, v in ((x, x), (p, x), (x, p)):
+        with pytest.raises(ValueError, match="overlaps"):
+            AdamW([p], state=dict(t=0, m=[m], v=[v]))

@@ -120,3 +120,13 @@ def test_refusals_on_the_device():
     for args in [(ids, m, 5), (ids, m[:4], 0), (ids, m[:4].expand(4, 6).double(), 5), (ids, m[:1].expand(4, 6), 5)]:
         with pytest.raises(ValueError):
             EmbedRows.backward(*args)
+
+
+def test_outputs_that_share_memory_are_refused():
+    from bidmach_b200 import EmbedRows
+    m = torch.randn(9, 8, device="cuda")
+    ids = torch.arange(9, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError, match="overlaps"):
+        EmbedRows.forward(ids, m, out=m)
+    with pytest.raises(ValueError, match="overlaps"):
+        EmbedRows.backward(ids, m, 9, out=m)

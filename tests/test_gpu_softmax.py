@@ -288,3 +288,23 @@ def test_many_short_calls_in_a_row():
     torch.cuda.synchronize()
     for i, (x, want) in enumerate(sets):
         assert all(torch.equal(a, b) for a, b in zip(last[i], want))
+
+
+def test_outputs_that_share_memory_are_refused():
+    from bidmach_b200 import Softmax
+    h, w = (torch.randn(n, 32, device="cuda") for n in (40, 50))
+    y = torch.zeros(40, dtype=torch.int32, device="cuda")
+    loss, lse = Softmax.loss(h, w, y)
+    one = torch.ones((), device="cuda")
+    for out in (dict(dhidden=h), dict(dweight=w), dict(dhidden=w[:40]), dict(dhidden=w[10:], dweight=w.clone()),
+                dict(zip(("dhidden", "dweight"), (lambda b: (b[:40], b[:50]))(torch.empty(60, 32, device="cuda"))))):
+        with pytest.raises(ValueError, match="overlaps"):
+            Softmax.grad(h, w, y, lse, one, **out)
+    with pytest.raises(ValueError, match="overlaps"):
+        Softmax.loss(h, w, y, loss=loss, lse=loss)
+    # the gradients beside their operands in one buffer each
+    both = torch.zeros(50, 64, device="cuda")
+    both[:, :32] = w
+    want = Softmax.grad(h, w, y, lse, one)
+    got = Softmax.grad(h, both[:, :32], y, lse, one, dweight=both[:, 32:])
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and torch.equal(both[:, :32], w)

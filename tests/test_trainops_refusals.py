@@ -76,3 +76,31 @@ def test_window_rows_refuses():
     for n, nskip, rows, ws, have in [(-1, 5, 64, 64, 1 << 20), (10, 0, 64, 64, size), (10, 513, 64, 64, size),
                                      (10, 5, 0, 64, size), (10, 5, 64, 0, size), (10, 5, 64, 64, size - 1)]:
         assert lib.w2v_window_rows(64, 64, 64, n, nskip, 64, 64, rows, ws, have, None) == 1
+
+
+def test_outputs_that_share_memory():
+    from bidmach_b200.embed import check_apart
+    buf = torch.zeros(12, 10)
+    a = buf[:, :4]
+    for b in (a, buf, buf[:, 3:6], buf[:6, 2:], buf.view(-1)[3:5], buf[5:6, 1:3], buf[3, 2], buf.view(24, 5)[:, :2],
+              buf.view(torch.int32)[:, :1]):
+        with pytest.raises(ValueError, match="out overlaps x"):
+            check_apart("out", a, x=b)
+        with pytest.raises(ValueError, match="out overlaps x"):
+            check_apart("out", b, x=a)
+    # other columns, other rows, nothing, other memory; rows that start in the columns and end in the next row
+    for b in (buf[:, 4:8], buf[:, 4:], buf[:0], torch.zeros(5), torch.tensor(1.0)):
+        check_apart("out", a, x=b)
+        check_apart("out", b, x=a)
+    check_apart("out", buf[:6], x=buf[6:])
+    wrap = buf.view(-1)[8:108].view(10, 10)[:, :3]      # columns 8, 9 and 0 of the next row
+    with pytest.raises(ValueError):
+        check_apart("out", a, x=wrap)
+    check_apart("out", buf[:, 2:4], x=wrap)
+
+
+def test_adamw_moments_that_share_memory():
+    x = torch.zeros(1024)
+    with pytest.raises(ValueError, match="state overlaps"):
+        AdamW._apart([x[:8], x[8:16], x[15:20]], "a tensor of the state overlaps")
+    AdamW._apart([x[:8], x[8:16], x[8:8]], "")
