@@ -10,8 +10,9 @@
 // table in device memory: nothing has to be uploaded before a step, and a captured step holds
 // its own.
 //
-// Measured: 51 million elements with fp32 moments 217 us (6.6 TB/s); 300 million with 8-bit moments 880 us
-// (5.5 TB/s; the codes cost about 40 of 70 instructions an element), their values as fp32 491 us.
+// Measured: 51 million elements with fp32 moments 217 us (6.6 TB/s); 300 million with 8-bit moments, and
+// their values as fp32, 1.41 ms (5.1 TB/s; the codes take more than half of the instructions, the values alone
+// 491 us).  Telling lanes without a code of zero apart, to spare them the selects, cost 7 %.
 //
 // Each operation on the moments is rounded on its own (no contraction to fused multiply-adds), so the
 // result does not depend on how a compiler groups them: next to the border of two 8-bit codes that
@@ -72,7 +73,10 @@ struct Rates {
   int advance;
 };
 
-// What a step computes once, each rounded to fp32 from its value in 64 bits.
+constexpr float kSmallest = 1.17549435e-38f;   // 2^-126: its reciprocal is still finite
+
+// What a step computes once, each rounded to fp32 from its value in 64 bits; eps is at least 2^-126, so
+// that an element without a gradient is not divided by zero (a root of v that is not zero is above 2^-75).
 struct Consts {
   float b1, ob1, b2, ob2, lrc1, rc2, eps, keep;
 };
@@ -81,7 +85,14 @@ __device__ __forceinline__ Consts constants(const Rates &r) {
   const double c1 = 1.0 - r.clock->b1t * r.beta1, c2 = 1.0 - r.clock->b2t * r.beta2;
   const double lr = r.lrate_dev ? (double)*r.lrate_dev : r.lrate;
   return Consts{(float)r.beta1, (float)(1.0 - r.beta1), (float)r.beta2, (float)(1.0 - r.beta2),
-                (float)(lr / c1), (float)(1.0 / sqrt(c2)), (float)r.eps, (float)(1.0 - lr * r.wdecay)};
+                (float)(lr / c1), (float)(1.0 / sqrt(c2)), fmaxf((float)r.eps, kSmallest), (float)(1.0 - lr * r.wdecay)};
+}
+
+// One unit in the last place off; zero from 2^126 on.
+__device__ __forceinline__ float reciprocal(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
 }
 
 __device__ __forceinline__ void step8(float (&p)[8], const float (&g)[8], float (&m)[8], float (&v)[8],
@@ -93,22 +104,28 @@ __device__ __forceinline__ void step8(float (&p)[8], const float (&g)[8], float 
     root[i] = __fsqrt_rn(v[i]);
     const float d = __fadd_rn(__fmul_rn(root[i], c.rc2), c.eps);
     // the quotient reaches the parameter only, not a stored moment: two units in its last place will do
-    p[i] = __fsub_rn(__fmul_rn(p[i], c.keep), __fdividef(__fmul_rn(m[i], c.lrc1), d));
+    p[i] = __fsub_rn(__fmul_rn(p[i], c.keep), __fmul_rn(__fmul_rn(m[i], c.lrc1), reciprocal(d)));
   }
 }
 
 constexpr int kOne = 0x3F800000;
-constexpr float kSmallestScale = 1.17549435e-38f;   // 2^-126: its reciprocal is still finite
+
+// NaN where a or b is one.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 
 // Scale of a unit, the largest of |x|; bits of non-negative floats order as unsigned numbers, NaN last.
 __device__ __forceinline__ float unit_scale(const float (&x)[8]) {
-  unsigned top = 0;
+  float most = fabsf(x[0]);
 #pragma unroll
-  for (int i = 0; i < 8; i++) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
-  top = __reduce_max_sync(kFullMask, top);
+  for (int i = 1; i < 8; i++) most = max_nan(most, fabsf(x[i]));
+  const unsigned top = __reduce_max_sync(kFullMask, __float_as_uint(most));
   if (top >= 0x7f800000u) return __uint_as_float(0x7fffffffu);   // infinity or NaN: the unit reads as NaN
   const float s = __uint_as_float(top);
-  return s >= kSmallestScale ? s : 0.f;
+  return s >= kSmallest ? s : 0.f;
 }
 
 template <bool SIGNED>

@@ -238,3 +238,19 @@ def test_moments_that_share_memory_are_refused():
     for m, v in ((x, x), (p, x), (x, p)):
         with pytest.raises(ValueError, match="overlaps"):
             AdamW([p], state=dict(t=0, m=[m], v=[v]))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_smallest_eps(bits):
+    """An eps that fp32 does not hold: an element without a gradient only decays."""
+    from bidmach_b200 import AdamW
+    p = torch.ones(300, device="cuda")
+    opt = AdamW([p], AdamW.Opts(lrate=0.5, eps=1e-60, wdecay=0.5, bits=bits))
+    g = torch.zeros(300, device="cuda")
+    g[7] = 2.0
+    opt.step([g])
+    want = torch.full((300,), 0.75)
+    want[7] = 0.25      # the first step is lrate in the gradient's direction
+    # m / c1 and sqrt(v / c2): six roundings each and three of the step, below 2^-19 in all
+    assert torch.allclose(p.cpu(), want, rtol=0, atol=2.0 ** -19)
+    assert torch.equal(p.cpu()[8:], want[8:])
