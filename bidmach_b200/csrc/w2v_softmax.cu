@@ -576,8 +576,13 @@ __device__ __forceinline__ uint32_t pair_begin(Pipe &s, int readers) {
   tmem_after_sync();
   return s.tmem;
 }
-// Neither CTA leaves while the other's products read its shared memory or its barriers are arrived on.
-__device__ __forceinline__ void pair_end(uint32_t tmem) {
+// Neither CTA leaves while the other's products read its shared memory or its barriers are arrived on.  What
+// arrives without a thread behind it is waited for before: copies (`full`) by the issuer, finished
+// tiles (`tfull`) by both CTAs' readers, stages that were read (`empty`) by both CTAs' producers
+// (Ring::drain).  Where a wait ran out that chain is broken: a millisecond is long enough for any of them.
+__device__ __forceinline__ void pair_end(Pipe &s, uint32_t tmem) {
+  if (*const_cast<volatile int *>(&s.gave_up))
+    for (int i = 0; i < 1000; i++) __nanosleep(1000);
   tmem_before_sync();
   __syncwarp();
   cluster_sync();
@@ -603,6 +608,13 @@ struct Ring {
     a = smem + i * kBytesStage;
     b = a + kBytesA;
     return true;
+  }
+  // The products tell both CTAs of each stage that they have read, the last ones too: a CTA that left before
+  // would have them arrive in the shared memory of the next one on its SM.
+  __device__ __forceinline__ bool drain() {
+    bool ok = true;
+    for (int i = max(0, it - STAGES); ok && i < it; i++) ok = mbar_wait(&s.empty[i % STAGES], (i / STAGES) & 1, gave_up);
+    return ok;
   }
   // Copies in flight still write into this CTA's shared memory.
   __device__ __forceinline__ void settle() {
@@ -812,7 +824,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) prod
             tma_load_2d(b, &p.b, p.pb[q] + kb * kK, col, bar);
           }
       }
-      if (!ok) ring.settle();
+      if (!ok || !ring.drain()) ring.settle();
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -959,7 +971,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) prod
     }
     if (USE == kProbs && lane == 0) bulk_wait_group_all();
   }
-  pair_end(tmem);
+  pair_end(pipe, tmem);
 }
 
 // ---- gradients from a piece of d -------------------------------------------------------------
@@ -1165,7 +1177,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGradThreads<SEGMENT
                 tma_load_2d(b + i * 8192, &s.b, s.pb[q] + col + i * 64, s.b_y + kb * kK, bar);
             }
       }
-      if (!ok) ring.settle();
+      if (!ok || !ring.drain()) ring.settle();
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -1246,7 +1258,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGradThreads<SEGMENT
       }
     }
   }
-  pair_end(tmem);
+  pair_end(pipe, tmem);
 }
 
 // The tiles that were cut: blockIdx.x is the tile in what is left, a warp a row.
@@ -1349,7 +1361,10 @@ struct Operand {
 
 // The kernels that work in pairs of CTAs with tensor memory are launched in the ordinary way, each after
 // its predecessor has ended; started early like the others (w2v_chain.cuh), short ones in a row were seen
-// to stop now and then.
+// to stop now and then, from a cause that reading has not shown.  Every wait of theirs on a barrier in shared
+// memory is bounded.  What is not: tcgen05.alloc, which never waits (a CTA's shared memory leaves no room
+// for a second one with tensor memory on its SM), the barriers of the pair, which all threads of both CTAs
+// reach, and the wait for the predecessor, of which no two kernels can form a circle.
 
 // An attribute of the function on the current device, set once for each (a call costs a microsecond).
 template <auto KERNEL>

@@ -308,3 +308,24 @@ def test_outputs_that_share_memory_are_refused():
     want = Softmax.grad(h, w, y, lse, one)
     got = Softmax.grad(h, both[:, :32], y, lse, one, dweight=both[:, 32:])
     assert all(torch.equal(a, b) for a, b in zip(got, want)) and torch.equal(both[:, :32], w)
+
+
+def test_short_calls_on_two_streams():
+    """Kernels of a few tiles from two streams, which follow one another on an SM without a gap: no arrival of
+    one reaches the next, so every call gives the bits of the call alone."""
+    from bidmach_b200 import Softmax
+    sets = []
+    for n, vocab, dim, t in ((20, 600, 64, "bf16"), (40, 300, 72, "f32"), (300, 700, 16, "f16"), (17, 260, 320, "bf16")):
+        x = [v.cuda() for v in inputs(n, vocab, dim, 1, t, seed=5)]
+        sets.append((x, run(*x)))
+    torch.cuda.synchronize()
+    streams, last = [torch.cuda.Stream(), torch.cuda.Stream()], {}
+    for i in range(800):
+        k = i % len(sets)
+        with torch.cuda.stream(streams[(i // len(sets) + i) % 2]):
+            x = sets[k][0]
+            loss, lse = Softmax.loss(*x[:3])
+            last[k, i % 2] = (loss, lse, *Softmax.grad(*x[:3], lse, x[3]))
+    torch.cuda.synchronize()
+    for (k, _), got in last.items():
+        assert all(torch.equal(a, b) for a, b in zip(got, sets[k][1]))
