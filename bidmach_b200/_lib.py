@@ -131,6 +131,8 @@ SIGNATURES = {
     "w2v_adamw_clock": (_I, [_P, C.c_double, C.c_double, C.c_int64, _P]),
     "w2v_adamw_step": (_I, [C.POINTER(W2VAdamwTensor), C.POINTER(_P), C.POINTER(_I), _I, _I,
                             C.POINTER(W2VAdamwOpts), _P, _P, _P]),
+    "w2v_adamw_step_random": (_I, [C.POINTER(W2VAdamwTensor), C.POINTER(_P), C.POINTER(_I), _I,
+                                   C.POINTER(W2VAdamwOpts), _P, C.c_uint64, _P, _P]),
     "w2v_adamw_moments": (_I, [C.POINTER(W2VAdamwTensor), C.POINTER(_P), C.POINTER(_P), _I, _P]),
 }
 

@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes as C
 import dataclasses
+import warnings
 
 import torch
 
@@ -48,13 +49,21 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
 
 @dataclasses.dataclass
 class Opts:
-    """``lrate`` and the usual constants; ``bits``: 32 or 8 for the moments."""
+    """``lrate`` and the usual constants; ``bits``: 32 or 8 for the moments.
+
+    ``rounding`` of 8-bit moments: ``"random"``, for training, rounds a code up or down so that the stored moments
+    are right in the mean (random bits from ``seed``, the step and the element: equal runs give equal
+    bits).  ``"nearest"`` is for a few steps, or for comparing with one: the codes of sqrt(v) are 3 to 6 %
+    apart and a step with ``beta2`` 0.999 lowers it by 0.05 %, so a moment rounded to nearest never falls and
+    hardly rises.  None is ``"nearest"`` with a warning."""
     lrate: float = 1e-3
     beta1: float = 0.9
     beta2: float = 0.999
     eps: float = 1e-8
     wdecay: float = 0.01
     bits: int = 32
+    rounding: str | None = None
+    seed: int = 0
 
 
 class AdamW:
@@ -83,6 +92,11 @@ class AdamW:
             raise ValueError("bits must be 32 or 8")
         if not (0 <= o.beta1 < 1 and 0 <= o.beta2 < 1 and o.eps > 0 and o.wdecay >= 0):
             raise ValueError("need 0 <= beta1, beta2 < 1, eps > 0, wdecay >= 0")
+        if o.rounding not in (None, "nearest", "random"):
+            raise ValueError("rounding is 'random' or 'nearest'")
+        if o.bits == 8 and o.rounding is None:
+            warnings.warn("8-bit moments rounded to nearest do not follow their gradients over many steps: "
+                          "give rounding='random' for training, or 'nearest'", stacklevel=2)
         if not self.params:
             raise ValueError("AdamW needs at least one tensor")
         for p in self.params:
@@ -185,9 +199,14 @@ class AdamW:
             rate = float(lrate)
         opts = _lib.W2VAdamwOpts(rate, o.beta1, o.beta2, o.eps, o.wdecay)
         with on_device(dev):
-            check(_lib.load().w2v_adamw_step(self._table, self._pointers(*map(torch.Tensor.data_ptr, grads)),
-                                             kinds, n, o.bits, C.byref(opts), rate_ptr,
-                                             self._clock_at, stream_of(dev)), "w2v_adamw_step")
+            pointers = self._pointers(*map(torch.Tensor.data_ptr, grads))
+            if o.bits == 8 and o.rounding == "random":
+                check(_lib.load().w2v_adamw_step_random(self._table, pointers, kinds, n, C.byref(opts), rate_ptr,
+                                                        o.seed & (2 ** 64 - 1), self._clock_at, stream_of(dev)),
+                      "w2v_adamw_step_random")
+            else:
+                check(_lib.load().w2v_adamw_step(self._table, pointers, kinds, n, o.bits, C.byref(opts), rate_ptr,
+                                                 self._clock_at, stream_of(dev)), "w2v_adamw_step")
 
     def moments(self, mout=None, vout=None):
         """Both moments as fp32 values: lists (m, v).  With 32 bits these are the state itself; with 8

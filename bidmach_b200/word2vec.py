@@ -58,7 +58,7 @@ class Opts:
     beta2: float = 0.999
     adamEps: float = 1e-8
     wdecay: float = 0.0
-    momentBits: int = 32        # 32 or 8
+    momentBits: int = 32        # 32 or 8 (rounded at random, from `seed`)
 
     def to_c(self) -> _lib.W2VOpts:
         return _lib.W2VOpts(self.dim, self.nskip, self.nneg, self.nreuse, self.vocabSize,
@@ -307,7 +307,8 @@ class Word2Vec:
             state = None if up is None else {"t": self._adam_steps, "m": up.m, "v": up.v, "mscale": up.mscale,
                                              "vscale": up.vscale}
             up = self._updater = AdamW(self.modelmats, AdamW.Opts(lrate=o.lrate, beta1=o.beta1, beta2=o.beta2,
-                                                                  eps=o.adamEps, wdecay=o.wdecay, bits=o.momentBits),
+                                                                  eps=o.adamEps, wdecay=o.wdecay, bits=o.momentBits,
+                                                                  rounding="random", seed=o.seed),
                                        state=state)
         up.step([dcontext, dcentre], o.lrate * (max(1, int(pos)) / self._firstPos) ** -o.texp)
         self._adam_steps += 1

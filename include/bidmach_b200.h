@@ -501,7 +501,7 @@ typedef struct w2v_adamw_opts {
 
 /* Sets the step counter of an updater, 32 bytes of device memory (8-byte aligned): t steps done. */
 int w2v_adamw_clock(void *clock, double beta1, double beta2, int64_t t, void *stream);
-/* One step for all `ntensors` tensors and the counter:
+/* One step for all `ntensors` tensors and the counter (8-bit codes rounded to nearest):
  *   m = b1 m + (1-b1) g;  v = b2 v + (1-b2) g^2;
  *   p = p (1 - lrate wdecay) - (lrate / (1-b1^t)) m / (sqrt(v) / sqrt(1-b2^t) + eps)
  * grads[i] holds n elements of gtypes[i]: fp32, or the type of the tensor.  `tensors`, `grads` and
@@ -510,6 +510,14 @@ int w2v_adamw_clock(void *clock, double beta1, double beta2, int64_t t, void *st
 int w2v_adamw_step(const w2v_adamw_tensor *tensors, const void *const *grads, const int *gtypes,
                    int ntensors, int bits, const w2v_adamw_opts *opts, const float *lrate_dev,
                    void *clock, void *stream);
+/* The same with 8-bit moments whose codes are rounded at random instead of to nearest: up with the
+ * probability that makes the mean of the stored m and v the values before rounding.  A moment that is
+ * rounded to nearest stands still where a step changes it by less than half the distance of two codes, 3 to
+ * 6 % of sqrt(v) (a step with beta2 = 0.999 lowers sqrt(v) by 0.05 % at most): of use for a few steps only.
+ * The random bits are a hash of `seed`, the step counter and the element's place: equal calls give equal bits. */
+int w2v_adamw_step_random(const w2v_adamw_tensor *tensors, const void *const *grads, const int *gtypes,
+                          int ntensors, const w2v_adamw_opts *opts, const float *lrate_dev, uint64_t seed,
+                          void *clock, void *stream);
 /* 8-bit moments as the fp32 values they stand for: mout[i], vout[i] are fp32[n]. */
 int w2v_adamw_moments(const w2v_adamw_tensor *tensors, float *const *mout, float *const *vout,
                       int ntensors, void *stream);

@@ -254,3 +254,133 @@ def test_smallest_eps(bits):
     # m / c1 and sqrt(v / c2): six roundings each and three of the step, below 2^-19 in all
     assert torch.allclose(p.cpu(), want, rtol=0, atol=2.0 ** -19)
     assert torch.equal(p.cpu()[8:], want[8:])
+
+
+def mix32(x):
+    x = np.asarray(x, np.uint32)
+    x = ((x ^ x >> 16) * np.uint32(0x85ebca6b)).astype(np.uint32)
+    x = ((x ^ x >> 13) * np.uint32(0xc2b2ae35)).astype(np.uint32)
+    return x ^ x >> 16
+
+
+def encode_random(x, signed, key, first):
+    """Codes rounded at random; `first` is the place of x[0] among the random bits."""
+    shift, top = (20, 127) if signed else (19, 255)
+    n = len(x)
+    x = np.concatenate([x, np.zeros(-n % 256, F)]).reshape(-1, 256)
+    scale = np.abs(x).max(1)
+    y = (x * np.where(scale >= F(2.0 ** -126), F(1) / np.maximum(scale, F(2.0 ** -126)), F(0)).astype(F)[:, None]).reshape(-1)
+    bits = np.abs(y).view(np.uint32)
+    h = mix32((first + np.arange(len(y))).astype(np.uint32) ^ key)
+    if signed:
+        code = (bits + (h & np.uint32(0xfffff))) >> 20
+    else:
+        f, m = (bits & np.uint32(2 ** 19 - 1)).astype(F) * F(2.0 ** -19), (32 + (bits >> 18 & 30)).astype(F)
+        up = (f * (m + f)) * (F(1) / (m + F(1)))
+        code = (bits >> 19) + (((up * F(2.0 ** 19)).astype(np.uint32) + (h >> 13)) >> 19)
+    code = np.minimum(code.astype(np.int64), 0x3F800000 >> shift) - ((0x3F800000 >> shift) - top)
+    code = np.where(bits == 0, 0, np.maximum(code, 0 if signed else 1))
+    if signed:
+        code = code + 128 * ((y < 0) & (code > 0))
+    return code[:n].astype(np.uint8), scale.astype(F)
+
+
+@pytest.mark.parametrize("sizes", [[1], [255, 256, 257], [0, 5, 1000], [70001], [3] * 300], ids=lambda s: f"{len(s)}x{s[0]}")
+@pytest.mark.parametrize("ptype", list(TYPES))
+def test_random_rounding_matches_the_restatement(ptype, sizes):
+    from bidmach_b200 import AdamW
+    seed = 0x123456789
+    ps, _ = make(sizes, ptype, "f32", 1)
+    opt = AdamW([p.cuda() for p in ps], AdamW.Opts(lrate=LR, beta1=B1, beta2=B2, eps=EPS, wdecay=WD, bits=8,
+                                                  rounding="random", seed=seed))
+    m, v = [np.zeros(n, F) for n in sizes], [np.zeros(n, F) for n in sizes]
+    with np.errstate(over="ignore"):
+        for t in range(3):
+            gs = make(sizes, ptype, "f32", 10 + t)[1]
+            opt.step([g.cuda() for g in gs])
+            unit, launch = 0, 0
+            for i, g in enumerate(gs):
+                if i == 256:          # the tensors of a launch
+                    unit, launch = 0, 1
+                key = mix32(mix32(np.uint32(seed & 0xffffffff) + mix32(np.uint32((seed >> 32) + launch * 0x9e3779b9))) +
+                            np.uint32(t * 0x9e3779b9 & 0xffffffff))
+                _, m[i], v[i], root = step_f32(np.zeros(sizes[i], F), f32(g), m[i], v[i], t + 1)
+                mc, ms = encode_random(m[i], True, key, unit * 256)
+                vc, vs = encode_random(root, False, key, unit * 256)
+                np.testing.assert_array_equal(opt.m[i].cpu().numpy(), mc)
+                np.testing.assert_array_equal(opt.v[i].cpu().numpy(), vc)
+                np.testing.assert_array_equal(opt.vscale[i].cpu().numpy(), vs[:(sizes[i] + 255) // 256])
+                m[i], v[i] = decode(mc, ms, True), decode(vc, vs, False) ** 2
+                unit += (sizes[i] + 255) // 256
+
+
+@pytest.mark.parametrize("beta1", [0.9, 0.99])
+@pytest.mark.parametrize("case", ["falling", "rising", "sparse"])
+def test_moments_in_8_bits_over_thousands_of_steps(case, beta1):
+    """Gradients whose size changes, beside 32-bit moments: the mean over 8160 elements of the stored v is the
+    32-bit one.  The first element of each block keeps gradients of size 1, so the others are relative to it.
+
+    Tolerance.  Rounding is right in the mean, so what is left is chance.  A code is at most 1/16 above the one
+    before, so a step that changes sqrt(v) relative to its scale by d adds at most 4 d / 16 to the relative
+    variance of v.  The 8000 steps of `falling` change it by 4.6 of its own and about 1e-3 a step with
+    the scale, 13 in all: the relative variance of an element is at most exp(13 / 4) - 1 = 25, the standard
+    deviation of the mean of 8160 is 0.055, and 0.3 is more than five times that.  The sums of m have
+    a spread of their own: they are compared as m against 32 bits in norm over one step's rounding,
+    below 1/8 each over about 1 / (1 - beta1) steps, in quadrature with weights beta1^k."""
+    from bidmach_b200 import AdamW
+    n = 32 * 256
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    first = torch.zeros(n, dtype=torch.bool, device="cuda")
+    first[::256] = True
+    o = dict(lrate=0.0, beta1=beta1, beta2=0.999, wdecay=0.0)
+    a = AdamW([torch.zeros(n, device="cuda")], AdamW.Opts(bits=32, **o))
+    b = AdamW([torch.zeros(n, device="cuda")], AdamW.Opts(bits=8, rounding="random", seed=3, **o))
+    size = {"falling": (1.0, 0.01), "rising": (0.2, 1.0), "sparse": (1.0, 1.0)}[case]
+    for t in range(10000):
+        g = torch.randn(n, generator=gen, device="cuda")
+        scale = size[0] if t < 2000 else size[1]
+        if case == "sparse":
+            scale = (torch.rand(n, generator=gen, device="cuda") < 0.01).float()
+        g = torch.where(first, g, g * scale)
+        a.step([g])
+        b.step([g])
+    (ma,), (va,) = a.moments()
+    (mb,), (vb,) = b.moments()
+    rest = ~first
+    ratio = float(vb[rest].double().mean() / va[rest].double().mean())
+    assert 0.7 <= ratio <= 1.3, ratio
+    off = float((mb - ma)[rest].double().norm() / ma[rest].double().norm())
+    # each step's rounding is below 1/8 of a code's value of m, whose size stays about that of the last one
+    assert off <= 0.125 / (1 - beta1 ** 2) ** 0.5, off
+
+
+def test_random_rounding_repeats_and_is_asked_for():
+    from bidmach_b200 import AdamW
+    (p,), (g,) = make([5000], "f32", "f32", 3)
+    g = g.cuda()
+
+    def after(seed, steps=3, start=0):
+        opt = AdamW([p.cuda()], AdamW.Opts(bits=8, rounding="random", seed=seed))
+        for _ in range(steps):
+            opt.step([g])
+        return torch.cat([opt.m[0], opt.v[0]])
+
+    assert torch.equal(after(5), after(5)) and not torch.equal(after(5), after(6)) and not torch.equal(after(5), after(5 + 2 ** 32))
+    # a captured step draws other bits in each replay, those of as many calls
+    q = p.cuda()
+    opt = AdamW([q], AdamW.Opts(bits=8, rounding="random", seed=5))
+    opt.step([g])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step([g])
+    graph.replay()
+    graph.replay()
+    assert torch.equal(torch.cat([opt.m[0], opt.v[0]]), after(5))
+    # a step count that goes on draws on
+    t2 = AdamW([p.cuda()], AdamW.Opts(bits=8, rounding="random", seed=5),
+               state=dict(t=3, m=[opt.m[0].clone()], v=[opt.v[0].clone()], mscale=[opt.mscale[0].clone()],
+                          vscale=[opt.vscale[0].clone()]))
+    t2.step([g])
+    assert torch.equal(torch.cat([t2.m[0], t2.v[0]]), after(5, 4))
+    with pytest.warns(UserWarning, match="rounding"):
+        AdamW([p.cuda()], AdamW.Opts(bits=8))

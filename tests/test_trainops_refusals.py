@@ -104,3 +104,15 @@ def test_adamw_moments_that_share_memory():
     with pytest.raises(ValueError, match="state overlaps"):
         AdamW._apart([x[:8], x[8:16], x[15:20]], "a tensor of the state overlaps")
     AdamW._apart([x[:8], x[8:16], x[8:8]], "")
+
+
+def test_rounding_is_checked():
+    with pytest.raises(ValueError, match="rounding"):
+        AdamW([torch.zeros(8)], AdamW.Opts(bits=8, rounding="up"))
+    lib, before = _lib.load(), _lib.load().w2v_launch_count()
+    t = (_lib.W2VAdamwTensor * 1)(_lib.W2VAdamwTensor(64, 64, 64, 0, 0, 4, 0))     # no scales
+    g, k = (C.c_void_p * 1)(64), (C.c_int * 1)(0)
+    o = _lib.W2VAdamwOpts(1e-3, 0.9, 0.999, 1e-8, 0.0)
+    assert lib.w2v_adamw_step_random(t, g, k, 1, C.byref(o), None, 1, 64, None) == 1
+    assert lib.w2v_adamw_step_random(t, g, k, 1, C.byref(o), None, 1, 0, None) == 1
+    assert lib.w2v_launch_count() == before
