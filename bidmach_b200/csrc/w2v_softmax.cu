@@ -66,14 +66,14 @@ struct RowCoef {
   unsigned hits;   // chunks of 32 columns of the tile at hand that hold a target (only in shared memory)
 };
 
-// Found on the device before a product: largest magnitudes (as bits) of H, W and g_n k_n.
+// Found on the device before a product: largest finite magnitudes (as bits) of H, W and g_n k_n.
 struct Scalars {
   unsigned h, w, g;
 };
 
-// 2^e such that the largest magnitude times it lies in [2^top, 2^(top+1)); 1 for zero and non-finite.
+// 2^e such that the largest magnitude times it lies in [2^top, 2^(top+1)); 1 for zero.
 __device__ __forceinline__ int scale_exp(unsigned bits, int top) {
-  if (bits == 0 || bits >= 0x7f800000u) return 0;
+  if (bits == 0) return 0;
   const int e = bits >= 0x800000u ? (int)(bits >> 23) - 127 : -118 - __clz((int)bits);
   return min(100, max(-100, top - e));
 }
@@ -455,7 +455,13 @@ __device__ __forceinline__ void block_max(unsigned top, unsigned *to) {
   if ((threadIdx.x & 31) == 0 && top) atomicMax(to, top);
 }
 
-// Largest magnitudes of fp32 operands (z = 0: H, 1: W) and of the rows' g_n k_n (z = 2).
+// Bits of a magnitude; an infinity or a NaN counts as zero: it spoils its own row, not the others' scale.
+__device__ __forceinline__ unsigned magnitude(float x) {
+  const unsigned bits = __float_as_uint(x) & 0x7fffffffu;
+  return bits < 0x7f800000u ? bits : 0u;
+}
+
+// Largest finite magnitudes of fp32 operands (z = 0: H, 1: W) and of the rows' g_n k_n (z = 2).
 __global__ void __launch_bounds__(256) amax_kernel(Source h, Source w, int dim, const float *gloss,
                                                    const int *targets, int labels, int64_t vocab, Scalars *sc) {
   chain_wait();
@@ -473,13 +479,13 @@ __global__ void __launch_bounds__(256) amax_kernel(Source h, Source w, int dim, 
         if (wide && have == 8) load8(a + r * s.ld + c, x);
         else load_some(a + r * s.ld + c, have, x);
 #pragma unroll
-        for (int e = 0; e < 8; e++) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+        for (int e = 0; e < 8; e++) top = max(top, magnitude(x[e]));
       }
     block_max(top, blockIdx.z == 0 ? &sc->h : &sc->w);
   } else if (gloss) {
     for (int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x; n < h.rows; n += (int64_t)gridDim.x * 256) {
       const int k = valid_targets(targets + n * labels, labels, vocab);
-      if (k) top = max(top, __float_as_uint(gloss[n] * (float)k) & 0x7fffffffu);
+      if (k) top = max(top, magnitude(gloss[n] * (float)k));
     }
     block_max(top, &sc->g);
   }

@@ -24,7 +24,8 @@ class Softmax:
     ``targets`` int32 ``[n]`` or ``[n, labels]``.  A target outside ``[0, vocab)`` (-1 by convention) stands
     for none; a row may have none (its loss and gradient are zero) or the same word more than once.
     fp32 operands are multiplied to 22 bits and accumulated in fp32; 16-bit ones are multiplied exactly.
-    Every row takes part in the products, so ``hidden`` has to be finite in rows without targets too.
+    Every row takes part in the products: an infinity or a NaN in a row of ``hidden``, with targets or without,
+    or in ``gloss`` spoils that row's results and ``dweight``, one in ``weight`` all rows'.
     Outputs that are given share no memory with the inputs or with each other."""
 
     @staticmethod

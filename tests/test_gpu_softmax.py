@@ -329,3 +329,28 @@ def test_short_calls_on_two_streams():
     torch.cuda.synchronize()
     for (k, _), got in last.items():
         assert all(torch.equal(a, b) for a, b in zip(got, sets[k][1]))
+
+
+@pytest.mark.parametrize("n", [9, 90])
+@pytest.mark.parametrize("t,size", [("f32", 1.0), ("f32", 1e-4), ("f32", 3e5), ("f16", 1.0), ("bf16", 1e-4)])
+@pytest.mark.parametrize("where", ["hidden", "gloss"])
+def test_not_finite_numbers_stay_in_their_rows(n, t, size, where):
+    """A NaN and an infinity in rows of hidden, or among the rows' factors: loss, lse and dhidden of all other
+    rows are within the usual bounds, whatever the size of the numbers beside them."""
+    hidden, weight, targets, gloss = inputs(n, 300, 32, 1, t)
+    hidden, weight = (hidden.float() * size).to(TYPES[t]), (weight.float() / size).to(TYPES[t])
+    gloss = gloss * (1e-3 if t == "f16" else 1.0)     # d of fp16 has to be scaled up
+    targets[:, 0] = torch.arange(n, dtype=torch.int32)
+    good = torch.ones(n, dtype=torch.bool)
+    good[1] = good[3] = False
+    broken = [hidden.clone(), weight, targets, gloss.clone()]
+    if where == "hidden":
+        broken[0][1, 3], broken[0][3, 5] = float("nan"), float("inf")
+    else:
+        broken[3][1], broken[3][3] = float("nan"), float("inf")
+    got = [x.cpu() for x in run(*broken)]
+    clean = run(hidden, weight, targets, gloss)      # its dweight stands in for the broken one, which is NaN
+    loss, lse, dh = (torch.where(good.view(-1, *[1] * (x.dim() - 1)), x, c.cpu()) for x, c in zip(got[:3], clean))
+    assert all(torch.isfinite(x).all() for x in (loss, lse, dh))
+    hold((loss, lse, dh, clean[3].cpu()), hidden, weight, targets, gloss, t)
+    assert torch.isnan(got[2][~good]).any(1).all()
