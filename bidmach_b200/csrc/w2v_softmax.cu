@@ -22,6 +22,11 @@
 // hi hi + hi lo + lo hi computed: 22 bits of each operand.  Products of fp16 or bf16 operands are exact in
 // the fp32 accumulators.  d is rounded once to the operands' type (fp32: to hi + lo with lo scaled by
 // 2^11, so that small probabilities keep their bits; the operand it meets carries the 2^-11).
+// One scale serves a matrix whose rows' largest magnitudes lie within 2^kRowSpan of each other.  Where they
+// do not (an outlier in one row), two fp16 numbers would lose the bits of the others: the operands are
+// then split into three bf16 numbers, which keep their own exponents, and six products computed.  The
+// device decides, from magnitudes that it has to find for the scale anyway (find_wide).  4096 x 100000 x 256:
+// loss 0.47 ms, with an outlier 0.96; gradients 2.08 ms, with one 3.78.
 //
 // For few rows the bound is reading W once: a kernel with eight rows in shared memory, W straight from
 // memory in its own type, plain fp32 arithmetic.  fp32 goes that way up to 16 rows, in two passes: the
@@ -66,16 +71,30 @@ struct RowCoef {
   unsigned hits;   // chunks of 32 columns of the tile at hand that hold a target (only in shared memory)
 };
 
-// Found on the device before a product: largest finite magnitudes (as bits) of H, W and g_n k_n.
+// Found on the device before a product: largest finite magnitudes (as bits) of H, W and g_n k_n, and the
+// smallest ones of a row that are not zero, as kInfBits less them (0: no row), so that all are maxima.
+constexpr unsigned kInfBits = 0x7f800000u;
 struct Scalars {
-  unsigned h, w, g;
+  unsigned h, w, g, h_low, w_low, g_low;
+  unsigned wide;   // three bf16 parts rather than two fp16 ones, set by stage_kernel
 };
+
+// With row maxima within 2^14 the last row's lies above 2^-1 after scaling, and the steps of its fp16 parts,
+// 2^-24 and more, are its 22nd bits or better.  Factors g_n k_n: d = g k p has 2^-36 as its smallest half
+// step; beyond 2^12 the probabilities of a row would be off by 2^-20 of their sum in a vocabulary of 2^17.
+constexpr int kRowSpan = 14, kFactorSpan = 12;
+__device__ __forceinline__ bool apart(unsigned top, unsigned low, int span) {
+  return low && (int)(top >> 23) - (int)((kInfBits - low) >> 23) > span;
+}
+__device__ __forceinline__ bool find_wide(const Scalars *sc) {
+  return apart(sc->h, sc->h_low, kRowSpan) || apart(sc->w, sc->w_low, kRowSpan) || apart(sc->g, sc->g_low, kFactorSpan);
+}
 
 // 2^e such that the largest magnitude times it lies in [2^top, 2^(top+1)); 1 for zero.
 __device__ __forceinline__ int scale_exp(unsigned bits, int top) {
   if (bits == 0) return 0;
   const int e = bits >= 0x800000u ? (int)(bits >> 23) - 127 : -118 - __clz((int)bits);
-  return min(100, max(-100, top - e));
+  return min(126, max(-126, top - e));
 }
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
 constexpr int kOperandTop = 13, kProbTop = 14;
@@ -450,7 +469,7 @@ struct Source {
   int64_t ld, rows;
 };
 
-__device__ __forceinline__ void block_max(unsigned top, unsigned *to) {
+__device__ __forceinline__ void warp_max(unsigned top, unsigned *to) {
   top = __reduce_max_sync(kFullMask, top);
   if ((threadIdx.x & 31) == 0 && top) atomicMax(to, top);
 }
@@ -458,83 +477,113 @@ __device__ __forceinline__ void block_max(unsigned top, unsigned *to) {
 // Bits of a magnitude; an infinity or a NaN counts as zero: it spoils its own row, not the others' scale.
 __device__ __forceinline__ unsigned magnitude(float x) {
   const unsigned bits = __float_as_uint(x) & 0x7fffffffu;
-  return bits < 0x7f800000u ? bits : 0u;
+  return bits < kInfBits ? bits : 0u;
 }
 
-// Largest finite magnitudes of fp32 operands (z = 0: H, 1: W) and of the rows' g_n k_n (z = 2).
+// Largest finite magnitudes of fp32 operands (z = 0: H, 1: W) and of the rows' g_n k_n (z = 2), and the smallest row's.
 __global__ void __launch_bounds__(256) amax_kernel(Source h, Source w, int dim, const float *gloss,
                                                    const int *targets, int labels, int64_t vocab, Scalars *sc) {
   chain_wait();
-  unsigned top = 0;
+  unsigned top = 0, low = 0;
   if (blockIdx.z < 2) {
     const Source s = blockIdx.z == 0 ? h : w;
     if (!s.p) return;
     const float *a = static_cast<const float *>(s.p);
     const int lane = threadIdx.x & 31;
     const bool wide = reinterpret_cast<uintptr_t>(a) % 32 == 0 && s.ld % 8 == 0;
-    for (int64_t r = (int64_t)blockIdx.x * 8 + threadIdx.x / 32; r < s.rows; r += (int64_t)gridDim.x * 8)
+    for (int64_t r = (int64_t)blockIdx.x * 8 + threadIdx.x / 32; r < s.rows; r += (int64_t)gridDim.x * 8) {
+      unsigned most = 0;
       for (int c = lane * 8; c < dim; c += 256) {
         const int have = min(8, dim - c);
         float x[8];
         if (wide && have == 8) load8(a + r * s.ld + c, x);
         else load_some(a + r * s.ld + c, have, x);
 #pragma unroll
-        for (int e = 0; e < 8; e++) top = max(top, magnitude(x[e]));
+        for (int e = 0; e < 8; e++) most = max(most, magnitude(x[e]));
       }
-    block_max(top, blockIdx.z == 0 ? &sc->h : &sc->w);
+      most = __reduce_max_sync(kFullMask, most);
+      top = max(top, most);
+      if (most) low = max(low, kInfBits - most);
+    }
+    warp_max(top, blockIdx.z == 0 ? &sc->h : &sc->w);
+    warp_max(low, blockIdx.z == 0 ? &sc->h_low : &sc->w_low);
   } else if (gloss) {
     for (int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x; n < h.rows; n += (int64_t)gridDim.x * 256) {
       const int k = valid_targets(targets + n * labels, labels, vocab);
-      if (k) top = max(top, magnitude(gloss[n] * (float)k));
+      const unsigned m = k ? magnitude(gloss[n] * (float)k) : 0u;
+      top = max(top, m);
+      if (m) low = max(low, kInfBits - m);
     }
-    block_max(top, &sc->g);
+    warp_max(top, &sc->g);
+    warp_max(low, &sc->g_low);
   }
 }
 
-// Rows of T as rows of `width` (a multiple of 64) 16-bit elements, zeros behind the last column;
-// fp32 as `parts` of them: hi, lo, and hi 2^-11.
+// Rows of T as rows of `width` (a multiple of 64) 16-bit elements, zeros behind the last column.
 template <typename T>
-__device__ __forceinline__ void stage_row(const T *src, int dim, T *dst, int width, int, float) {
+__device__ __forceinline__ void stage_row(const T *src, int dim, T *dst, int width) {
   for (int c = (threadIdx.x & 31) * 8; c < width; c += 256) {
     float x[8];
     load_some(src + c, min(8, max(0, dim - c)), x);
     store8(dst + c, x);
   }
 }
-template <>
-__device__ __forceinline__ void stage_row<float>(const float *src, int dim, float *to, int width, int parts,
-                                                 float scale) {
-  __half *dst = reinterpret_cast<__half *>(to);
+
+// x as T, and in its place what that lacks (nothing where it is not finite).
+template <typename T>
+__device__ __forceinline__ float take_part(float &x) {
+  float hi = to_float(from_float<T>(x));
+  if (isinf(hi) && isfinite(x)) hi = __uint_as_float(__float_as_uint(x) & 0xffff0000u);   // bf16 rounds up to infinity
+  x = isfinite(hi) ? x - hi : 0.f;
+  return hi;
+}
+
+// fp32 as `parts` of them: fp16 hi, lo and hi 2^-11, or, WIDE, three bf16 ones that add up to it.
+template <bool WIDE>
+__device__ __forceinline__ void stage_split(const float *src, int dim, uint16_t *to, int width, int parts, float scale) {
+  using P = typename std::conditional<WIDE, __nv_bfloat16, __half>::type;
+  P *dst = reinterpret_cast<P *>(to);
   for (int c = (threadIdx.x & 31) * 8; c < width; c += 256) {
     const int have = min(8, max(0, dim - c));
-    float x[8], lo[8], small[8];
+    float x[8], hi[8], lo[8], small[8];
     if (have == 8 && reinterpret_cast<uintptr_t>(src + c) % 32 == 0) load8(src + c, x);
     else load_some(src + c, have, x);
 #pragma unroll
     for (int e = 0; e < 8; e++) {
-      const float y = x[e] * scale;
-      x[e] = __half2float(__float2half_rn(y));
-      lo[e] = isfinite(x[e]) ? y - x[e] : 0.f;
-      small[e] = x[e] * 0x1p-11f;
+      x[e] *= scale;
+      hi[e] = take_part<P>(x[e]);
+      if (WIDE) {
+        lo[e] = take_part<P>(x[e]);
+        small[e] = x[e];
+      } else {
+        lo[e] = x[e];
+        small[e] = hi[e] * 0x1p-11f;
+      }
     }
-    store8(dst + c, x);
+    store8(dst + c, hi);
     store8(dst + width + c, lo);
-    if (parts == 3) store8(dst + 2 * width + c, small);
+    if (WIDE || parts == 3) store8(dst + 2 * width + c, small);
   }
 }
 
+// Rows lie `pitch` elements apart; `parts` of fp32 are needed (three where they are bf16).
 template <typename T>
-__global__ void __launch_bounds__(256) stage_kernel(Source h, Source w, int dim, void *hs, void *ws, int width, int parts,
-                                                    const Scalars *sc) {
+__global__ void __launch_bounds__(256) stage_kernel(Source h, Source w, int dim, uint16_t *hs, uint16_t *ws, int width,
+                                                    int64_t pitch, int parts, Scalars *sc) {
   chain_wait();
   const Source s = blockIdx.z == 0 ? h : w;
-  void *to = blockIdx.z == 0 ? hs : ws;
+  uint16_t *to = blockIdx.z == 0 ? hs : ws;
   if (!to) return;
   constexpr bool split = sizeof(T) == 4;
   const float scale = split ? pow2(scale_exp(blockIdx.z == 0 ? sc->h : sc->w, kOperandTop)) : 1.f;
+  const bool wide = split && find_wide(sc);
+  if (wide && blockIdx.x == 0 && blockIdx.z == 0 && threadIdx.x == 0) sc->wide = 1;
   for (int64_t r = (int64_t)blockIdx.x * 8 + threadIdx.x / 32; r < s.rows; r += (int64_t)gridDim.x * 8) {
-    char *dst = static_cast<char *>(to) + r * width * parts * 2;
-    stage_row<T>(static_cast<const T *>(s.p) + r * s.ld, dim, reinterpret_cast<T *>(dst), width, parts, scale);
+    const T *src = static_cast<const T *>(s.p) + r * s.ld;
+    uint16_t *dst = to + r * pitch;
+    if constexpr (!split) stage_row<T>(src, dim, reinterpret_cast<T *>(dst), width);
+    else if (wide) stage_split<true>(src, dim, dst, width, parts, scale);
+    else stage_split<false>(src, dim, dst, width, parts, scale);
   }
 }
 
@@ -723,6 +772,25 @@ struct Reader {
   }
 };
 
+// The products of parts, the smaller ones first (the tensor cores truncate what they accumulate): the parts
+// of A and of B in product q at bits 2 q.
+struct Parts {
+  int count;
+  unsigned a, b;
+  __device__ __forceinline__ int of_a(int q) const { return a >> 2 * q & 3; }
+  __device__ __forceinline__ int of_b(int q) const { return b >> 2 * q & 3; }
+};
+__host__ __device__ constexpr unsigned part_list(int a, int b, int c, int d = 0, int e = 0, int f = 0) {
+  return a | b << 2 | c << 4 | d << 6 | e << 8 | f << 10;
+}
+template <bool SPLIT, bool GRADIENTS>
+__device__ __forceinline__ Parts parts_of(bool wide) {
+  if (!SPLIT) return Parts{1, 0, 0};
+  if (wide) return Parts{6, part_list(1, 2, 0, 1, 0, 0), part_list(1, 0, 2, 0, 1, 0)};
+  // lo hi, hi lo, hi hi; of gradients (lo 2^11) (hi 2^-11), hi lo, hi hi
+  return Parts{3, part_list(1, 0, 0), GRADIENTS ? part_list(2, 1, 0) : part_list(0, 1, 0)};
+}
+
 // ---- logits, and d ---------------------------------------------------------------------------
 enum Use { kLogits, kProbs };
 
@@ -730,11 +798,10 @@ struct Product {
   CUtensorMap a, b;         // H and W
   int mt, nt;               // tiles
   int kblocks, k16;         // of 64 for one pair of parts; steps of 16 in the last one
-  int pairs, pa[3], pb[3];  // offsets of the parts that are multiplied, the smaller products first
+  int a_part, b_part;       // from one part of an operand to the next
   int a_y, b_y;             // first row of each
   int bf16;
-  const Scalars *sc;
-  int split_scale;          // operands carry the scales of sc
+  const Scalars *sc;        // operands in parts carry its scales
   int64_t vocab;
   int rows;                 // rows that exist
   Part *parts;
@@ -745,7 +812,7 @@ struct Product {
   int labels;
   uint16_t *probs;          // d in strips of 64 columns: [part][strip][row][64], see put_strip
   int strip;                // rows of a strip
-  int64_t prob_lo;          // offset of the second part, 0 for none
+  int64_t prob_part;        // from one part to the next
 };
 
 template <bool BF16>
@@ -758,16 +825,22 @@ __device__ __forceinline__ uint32_t halves(float a, float b) {
   return *reinterpret_cast<const uint32_t *>(&p);
 }
 
-// 32 values as 16 bits, and for LO what those lack, times 2^11.
-template <bool BF16, bool LO>
-__device__ __forceinline__ void pack32(const float (&x)[32], uint32_t *hi, uint32_t *lo) {
+// 32 values as 16 bits.
+template <bool BF16>
+__device__ __forceinline__ void pack32(const float *x, uint32_t *to) {
 #pragma unroll
-  for (int i = 0; i < 16; i++) {
-    hi[i] = halves<BF16>(x[2 * i], x[2 * i + 1]);
-    if (LO) {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi[i]));
-      lo[i] = halves<false>((x[2 * i] - f.x) * 2048.f, (x[2 * i + 1] - f.y) * 2048.f);
-    }
+  for (int i = 0; i < 16; i++) to[i] = halves<BF16>(x[2 * i], x[2 * i + 1]);
+}
+// What 16-bit values lack of the 64 they were made from, times 2^11 for fp16, in their place.
+template <bool BF16>
+__device__ __forceinline__ void leave_rest(float (&x)[64], const uint32_t (&taken)[32]) {
+#pragma unroll
+  for (int i = 0; i < 32; i++) {
+    float a, b;
+    if (BF16) unpack2(taken[i], a, b, __nv_bfloat16());
+    else unpack2(taken[i], a, b, __half());
+    x[2 * i] = (x[2 * i] - a) * (BF16 ? 1.f : 2048.f);
+    x[2 * i + 1] = (x[2 * i + 1] - b) * (BF16 ? 1.f : 2048.f);
   }
 }
 
@@ -799,7 +872,8 @@ constexpr int kProductStages = USE == kProbs ? 5 : 6;
 template <Use USE>
 constexpr int kProductSmem = smem_bytes(kProductStages<USE>, USE == kProbs ? 8 * 4096 : 0);
 
-template <Use USE>
+// SPLIT: fp32 operands in parts.
+template <Use USE, bool SPLIT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) product_kernel(const __grid_constant__ Product p) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char *smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
@@ -811,6 +885,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) prod
   const uint32_t tmem = pair_begin(pipe, 8);
   const int rank = (int)cluster_rank(), pair = blockIdx.x / 2, npairs = gridDim.x / 2;
   const int tiles = p.mt * p.nt;
+  const bool wide = SPLIT && p.sc->wide;
+  const Parts parts = parts_of<SPLIT, false>(wide);
   // pairs that run together share a few tiles of W, against all rows
   auto first_row = [&](int t) { return t % p.mt * kPairM + rank * kM; };
   auto column_tile = [&](int t) { return t / p.mt; };
@@ -821,13 +897,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) prod
       bool ok = true;
       for (int t = pair; ok && t < tiles; t += npairs) {
         const int row = p.a_y + first_row(t), col = p.b_y + column_tile(t) * kN + rank * (kN / 2);
-        for (int q = 0; ok && q < p.pairs; q++)
+        for (int q = 0; ok && q < parts.count; q++)
           for (int kb = 0; kb < p.kblocks; kb++) {
             unsigned char *a, *b;
             uint32_t bar;
             if (!(ok = ring.next(2 * kBytesStage, a, b, bar))) break;
-            tma_load_2d(a, &p.a, p.pa[q] + kb * kK, row, bar);
-            tma_load_2d(b, &p.b, p.pb[q] + kb * kK, col, bar);
+            tma_load_2d(a, &p.a, parts.of_a(q) * p.a_part + kb * kK, row, bar);
+            tma_load_2d(b, &p.b, parts.of_b(q) * p.b_part + kb * kK, col, bar);
           }
       }
       if (!ok || !ring.drain()) ring.settle();
@@ -837,13 +913,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) prod
     if (rank == 0 && elected()) {
       Issue<STAGES> issue{pipe, gave_up, tmem, smem_addr(smem)};
       bool ok = true;
-      const uint32_t idesc = mma_desc(p.bf16, false, false, kPairM, kN);
+      const uint32_t idesc = mma_desc(SPLIT ? wide : p.bf16, false, false, kPairM, kN);
       const uint64_t da = issue.desc(0, false), db = issue.desc(kBytesA, false);
       for (int t = pair; ok && t < tiles; t += npairs) {
         uint32_t d;
         if (!(ok = issue.begin(d))) break;
         bool add = false;
-        for (int q = 0; ok && q < p.pairs; q++)
+        for (int q = 0; ok && q < parts.count; q++)
           for (int kb = 0; ok && kb < p.kblocks; kb++) {
             ok = issue.template block<false>(d, da, db, 2, 2, idesc, add, kb == p.kblocks - 1 ? p.k16 : kK / 16);
             add = true;
@@ -898,7 +974,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) prod
   } else if (warp >= 4) {
     const int half = (warp - 4) / 4, row = (warp & 3) * 32 + lane;
     float c = kLog2e;
-    if (p.split_scale) c = kLog2e * pow2(-scale_exp(p.sc->h, kOperandTop)) * pow2(-scale_exp(p.sc->w, kOperandTop));
+    if (SPLIT) c = kLog2e * pow2(-scale_exp(p.sc->h, kOperandTop)) * pow2(-scale_exp(p.sc->w, kOperandTop));
     Reader reader(pipe, gave_up, tmem);
     for (int t = pair; t < tiles; t += npairs) {
       const int n = column_tile(t);
@@ -942,7 +1018,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) prod
         const int *y = p.targets + r * p.labels;
         unsigned char *buffer = smem + STAGES * kBytesStage + (warp - 4) * 4096;
         for (int strip = 2 * half; strip < 2 * half + 2; strip++) {
-          uint32_t hi[32], lo[32];
+          uint32_t taken[32];
+          float all[64];   // both halves of the strip, while parts of them are taken
 #pragma unroll
           for (int b = 0; b < 2; b++) {
             const int ch = 2 * strip + b;
@@ -964,13 +1041,35 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) prod
                 }
               __syncwarp();
             }
-            if (p.bf16) pack32<true, false>(x, hi + 16 * b, nullptr);
-            else if (p.prob_lo) pack32<false, true>(x, hi + 16 * b, lo + 16 * b);
-            else pack32<false, false>(x, hi + 16 * b, nullptr);
+            if (SPLIT) {
+#pragma unroll
+              for (int i = 0; i < 32; i++) all[32 * b + i] = x[i];
+            } else if (p.bf16) {
+              pack32<true>(x, taken + 16 * b);
+            } else {
+              pack32<false>(x, taken + 16 * b);
+            }
           }
           uint16_t *to = p.probs + ((int64_t)(n * (kN / 64) + strip) * p.strip + r - lane) * 64;
-          put_strip(buffer, to, hi);
-          if (p.prob_lo) put_strip(buffer, to + p.prob_lo, lo);
+          if (!SPLIT) {
+            put_strip(buffer, to, taken);
+          } else if (!wide) {
+#pragma unroll
+            for (int part = 0; part < 2; part++) {
+              pack32<false>(all, taken);
+              pack32<false>(all + 32, taken + 16);
+              if (part == 0) leave_rest<false>(all, taken);
+              put_strip(buffer, to + part * p.prob_part, taken);
+            }
+          } else {
+#pragma unroll 1
+            for (int part = 0; part < 3; part++) {
+              pack32<true>(all, taken);
+              pack32<true>(all + 32, taken + 16);
+              leave_rest<true>(all, taken);
+              put_strip(buffer, to + part * p.prob_part, taken);
+            }
+          }
         }
       }
       reader.end();
@@ -991,7 +1090,7 @@ struct Side {
   int kblocks, tiles, whole;// of 64; tiles, and how many each pair takes whole
   int a_mn;                 // d transposed
   int b_y;                  // first row of the operand
-  int pa[3], pb[3];
+  int a_part, b_part;       // from one part of d and of the operand to the next
   int rows;
   float *acc;               // sums of earlier launches, or of this one for later ones
   int add, last;
@@ -1007,7 +1106,6 @@ struct Gradients {
   int nt, ntile, nlast;     // column tiles, their width and the last one's (multiples of 32)
   int npairs, sharers;      // pairs of CTAs; how many of them share what is left
   int64_t left;             // its blocks of K
-  int pairs, segment;       // pairs of parts; blocks of K that are accumulated in tensor memory at a time
   int bf16, strip, dim, out_type;
   int64_t ldacc;
   float *pieces;            // [pair][2][kPairM][ntile]
@@ -1133,6 +1231,11 @@ __device__ __forceinline__ void put_tile(const Gradients &g, const Side &s, int6
   __syncwarp();
 }
 
+// Blocks of K that are accumulated in tensor memory at a time: all, or for SEGMENTS (fp32) as many as have
+// six products.
+template <bool SEGMENTS>
+__device__ __forceinline__ int segment_of(bool wide) { return !SEGMENTS ? 1 << 30 : wide ? 1 : 2; }
+
 constexpr int kGradStages = 5, kGradSmem = smem_bytes(kGradStages, 0);
 
 // SEGMENTS (fp32): the tensor cores truncate what they accumulate, so after `segment` blocks of K the sum
@@ -1154,6 +1257,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGradThreads<SEGMENT
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
   const uint32_t tmem = pair_begin(pipe, kGradReaders<SEGMENTS>);
   const int rank = (int)cluster_rank();
+  const bool wide = SEGMENTS && g.side[0].rescale.sc->wide;
+  const Parts parts = parts_of<SEGMENTS, true>(wide);
+  const int segment = segment_of<SEGMENTS>(wide);
   Walk walk(g, blockIdx.x / 2);
   Piece p;
 
@@ -1167,20 +1273,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGradThreads<SEGMENT
         const int half_n = g.width(p.tile % g.nt) / 2, groups = (half_n + 63) / 64;
         const unsigned bytes = 2 * (kBytesA + groups * 8192);
         const int row = p.tile / g.nt * kPairM + rank * kM, col = p.tile % g.nt * g.ntile + rank * half_n;
-        for (int k0 = p.k0; ok && k0 < p.k1; k0 += g.segment)
-          for (int q = 0; ok && q < g.pairs; q++)
-            for (int kb = k0; kb < min(p.k1, k0 + g.segment); kb++) {
+        for (int k0 = p.k0; ok && k0 < p.k1; k0 += segment)
+          for (int q = 0; ok && q < parts.count; q++)
+            for (int kb = k0; kb < min(p.k1, k0 + segment); kb++) {
               unsigned char *a, *b;
               uint32_t bar;
               if (!(ok = ring.next(bytes, a, b, bar))) break;
+              const int a_at = parts.of_a(q) * s.a_part;
               if (s.a_mn) {   // 64 rows of two strips
                 for (int i = 0; i < 2; i++)
-                  tma_load_2d(a + i * 8192, &s.a, 0, s.pa[q] + (row / 64 + i) * g.strip + kb * kK, bar);
+                  tma_load_2d(a + i * 8192, &s.a, 0, a_at + (row / 64 + i) * g.strip + kb * kK, bar);
               } else {        // 128 rows of a strip
-                tma_load_2d(a, &s.a, 0, s.pa[q] + kb * g.strip + row, bar);
+                tma_load_2d(a, &s.a, 0, a_at + kb * g.strip + row, bar);
               }
               for (int i = 0; i < groups; i++)
-                tma_load_2d(b + i * 8192, &s.b, s.pb[q] + col + i * 64, s.b_y + kb * kK, bar);
+                tma_load_2d(b + i * 8192, &s.b, parts.of_b(q) * s.b_part + col + i * 64, s.b_y + kb * kK, bar);
             }
       }
       if (!ok || !ring.drain()) ring.settle();
@@ -1192,13 +1299,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGradThreads<SEGMENT
       bool ok = true;
       while (ok && walk.next(p)) {
         const bool mn = g.side[p.side].a_mn;
-        const uint32_t idesc = mma_desc(g.bf16, mn, true, kPairM, g.width(p.tile % g.nt));
+        const uint32_t idesc = mma_desc(SEGMENTS ? wide : g.bf16, mn, true, kPairM, g.width(p.tile % g.nt));
         const uint64_t da = issue.desc(0, mn), db = issue.desc(kBytesA, true);
         const uint32_t step_a = mn ? 2048 >> 4 : 32 >> 4;
-        for (int k0 = p.k0; ok && k0 < p.k1; k0 += g.segment) {
+        for (int k0 = p.k0; ok && k0 < p.k1; k0 += segment) {
           uint32_t d;
           if (!(ok = issue.begin(d))) break;
-          const int blocks = g.pairs * (min(p.k1, k0 + g.segment) - k0);
+          const int blocks = parts.count * (min(p.k1, k0 + segment) - k0);
           for (int b = 0; ok && b < blocks; b++) ok = issue.template block<true>(d, da, db, step_a, 2048 >> 4, idesc, b > 0, kK / 16);
           if (ok) issue.end();
         }
@@ -1245,7 +1352,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGradThreads<SEGMENT
         for (int i = 0; i < 4; i++)
 #pragma unroll
           for (int e = 0; e < 16; e++) acc[i][e] = 0.f;
-        for (int k0 = p.k0; k0 < p.k1; k0 += g.segment) {
+        for (int k0 = p.k0; k0 < p.k1; k0 += segment) {
           reader.begin();
           if (part * 64 < width) {
 #pragma unroll
@@ -1387,11 +1494,12 @@ int allow_smem(size_t bytes) {
 }
 int sm_pairs() { return std::max(1, device_sm_count() / 2); }
 
-template <Use USE>
+template <Use USE, typename T>
 int launch_product(const Product &p, cudaStream_t s) {
-  const int err = allow_smem<product_kernel<USE>>(kProductSmem<USE>);
+  constexpr bool split = sizeof(T) == 4;
+  const int err = allow_smem<product_kernel<USE, split>>(kProductSmem<USE>);
   if (err) return err;
-  product_kernel<USE><<<2 * std::min(p.mt * p.nt, sm_pairs()), kMmaThreads, kProductSmem<USE>, s>>>(p);
+  product_kernel<USE, split><<<2 * std::min(p.mt * p.nt, sm_pairs()), kMmaThreads, kProductSmem<USE>, s>>>(p);
   count_launch(1);
   return (int)cudaGetLastError();
 }
@@ -1424,7 +1532,6 @@ bool good_shape(const Shape &x) {
 constexpr int64_t kLossRows = 16384;            // rows whose parts are kept at a time
 constexpr int64_t kGradRows = 8192;             // rows of a piece of d
 constexpr int64_t kProbBytes = (int64_t)256 << 20;
-constexpr int kSegment = 2;                     // fp32 gradients: blocks of K between two roundings
 
 int few_blocks(int64_t vocab) {
   const int64_t need = (vocab + kFewThreads / 32 * kFewWords - 1) / (kFewThreads / 32 * kFewWords);
@@ -1473,7 +1580,7 @@ Layout plan(const Shape &x, bool grad) {
     return l;
   }
   l.width = (int)up(x.dim, 64);
-  l.nparts = x.type == W2V_F32 ? (grad ? 3 : 2) : 1;
+  l.nparts = x.type == W2V_F32 ? 3 : 1;
   l.hs = take(x.n * l.width * l.nparts * 2);
   l.ws = take(x.vocab * l.width * l.nparts * 2);
   if (!grad) {
@@ -1487,7 +1594,7 @@ Layout plan(const Shape &x, bool grad) {
     l.words = up((x.vocab + pieces - 1) / pieces, kN);
     column_tiles(x.dim, &l.nt, &l.ntile, &l.nlast);
     const int64_t cols = (int64_t)l.nt * l.ntile * 4;
-    l.probs = take(l.rows * l.words * bytes);
+    l.probs = take(l.rows * l.words * 2 * l.nparts);
     l.pieces = take((int64_t)sm_pairs() * 2 * kPairM * l.ntile * 4);
     if (l.words < x.vocab) l.acc_h = take(l.rows * cols);
     if (l.rows < x.n) l.acc_w = take(up(x.vocab, kPairM) * cols);
@@ -1504,7 +1611,7 @@ bool direct(const void *p, int64_t ld) {   // TMA can read the caller's matrix
 // Operands for the products: the caller's own where TMA can read them, else staged ones.
 template <typename T>
 int stage(const Shape &x, const Layout &l, const void *h, int64_t ldh, const void *w, int64_t ldw, const float *gloss,
-          const int *targets, char *ws, Operand *oh, Operand *ow, cudaStream_t s) {
+          const int *targets, int parts, char *ws, Operand *oh, Operand *ow, cudaStream_t s) {
   constexpr bool split = sizeof(T) == 4;
   Scalars *sc = reinterpret_cast<Scalars *>(ws + l.scalars);
   const Source sh{h, ldh, x.n}, sw{w, ldw, x.vocab};
@@ -1517,12 +1624,13 @@ int stage(const Shape &x, const Layout &l, const void *h, int64_t ldh, const voi
                                    split ? sw : Source{nullptr, 0, 0}, x.dim, gloss, targets, x.labels, x.vocab, sc);
     if (err) return err;
   }
-  void *hs = direct<T>(h, ldh) ? nullptr : ws + l.hs, *wst = direct<T>(w, ldw) ? nullptr : ws + l.ws;
+  uint16_t *hs = direct<T>(h, ldh) ? nullptr : reinterpret_cast<uint16_t *>(ws + l.hs);
+  uint16_t *wst = direct<T>(w, ldw) ? nullptr : reinterpret_cast<uint16_t *>(ws + l.ws);
+  const int64_t staged = (int64_t)l.width * l.nparts;
   if (hs || wst) {
-    const int err = launch_chained(stage_kernel<T>, dim3(blocks, 1, 2), 256, 0, s, sh, sw, x.dim, hs, wst, l.width, l.nparts, sc);
+    const int err = launch_chained(stage_kernel<T>, dim3(blocks, 1, 2), 256, 0, s, sh, sw, x.dim, hs, wst, l.width, staged, parts, sc);
     if (err) return err;
   }
-  const int64_t staged = (int64_t)l.width * l.nparts;
   *oh = hs ? Operand{hs, staged, staged, x.n, l.width} : Operand{h, ldh, x.dim, x.n, 0};
   *ow = wst ? Operand{wst, staged, staged, x.vocab, l.width} : Operand{w, ldw, x.dim, x.vocab, 0};
   return 0;
@@ -1531,19 +1639,14 @@ int stage(const Shape &x, const Layout &l, const void *h, int64_t ldh, const voi
 template <typename T>
 int logits_product(const Shape &x, const Operand &oh, const Operand &ow, const Scalars *sc, Product *to) {
   Product p{};
-  constexpr bool split = sizeof(T) == 4;
   int err = tensor_map(&p.a, oh.p, oh.inner, oh.rows, oh.ld, kM);
   if (!err) err = tensor_map(&p.b, ow.p, ow.inner, ow.rows, ow.ld, kN / 2);
   p.kblocks = (x.dim + kK - 1) / kK;
   p.k16 = (x.dim - (p.kblocks - 1) * kK + 15) / 16;
-  p.pairs = split ? 3 : 1;
-  if (split) {   // lo hi, hi lo, hi hi
-    p.pa[0] = oh.width;
-    p.pb[1] = ow.width;
-  }
+  p.a_part = oh.width;
+  p.b_part = ow.width;
   p.bf16 = x.type == W2V_BF16;
   p.sc = sc;
-  p.split_scale = split;
   p.vocab = x.vocab;
   *to = p;
   return err;
@@ -1589,7 +1692,7 @@ int run_loss(const Shape &x, const Layout &l, const void *h, int64_t ldh, const 
     return err;
   }
   Operand oh, ow;
-  int err = stage<T>(x, l, h, ldh, w, ldw, nullptr, nullptr, ws, &oh, &ow, s);
+  int err = stage<T>(x, l, h, ldh, w, ldw, nullptr, nullptr, 2, ws, &oh, &ow, s);
   if (err) return err;
   Product p;
   err = logits_product<T>(x, oh, ow, reinterpret_cast<const Scalars *>(ws + l.scalars), &p);
@@ -1601,7 +1704,7 @@ int run_loss(const Shape &x, const Layout &l, const void *h, int64_t ldh, const 
     p.mt = (p.rows + kPairM - 1) / kPairM;
     p.a_y = (int)r0;
     p.ldparts = p.rows;
-    err = launch_product<kLogits>(p, s);
+    err = launch_product<kLogits, T>(p, s);
     if (!err) err = join_rows(2 * p.nt, p.ldparts, r0, p.rows);
     if (err) return err;
   }
@@ -1657,7 +1760,7 @@ int run_grad(const Shape &x, const Layout &l, const void *h, int64_t ldh, const 
   constexpr bool split = sizeof(T) == 4;
   const float *each_gloss = ldg ? gloss : nullptr, *one_gloss = ldg ? nullptr : gloss;
   Operand oh, ow;
-  int err = stage<T>(x, l, h, ldh, w, ldw, each_gloss, targets, ws, &oh, &ow, s);
+  int err = stage<T>(x, l, h, ldh, w, ldw, each_gloss, targets, 3, ws, &oh, &ow, s);
   if (err) return err;
   const Scalars *sc = reinterpret_cast<const Scalars *>(ws + l.scalars);
   // one factor for all rows is left to the end: the targets' -1 then has no rounding in d
@@ -1673,15 +1776,13 @@ int run_grad(const Shape &x, const Layout &l, const void *h, int64_t ldh, const 
   p.given = given;
   p.probs = reinterpret_cast<uint16_t *>(ws + l.probs);
   p.strip = (int)l.rows;
-  p.prob_lo = split ? (int64_t)strip_rows * 64 : 0;
+  p.prob_part = (int64_t)strip_rows * 64;
 
   Gradients g{};
   g.nt = l.nt;
   g.ntile = l.ntile;
   g.nlast = l.nlast;
   g.npairs = sm_pairs();
-  g.pairs = split ? 3 : 1;
-  g.segment = split ? kSegment : 1 << 30;
   g.bf16 = x.type == W2V_BF16;
   g.strip = (int)l.rows;
   g.dim = x.dim;
@@ -1692,13 +1793,10 @@ int run_grad(const Shape &x, const Layout &l, const void *h, int64_t ldh, const 
     Side &side = g.side[i];
     const Operand &o = i == 0 ? oh : ow;
     side.a_mn = i == 0;
-    err = tensor_map(&side.a, ws + l.probs, 64, (int64_t)strip_rows * (split ? 2 : 1), 64, side.a_mn ? 64 : kM, true);
+    err = tensor_map(&side.a, ws + l.probs, 64, (int64_t)strip_rows * l.nparts, 64, side.a_mn ? 64 : kM, true);
     if (!err) err = tensor_map(&side.b, o.p, o.inner, o.rows, o.ld, 64);
-    if (split) {   // (lo 2^11) (hi 2^-11), hi lo, hi hi
-      side.pa[0] = strip_rows;
-      side.pb[0] = 2 * o.width;
-      side.pb[1] = o.width;
-    }
+    side.a_part = strip_rows;
+    side.b_part = o.width;
     side.rescale = Rescale{sc, one_gloss, given, split ? (i == 0 ? 2 : 1) : 0};
     side.ldout = i == 0 ? lddw : lddh;
   }
@@ -1716,7 +1814,7 @@ int run_grad(const Shape &x, const Layout &l, const void *h, int64_t ldh, const 
       p.lse = lse + r0;
       p.gloss = each_gloss ? each_gloss + r0 : nullptr;
       p.targets = targets + r0 * x.labels;
-      err = launch_product<kProbs>(p, s);
+      err = launch_product<kProbs, T>(p, s);
       if (err) return err;
       g.left = 0;
       for (int i = 0; i < 2; i++) {

@@ -23,7 +23,10 @@ class Softmax:
     ``hidden`` is ``[n, dim]``, ``weight`` ``[vocab, dim]``, both fp32, bf16 or fp16, ``dim`` up to 4096;
     ``targets`` int32 ``[n]`` or ``[n, labels]``.  A target outside ``[0, vocab)`` (-1 by convention) stands
     for none; a row may have none (its loss and gradient are zero) or the same word more than once.
-    fp32 operands are multiplied to 22 bits and accumulated in fp32; 16-bit ones are multiplied exactly.
+    fp32 operands are multiplied to 22 bits, counted from the largest number of each one's row, and accumulated
+    in fp32; 16-bit ones are multiplied exactly.  (Rows or factors of very different sizes, beyond 2^14 or 2^12
+    between the largest and the smallest that is not zero, take twice the time; what is below 2^-60
+    of the largest may be lost.)
     Every row takes part in the products: an infinity or a NaN in a row of ``hidden``, with targets or without,
     or in ``gloss`` spoils that row's results and ``dweight``, one in ``weight`` all rows'.
     Outputs that are given share no memory with the inputs or with each other."""

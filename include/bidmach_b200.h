@@ -461,7 +461,8 @@ int w2v_window_rows(const int *words, const int *lb, const int *ub, int n, int n
  *   lse[i]  = log sum_v exp l[i][v]
  *   loss[i] = sum over the targets y of row i of (lse[i] - l[i][y])        (0 without any)
  * hidden is n x dim, weight vocab x dim, both of `type`; loss and lse are fp32[n].  dim <= 4096,
- * labels <= 1024.  A row of hidden with an infinity or a NaN gives a NaN in its own lse (and in dweight),
+ * labels <= 1024.  fp32 operands are multiplied to 22 bits, counted from the largest number of each one's
+ * row (rows down to 2^-60 of the largest one).  A row of hidden with an infinity or a NaN gives a NaN in its own lse (and in dweight),
  * a row of weight in all of them. */
 int64_t w2v_softmax_workspace(int64_t n, int64_t vocab, int dim, int labels, int type, int grad);   /* -1: refused */
 int w2v_softmax_loss(const void *hidden, int64_t ldh, const void *weight, int64_t ldw,
