@@ -445,8 +445,10 @@ __global__ void __launch_bounds__(kJoinThreads) loss_join_kernel(const Part *par
     }
 #pragma unroll
     for (int q = 0; q < 2; q++) {
-      const float l = warp_sum(x[q]);
-      if (at[q] >= 0 && at[q] < vocab) sum += z - l;
+      // z and l are sums of their own, each with its own rounding: for a row that is sure of its target their
+      // difference may come out below zero, which it never is (a NaN stays)
+      const float term = z - warp_sum(x[q]);
+      if (at[q] >= 0 && at[q] < vocab) sum += term < 0.f ? 0.f : term;
     }
   }
   if (lane == 0) {

@@ -354,3 +354,16 @@ def test_not_finite_numbers_stay_in_their_rows(n, t, size, where):
     assert all(torch.isfinite(x).all() for x in (loss, lse, dh))
     hold((loss, lse, dh, clean[3].cpu()), hidden, weight, targets, gloss, t)
     assert torch.isnan(got[2][~good]).any(1).all()
+
+
+@pytest.mark.parametrize("n", [1, 4, 16, 200])
+@pytest.mark.parametrize("t", list(TYPES))
+def test_loss_of_sure_rows_is_not_negative(n, t):
+    """Rows whose target has nearly all of the probability: the loss is the difference of two rounded numbers."""
+    for seed in range(4):
+        hidden, weight, targets, gloss = inputs(n, 700, 96, 3, t, seed=seed, size=12.0)
+        top = (hidden.double() @ weight.double().T).argmax(1)
+        targets[:] = top[:, None].int()
+        got = run(hidden, weight, targets, gloss)
+        assert (got[0] >= 0).all()
+        hold(got, hidden, weight, targets, gloss, t)
