@@ -125,6 +125,7 @@ SIGNATURES = {
                               C.c_int64, _P]),
     "w2v_softmax_grad": (_I, [_P, C.c_int64, _P, C.c_int64, _P, C.c_int64, C.c_int64, _I, _I, _I, _P, _P, C.c_int64,
                               _P, C.c_int64, _P, C.c_int64, _P, C.c_int64, _P]),
+    "w2v_softmax_fault": (C.POINTER(_I), []),
     "w2v_embed_rows": (_I, [_P, C.c_int64, _P, C.c_int64, C.c_int64, _I, _I, _P, C.c_int64, _P]),
     "w2v_embed_grad_workspace": (C.c_int64, [C.c_int64, C.c_int64, _I, _I]),
     "w2v_embed_grad": (_I, [_P, C.c_int64, _P, C.c_int64, C.c_int64, _I, _I, _P, C.c_int64, _P, C.c_int64, _P]),

@@ -637,9 +637,15 @@ __device__ __forceinline__ uint32_t pair_begin(Pipe &s, int readers) {
 // arrives without a thread behind it is waited for before: copies (`full`) by the issuer, finished
 // tiles (`tfull`) by both CTAs' readers, stages that were read (`empty`) by both CTAs' producers
 // (Ring::drain).  Where a wait ran out that chain is broken: a millisecond is long enough for any of them.
-__device__ __forceinline__ void pair_end(Pipe &s, uint32_t tmem) {
-  if (*const_cast<volatile int *>(&s.gave_up))
+// The host is told by `fault`.
+__device__ __forceinline__ void pair_end(Pipe &s, uint32_t tmem, int *fault) {
+  if (*const_cast<volatile int *>(&s.gave_up)) {
+    if (fault) {
+      *const_cast<volatile int *>(fault) = 1;
+      __threadfence_system();
+    }
     for (int i = 0; i < 1000; i++) __nanosleep(1000);
+  }
   tmem_before_sync();
   __syncwarp();
   cluster_sync();
@@ -815,6 +821,7 @@ struct Product {
   uint16_t *probs;          // d in strips of 64 columns: [part][strip][row][64], see put_strip
   int strip;                // rows of a strip
   int64_t prob_part;        // from one part to the next
+  int *fault;               // of pair_end
 };
 
 template <bool BF16>
@@ -1078,7 +1085,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) prod
     }
     if (USE == kProbs && lane == 0) bulk_wait_group_all();
   }
-  pair_end(pipe, tmem);
+  pair_end(pipe, tmem, p.fault);
 }
 
 // ---- gradients from a piece of d -------------------------------------------------------------
@@ -1111,6 +1118,7 @@ struct Gradients {
   int bf16, strip, dim, out_type;
   int64_t ldacc;
   float *pieces;            // [pair][2][kPairM][ntile]
+  int *fault;               // of pair_end
   __device__ __forceinline__ int width(int n) const { return n == nt - 1 ? nlast : ntile; }
 };
 
@@ -1373,7 +1381,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGradThreads<SEGMENT
       }
     }
   }
-  pair_end(pipe, tmem);
+  pair_end(pipe, tmem, g.fault);
 }
 
 // The tiles that were cut: blockIdx.x is the tile in what is left, a warp a row.
@@ -1494,6 +1502,32 @@ int allow_smem(size_t bytes) {
   if (e == cudaSuccess && device < kDevices) allowed[device].store(bytes);
   return (int)e;
 }
+// Raised by a kernel that gave up waiting: pinned host memory that every device can write, null where there
+// is none.
+int *fault_flag() {
+  static int *flag = [] {
+    int *f = nullptr;
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;   // the first call may be captured
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    const cudaError_t e = cudaHostAlloc(&f, sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    if (e != cudaSuccess) {
+      (void)cudaGetLastError();
+      return (int *)nullptr;
+    }
+    *f = 0;
+    return f;
+  }();
+  return flag;
+}
+// Reported once, by the first call that finds the flag raised.
+int take_fault() {
+  int *flag = fault_flag();
+  if (!flag || !*const_cast<volatile int *>(flag)) return 0;
+  *flag = 0;
+  return (int)cudaErrorLaunchTimeout;
+}
+
 int sm_pairs() { return std::max(1, device_sm_count() / 2); }
 
 template <Use USE, typename T>
@@ -1648,6 +1682,7 @@ int logits_product(const Shape &x, const Operand &oh, const Operand &ow, const S
   p.a_part = oh.width;
   p.b_part = ow.width;
   p.bf16 = x.type == W2V_BF16;
+  p.fault = fault_flag();
   p.sc = sc;
   p.vocab = x.vocab;
   *to = p;
@@ -1791,6 +1826,7 @@ int run_grad(const Shape &x, const Layout &l, const void *h, int64_t ldh, const 
   g.out_type = x.type;
   g.ldacc = (int64_t)l.nt * l.ntile;
   g.pieces = reinterpret_cast<float *>(ws + l.pieces);
+  g.fault = p.fault;
   for (int i = 0; i < 2 && !err; i++) {
     Side &side = g.side[i];
     const Operand &o = i == 0 ? oh : ow;
@@ -1845,6 +1881,8 @@ int run_grad(const Shape &x, const Layout &l, const void *h, int64_t ldh, const 
 
 }  // namespace
 
+extern "C" int *w2v_softmax_fault(void) { return fault_flag(); }
+
 extern "C" int64_t w2v_softmax_workspace(int64_t n, int64_t vocab, int dim, int labels, int type, int grad) {
   const Shape x{n, vocab, dim, labels, type};
   return good_shape(x) ? plan(x, grad != 0).total : -1;
@@ -1859,6 +1897,7 @@ extern "C" int w2v_softmax_loss(const void *hidden, int64_t ldh, const void *wei
   if (!hidden || !targets || !loss || !lse) return 1;
   const Layout l = plan(x, false);
   if (workspace_bytes < l.total) return 1;
+  if (const int fault = take_fault()) return fault;
   char *ws = static_cast<char *>(workspace);
   const auto s = static_cast<cudaStream_t>(stream);
   if (type == W2V_F32) return run_loss<float>(x, l, hidden, ldh, weight, ldw, targets, loss, lse, ws, s);
@@ -1877,6 +1916,7 @@ extern "C" int w2v_softmax_grad(const void *hidden, int64_t ldh, const void *wei
   if (n > 0 && (!hidden || !targets || !lse || !gloss || !dhidden)) return 1;
   const Layout l = plan(x, true);
   if (workspace_bytes < l.total) return 1;
+  if (const int fault = take_fault()) return fault;
   char *ws = static_cast<char *>(workspace);
   const auto s = static_cast<cudaStream_t>(stream);
   if (type == W2V_F32)

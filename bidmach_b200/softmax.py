@@ -7,6 +7,8 @@ from . import _lib
 from .adamw import TYPES, check, on_device, stream_of
 from .embed import check_apart, check_ids, check_matrix
 
+CUDA_ERROR_LAUNCH_TIMEOUT = 702
+
 
 def _vector(x, name: str, n: int, device):
     if not isinstance(x, torch.Tensor) or x.dtype is not torch.float32 or x.dim() != 1 or x.shape[0] != n \
@@ -54,6 +56,16 @@ class Softmax:
         if size < 0:
             raise ValueError("w2v_softmax_workspace refused the sizes")
         return torch.empty(size, dtype=torch.uint8, device=device), size
+
+    @staticmethod
+    def check():
+        """Raises where a kernel of an earlier call gave up waiting for its copies or products (its results
+        hold NaN then).  ``loss`` and ``grad`` do the same for the calls before them; this is for the last ones,
+        and for replayed graphs, when their stream has been waited for."""
+        flag = _lib.load().w2v_softmax_fault()
+        if flag and flag[0]:
+            flag[0] = 0
+            check(CUDA_ERROR_LAUNCH_TIMEOUT, "Softmax: a kernel gave up waiting:")
 
     @staticmethod
     def loss(hidden, weight, targets, loss=None, lse=None):

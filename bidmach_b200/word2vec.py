@@ -320,7 +320,9 @@ class Word2Vec:
         if pairs == 0:
             return 0.0
         loss, _ = Softmax.loss(EmbedRows.forward(ids, self.modelmats[0]), self.modelmats[1], targets)
-        return -float(loss.cpu().numpy().sum(dtype=np.float64)) / pairs
+        total = float(loss.cpu().numpy().sum(dtype=np.float64))
+        Softmax.check()
+        return -total / pairs
 
     # -- the pieces, one reference method each ------------------------------
     def wordMats(self, gmats, ipass: int = 0, pos: int = 0, uniforms=None, batch_id: int = 0):

@@ -478,6 +478,12 @@ int w2v_softmax_grad(const void *hidden, int64_t ldh, const void *weight, int64_
                      const float *lse, const float *gloss, int64_t ldg, void *dhidden, int64_t lddh,
                      void *dweight, int64_t lddw, void *workspace, int64_t workspace_bytes,
                      void *stream);
+/* A kernel of these two whose waits for its copies or products run out (some seconds; they take
+ * microseconds) writes NaN for what it did not compute and raises a flag in host memory.  The next call of
+ * either then returns cudaErrorLaunchTimeout, once, and does nothing else.  This is the flag, for callers
+ * that replay a graph or make no further call: read it when the work has finished, and clear it.  Null where no
+ * host memory could be pinned. */
+int *w2v_softmax_fault(void);
 
 /* One tensor of an AdamW step: `n` contiguous elements of `ptype`.  With 32-bit moments m and v are
  * fp32[n] and the scales null.  With 8-bit ones m and v are uint8[n] and every 256 elements share a

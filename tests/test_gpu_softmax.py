@@ -367,3 +367,20 @@ def test_loss_of_sure_rows_is_not_negative(n, t):
         got = run(hidden, weight, targets, gloss)
         assert (got[0] >= 0).all()
         hold(got, hidden, weight, targets, gloss, t)
+
+
+def test_the_next_call_says_that_a_kernel_gave_up():
+    """The flag that such a kernel raises, raised here by the host: the next call reports it and is then done with it,
+    before it has launched anything."""
+    from bidmach_b200 import Softmax, _lib
+    hidden, weight, targets, gloss = (x.cuda() for x in inputs(50, 300, 32, 1, "bf16"))
+    loss, lse = Softmax.loss(hidden, weight, targets)
+    flag, count = _lib.load().w2v_softmax_fault(), _lib.load().w2v_launch_count
+    for call in (lambda: Softmax.loss(hidden, weight, targets), lambda: Softmax.grad(hidden, weight, targets, lse, gloss),
+                 Softmax.check):
+        flag[0], before = 1, count()
+        with pytest.raises(RuntimeError, match="702|gave up|timed out|time"):
+            call()
+        assert count() == before and flag[0] == 0
+        call()
+    assert torch.equal(Softmax.loss(hidden, weight, targets)[0], loss)

@@ -116,3 +116,24 @@ def test_rounding_is_checked():
     assert lib.w2v_adamw_step_random(t, g, k, 1, C.byref(o), None, 1, 64, None) == 1
     assert lib.w2v_adamw_step_random(t, g, k, 1, C.byref(o), None, 1, 0, None) == 1
     assert lib.w2v_launch_count() == before
+
+
+def test_softmax_says_when_a_kernel_gave_up(monkeypatch):
+    """The flag that such a kernel raises, raised here on the host."""
+    from bidmach_b200 import Softmax, softmax
+
+    class Fake:
+        flag = (C.c_int * 1)(0)
+
+        def w2v_softmax_fault(self):
+            return self.flag
+
+    fake = Fake()
+    monkeypatch.setattr(softmax._lib, "load", lambda: fake)
+    Softmax.check()
+    fake.flag[0] = 1
+    with pytest.raises(RuntimeError, match="gave up"):
+        Softmax.check()
+    Softmax.check()      # said once
+    fake.w2v_softmax_fault = lambda: None      # no pinned memory
+    Softmax.check()
