@@ -8,6 +8,7 @@ from __future__ import annotations
 import ctypes as C
 import dataclasses
 import warnings
+from array import array
 
 import torch
 
@@ -80,6 +81,9 @@ class AdamW:
     the moments start at zero.  The arithmetic is fp32; a 16-bit parameter is rounded to nearest
     once a step, so a step smaller than half of its last place leaves it as it is.
 
+    A parameter may be given other memory between steps (``p.data = ...``); a captured step keeps the addresses
+    that it was captured with.
+
     The step count lives on the device: a captured step counts its replays."""
 
     Opts = Opts
@@ -99,6 +103,25 @@ class AdamW:
                           "give rounding='random' for training, or 'nearest'", stacklevel=2)
         if not self.params:
             raise ValueError("AdamW needs at least one tensor")
+        self._check_params()
+        self.device = self.params[0].device
+        if any(p.device != self.device for p in self.params):
+            raise ValueError("parameters on more than one device")
+        self.m, self.v, self.mscale, self.vscale, t = self._state(state)
+        n = len(self.params)
+        self._sizes = [p.numel() for p in self.params]
+        self._types = [p.dtype for p in self.params]
+        self._pointers = C.c_void_p * n
+        self._kinds = (C.c_int * n)(*[TYPES[t] for t in self._types])
+        self._table = (_lib.W2VAdamwTensor * n)()
+        self._fill()
+        self._clock = torch.zeros(4, dtype=torch.float64, device=self.device)
+        self._clock_at = self._clock.data_ptr()
+        with on_device(self.device):
+            check(_lib.load().w2v_adamw_clock(self._clock_at, o.beta1, o.beta2, t, stream_of(self.device)),
+                  "w2v_adamw_clock")
+
+    def _check_params(self):
         for p in self.params:
             if not isinstance(p, torch.Tensor) or p.dtype not in TYPES:
                 raise ValueError("parameters are fp32, bf16 or fp16 tensors")
@@ -107,28 +130,27 @@ class AdamW:
         self._apart(self.params, "two parameters overlap")
         if any(not p.is_cuda for p in self.params):
             raise ValueError("AdamW expects CUDA tensors")
-        self.device = self.params[0].device
-        if any(p.device != self.device for p in self.params):
-            raise ValueError("parameters on more than one device")
-        self.m, self.v, self.mscale, self.vscale, t = self._state(state)
+
+    def _fill(self):
+        """The table of addresses.  Aliases of the parameters are kept beside it, so that the memory it names
+        stays theirs until it is filled again."""
         self._apart([*self.params, *self.m, *self.v, *(self.mscale or ()), *(self.vscale or ())],
                     "a tensor of the state overlaps another or a parameter")
-        n = len(self.params)
-        self._sizes = [p.numel() for p in self.params]
-        self._types = [p.dtype for p in self.params]
-        self._pointers = C.c_void_p * n
-        self._kinds = (C.c_int * n)(*[TYPES[t] for t in self._types])
-        self._table = (_lib.W2VAdamwTensor * n)()
+        self._held = [p.detach() for p in self.params]
+        self._at = list(map(torch.Tensor.data_ptr, self.params))
         for i, p in enumerate(self.params):
             self._table[i] = _lib.W2VAdamwTensor(
-                p.data_ptr(), self.m[i].data_ptr(), self.v[i].data_ptr(),
+                self._at[i], self.m[i].data_ptr(), self.v[i].data_ptr(),
                 self.mscale[i].data_ptr() if self.mscale else 0, self.vscale[i].data_ptr() if self.vscale else 0,
-                p.numel(), TYPES[p.dtype])
-        self._clock = torch.zeros(4, dtype=torch.float64, device=self.device)
-        self._clock_at = self._clock.data_ptr()
-        with on_device(self.device):
-            check(_lib.load().w2v_adamw_clock(self._clock_at, o.beta1, o.beta2, t, stream_of(self.device)),
-                  "w2v_adamw_clock")
+                self._sizes[i], TYPES[p.dtype])
+
+    def _moved(self):
+        """Parameters whose memory is another now (``p.data = ...``, ``p.set_``, ``p.resize_``)."""
+        self._check_params()
+        if list(map(torch.Tensor.numel, self.params)) != self._sizes or [p.dtype for p in self.params] != self._types \
+                or any(p.device != self.device for p in self.params):
+            raise ValueError("a parameter has changed its size, type or device")
+        self._fill()
 
     def _state(self, state):
         bits = self.opts.bits
@@ -151,7 +173,7 @@ class AdamW:
                 if x.dtype != dt or x.numel() != n or x.device != self.device or not x.is_contiguous():
                     raise ValueError(f"state[{name!r}] wants contiguous {dt} tensors of {self.device}, "
                                      "as many elements as it describes")
-            return got
+            return [x.detach() for x in got]      # aliases of our own: they stay where the state is now
 
         if int(state["t"]) < 0:
             raise ValueError("state['t'] is negative")
@@ -181,6 +203,8 @@ class AdamW:
         if len(grads) != n:
             raise ValueError(f"{len(grads)} gradients for {n} parameters")
         dev = self.device
+        if list(map(torch.Tensor.data_ptr, self.params)) != self._at:
+            self._moved()
         self._like(grads, self._sizes, "a gradient has its parameter's device and size and is contiguous")
         types = [g.dtype for g in grads]
         if types == self._types:
@@ -199,7 +223,7 @@ class AdamW:
             rate = float(lrate)
         opts = _lib.W2VAdamwOpts(rate, o.beta1, o.beta2, o.eps, o.wdecay)
         with on_device(dev):
-            pointers = self._pointers(*map(torch.Tensor.data_ptr, grads))
+            pointers = self._pointers.from_buffer(array("Q", map(torch.Tensor.data_ptr, grads)))
             if o.bits == 8 and o.rounding == "random":
                 check(_lib.load().w2v_adamw_step_random(self._table, pointers, kinds, n, C.byref(opts), rate_ptr,
                                                         o.seed & (2 ** 64 - 1), self._clock_at, stream_of(dev)),

@@ -384,3 +384,48 @@ def test_random_rounding_repeats_and_is_asked_for():
     assert torch.equal(torch.cat([t2.m[0], t2.v[0]]), after(5, 4))
     with pytest.warns(UserWarning, match="rounding"):
         AdamW([p.cuda()], AdamW.Opts(bits=8))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_parameters_that_move(bits):
+    """After p.data = ... or p.set_ a step works on the new memory and leaves the old alone."""
+    from bidmach_b200 import AdamW
+    ps, gs = make([700, 300], "f32", "f32", 4)
+    gs = [g.cuda() for g in gs]
+    a, b = [p.cuda() for p in ps], [p.cuda() for p in ps]
+    o = AdamW.Opts(bits=bits, rounding="random")
+    oa, ob = AdamW(a, o), AdamW(b, o)
+    oa.step(gs)
+    ob.step(gs)
+    for change in (lambda x: setattr(x, "data", x.clone()), lambda x: x.set_(x.clone()),
+                   lambda x: setattr(x, "data", torch.cat([x.new_zeros(5), x])[5:])):
+        old = b[1].detach()
+        kept = old.clone()
+        change(b[1])
+        assert b[1].data_ptr() != old.data_ptr()
+        oa.step(gs)
+        ob.step(gs)
+        assert all(torch.equal(x, y) for x, y in zip(a, b)) and torch.equal(old, kept)
+    for bad, match in ((lambda: setattr(b[1], "data", torch.zeros(301, device="cuda")), "size"),
+                       (lambda: setattr(b[1], "data", b[0].data[:300]), "overlap"),
+                       (lambda: setattr(b[1], "data", torch.zeros(600, device="cuda")[::2]), "contiguous")):
+        good = b[1].data
+        bad()
+        with pytest.raises(ValueError, match=match):
+            ob.step(gs)
+        b[1].data = good
+    oa.step(gs)
+    ob.step(gs)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_a_state_that_is_given_other_memory():
+    """The updater goes on with the moments that it was given."""
+    from bidmach_b200 import AdamW
+    p, m, v = (torch.zeros(300, device="cuda") for _ in range(3))
+    opt = AdamW([p], state=dict(t=0, m=[m], v=[v]))
+    was = m.detach()
+    m.set_(torch.zeros(300, device="cuda"))
+    opt.step([torch.ones(300, device="cuda")])
+    assert torch.equal(opt.m[0], was) and not m.any()
+    assert abs(float(was[0]) - 0.1) <= 2.0 ** -24
