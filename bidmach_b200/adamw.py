@@ -9,6 +9,7 @@ import ctypes as C
 import dataclasses
 import warnings
 from array import array
+from bisect import bisect_right
 
 import torch
 
@@ -137,12 +138,30 @@ class AdamW:
         self._apart([*self.params, *self.m, *self.v, *(self.mscale or ()), *(self.vscale or ())],
                     "a tensor of the state overlaps another or a parameter")
         self._held = [p.detach() for p in self.params]
+        mine = [*self.params, *self.m, *self.v, *(self.mscale or ()), *(self.vscale or ())]
+        spans = sorted((x.data_ptr(), x.data_ptr() + x.numel() * x.element_size()) for x in mine if x.numel())
+        self._begins, self._ends = [a for a, _ in spans], [b for _, b in spans]
+        self._seen = set()      # addresses that have passed `_foreign`
         self._at = list(map(torch.Tensor.data_ptr, self.params))
         for i, p in enumerate(self.params):
             self._table[i] = _lib.W2VAdamwTensor(
                 self._at[i], self.m[i].data_ptr(), self.v[i].data_ptr(),
                 self.mscale[i].data_ptr() if self.mscale else 0, self.vscale[i].data_ptr() if self.vscale else 0,
                 self._sizes[i], TYPES[p.dtype])
+
+    def _foreign(self, tensors, key, what):
+        """Refuses tensors that share memory with a parameter or the state.  `key` is what the answer hangs on,
+        the tensors' addresses and types: those that have passed need no second look."""
+        if key in self._seen:
+            return
+        for x in tensors:
+            a, n = x.data_ptr(), x.numel()
+            i = bisect_right(self._begins, a)
+            if n and (i and self._ends[i - 1] > a or i < len(self._begins) and self._begins[i] < a + n * x.element_size()):
+                raise ValueError(what)
+        if len(self._seen) >= 64:
+            self._seen.clear()
+        self._seen.add(key)
 
     def _moved(self):
         """Parameters whose memory is another now (``p.data = ...``, ``p.set_``, ``p.resize_``)."""
@@ -221,9 +240,11 @@ class AdamW:
             rate_ptr = lrate.data_ptr()
         elif lrate is not None:
             rate = float(lrate)
+        at = array("Q", map(torch.Tensor.data_ptr, grads))
+        self._foreign(grads, (at.tobytes(), bytes(kinds)), "a gradient shares memory with a parameter or the state")
         opts = _lib.W2VAdamwOpts(rate, o.beta1, o.beta2, o.eps, o.wdecay)
         with on_device(dev):
-            pointers = self._pointers.from_buffer(array("Q", map(torch.Tensor.data_ptr, grads)))
+            pointers = self._pointers.from_buffer(at)
             if o.bits == 8 and o.rounding == "random":
                 check(_lib.load().w2v_adamw_step_random(self._table, pointers, kinds, n, C.byref(opts), rate_ptr,
                                                         o.seed & (2 ** 64 - 1), self._clock_at, stream_of(dev)),
@@ -235,7 +256,7 @@ class AdamW:
     def moments(self, mout=None, vout=None):
         """Both moments as fp32 values: lists (m, v).  With 32 bits these are the state itself; with 8
         the codes are decoded into new tensors or into the lists ``mout`` and ``vout``, whose tensors
-        overlap neither each other nor the state."""
+        overlap neither each other nor the state nor a parameter."""
         if self.opts.bits == 32:
             if mout is not None or vout is not None:
                 raise ValueError("32-bit moments are not copied: mout and vout are for 8 bits")
@@ -253,8 +274,13 @@ class AdamW:
         self._like(both, self._sizes * 2, what)
         if any(x.dtype is not torch.float32 for x in both):
             raise ValueError(what)
+        at = array("Q", map(torch.Tensor.data_ptr, both))
+        key = at.tobytes()
+        if key not in self._seen:
+            self._apart(both, "two tensors of mout and vout overlap")
+            self._foreign(both, key, "mout or vout shares memory with a parameter or the state")
         with on_device(dev):
-            check(_lib.load().w2v_adamw_moments(self._table, self._pointers(*map(torch.Tensor.data_ptr, mout)),
-                                                self._pointers(*map(torch.Tensor.data_ptr, vout)), n,
-                                                stream_of(dev)), "w2v_adamw_moments")
+            check(_lib.load().w2v_adamw_moments(self._table, self._pointers.from_buffer(at),
+                                                self._pointers.from_buffer(at, 8 * n), n, stream_of(dev)),
+                  "w2v_adamw_moments")
         return mout, vout

@@ -429,3 +429,43 @@ def test_a_state_that_is_given_other_memory():
     opt.step([torch.ones(300, device="cuda")])
     assert torch.equal(opt.m[0], was) and not m.any()
     assert abs(float(was[0]) - 0.1) <= 2.0 ** -24
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_gradients_in_the_state_are_refused(bits):
+    from bidmach_b200 import AdamW
+    buf = torch.zeros(2048, device="cuda")
+    p, g = buf[:512], buf[512:1024]
+    opt = AdamW([p], AdamW.Opts(bits=bits, rounding="random"))
+    state = opt.m[0] if bits == 32 else opt.mscale[0]
+    opt.step([g])
+    before = [x.clone() for x in (p, opt.m[0], opt.v[0])]
+    for bad in ([p], [buf[256:768]], [opt.m[0]] if bits == 32 else [opt.m[0].view(torch.float32)]):
+        if bad[0].numel() == 512:
+            with pytest.raises(ValueError, match="shares memory"):
+                opt.step(bad)
+    assert all(torch.equal(x, y) for x, y in zip(before, (p, opt.m[0], opt.v[0])))
+    # one tensor for several parameters is fine, next to the parameters too
+    two = AdamW([buf[:512], buf[1024:1536]], AdamW.Opts(bits=bits, rounding="random"))
+    two.step([g, g])
+    two.step([g, g])
+    with pytest.raises(ValueError, match="shares memory"):
+        two.step([g, buf[1000:1512]])
+    assert state.is_cuda
+
+
+def test_moments_into_shared_memory_are_refused():
+    from bidmach_b200 import AdamW
+    ps = [torch.zeros(n, device="cuda") for n in (600, 256)]
+    opt = AdamW(ps, AdamW.Opts(bits=8, rounding="random"))
+    opt.step([torch.randn(n, device="cuda") for n in (600, 256)])
+    want = opt.moments()
+    x, y, z = (torch.zeros(n, device="cuda") for n in (600, 256, 1000))
+    for m, v in (([x, y], [x, y]), ([x, z[:256]], [z[200:800], y]), ([ps[0], y], [x, z[:256]]),
+                 ([x, y], [z[:600], ps[1]]), ([x, z[:256]], [z[400:], z[100:356]])):
+        with pytest.raises(ValueError, match="overlap|shares memory"):
+            opt.moments(m, v)
+    got = opt.moments([x, y], [z[:600], z[600:856]])
+    for _ in range(2):
+        assert all(torch.equal(a, b) for g, w in zip(got, want) for a, b in zip(g, w))
+        got = opt.moments([x, y], [z[:600], z[600:856]])
