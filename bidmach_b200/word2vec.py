@@ -18,9 +18,9 @@ import numpy as np
 import torch
 
 from . import _lib, modelio
-from .adamw import AdamW
+from .adamw import AdamW, stream_of
 from .cumach import CUMACH, CUMACHSlice, cuda_error_string
-from .embed import EmbedRows
+from .embed import EmbedRows, check_ids
 from .softmax import Softmax
 
 
@@ -267,6 +267,12 @@ class Word2Vec:
         """The positive pairs of a minibatch grouped by context word: ``(ids, targets)``, int32 ``[rows]``
         and ``[rows, 2 * nskip]``; row by row, in the order of the text, a word and the centre words that
         have it in their window, -1 behind the last.  Positions without a pair have no row."""
+        for x, name in ((words, "words"), (lbound, "lbound"), (ubound, "ubound")):
+            check_ids(x, name, 1)
+            if x.numel() != words.numel() or x.device != words.device:
+                raise ValueError(f"{name} has {x.numel()} elements on {x.device}, words {words.numel()} on {words.device}")
+        if not 1 <= self.opts.nskip <= 512:
+            raise ValueError("need 1 <= nskip <= 512")
         n, width = words.numel(), 2 * self.opts.nskip
         ids = torch.empty(n, dtype=torch.int32, device=words.device)
         targets = torch.empty(n, width, dtype=torch.int32, device=words.device)
@@ -276,7 +282,7 @@ class Word2Vec:
         with torch.cuda.device(words.device):
             _check(lib.w2v_window_rows(words.data_ptr(), lbound.data_ptr(), ubound.data_ptr(), n, self.opts.nskip,
                                        ids.data_ptr(), targets.data_ptr(), work[size // 4:].data_ptr(),
-                                       work.data_ptr(), size, self._stream()), "w2v_window_rows")
+                                       work.data_ptr(), size, stream_of(words.device)), "w2v_window_rows")
         rows = int(work[size // 4].item())
         return ids[:rows], targets[:rows]
 

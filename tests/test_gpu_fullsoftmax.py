@@ -157,3 +157,15 @@ def test_refused_with_slices():
     from bidmach_b200.word2vec import Opts
     with pytest.raises(ValueError, match="nSlices"):
         Word2Vec(Opts(fullSoftmax=True, nSlices=2))
+
+
+def test_window_rows_refuses():
+    from bidmach_b200 import Word2Vec
+    from bidmach_b200.word2vec import Opts
+    m = Word2Vec(Opts(vocabSize=50, dim=4))
+    w = torch.zeros(10, dtype=torch.int32, device="cuda")
+    for args in ((w, w[:9], w), (w, w, w[:9]), (w, w, w.cpu()), (w[::2], w[:5], w[:5]), (w, w.float(), w)):
+        with pytest.raises(ValueError):
+            m.windowRows(*args)
+    with pytest.raises(ValueError, match="nskip"):
+        Word2Vec(Opts(vocabSize=50, dim=4, nskip=513)).windowRows(w, w, w)

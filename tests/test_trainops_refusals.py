@@ -137,3 +137,13 @@ def test_softmax_says_when_a_kernel_gave_up(monkeypatch):
     Softmax.check()      # said once
     fake.w2v_softmax_fault = lambda: None      # no pinned memory
     Softmax.check()
+
+
+def test_window_rows_wants_equal_int32_vectors_of_the_device():
+    from bidmach_b200 import Word2Vec
+    from bidmach_b200.word2vec import Opts
+    m = Word2Vec(Opts(vocabSize=50, dim=4))
+    w = torch.zeros(10, dtype=torch.int32)
+    for bad, match in ((w.long(), "int32"), (w.view(2, 5), "dimension"), (w, "CUDA"), ([0] * 10, "int32")):
+        with pytest.raises(ValueError, match=match):
+            m.windowRows(bad, w, w)
