@@ -113,8 +113,7 @@ class Word2Vec:
                                       "CPU kernels; this build has no CPU path")
         if self.opts.nSlices < 1 or not 0 <= self.opts.iSlice < self.opts.nSlices or self.opts.nHeadTerms < 0:
             raise ValueError("need nSlices >= 1, 0 <= iSlice < nSlices, nHeadTerms >= 0")
-        if self.opts.fullSoftmax and self.opts.nSlices > 1:
-            raise ValueError("fullSoftmax needs the whole vocabulary: nSlices must be 1")
+        self._check_full()
         self.device = torch.device(device if device is not None else "cuda")
         self.modelmats: list[torch.Tensor] = []
         self.ncols = 0
@@ -130,6 +129,18 @@ class Word2Vec:
         self._adam_steps = 0
         self._firstPos = None
 
+    def _check_full(self):
+        """What the operators behind fullSoftmax take."""
+        o = self.opts
+        if not o.fullSoftmax:
+            return
+        if o.nSlices > 1:
+            raise ValueError("fullSoftmax needs the whole vocabulary: nSlices must be 1")
+        if not 1 <= o.dim <= 4096 or not 1 <= o.nskip <= 512:
+            raise ValueError("fullSoftmax needs dim up to 4096 and nskip up to 512")
+        if o.momentBits not in (8, 32) or not (0 <= o.beta1 < 1 and 0 <= o.beta2 < 1 and o.adamEps > 0 and o.wdecay >= 0):
+            raise ValueError("need momentBits 8 or 32, 0 <= beta1, beta2 < 1, adamEps > 0, wdecay >= 0")
+
     def sliceRows(self) -> int:
         """Rows of each matrix: nHeadTerms + 1 + (vocabSize - nHeadTerms - 1) / nSlices
         (Word2Vec.scala:106), the whole vocabulary for one slice."""
@@ -140,6 +151,7 @@ class Word2Vec:
     def init(self, ncols: int, refresh: bool = True):
         """Word2Vec.init (Word2Vec.scala:100-165): allocate both matrices and the
         per-minibatch work buffers for minibatches of ``ncols`` tokens."""
+        self._check_full()
         o = self.opts
         lib = _lib.load()
         self.ncols = int(ncols)

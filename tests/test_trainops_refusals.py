@@ -147,3 +147,17 @@ def test_window_rows_wants_equal_int32_vectors_of_the_device():
     for bad, match in ((w.long(), "int32"), (w.view(2, 5), "dimension"), (w, "CUDA"), ([0] * 10, "int32")):
         with pytest.raises(ValueError, match=match):
             m.windowRows(bad, w, w)
+
+
+def test_fullsoftmax_options_are_checked_when_the_model_is_made():
+    from bidmach_b200 import Word2Vec
+    from bidmach_b200.word2vec import Opts
+    for bad in (dict(dim=4097), dict(nskip=513), dict(nskip=0), dict(momentBits=16), dict(beta1=1.0), dict(beta2=-0.1),
+                dict(adamEps=0.0), dict(wdecay=-1.0), dict(nSlices=2)):
+        with pytest.raises(ValueError):
+            Word2Vec(Opts(fullSoftmax=True, **bad))
+    o = Opts(fullSoftmax=True)
+    m = Word2Vec(o)
+    o.momentBits = 4
+    with pytest.raises(ValueError, match="momentBits"):
+        m.init(16)
