@@ -75,8 +75,8 @@ class EmbedRows:
         check_ids(ids, "ids", 1)
         ldm = check_matrix(matrix, "matrix", ids.device)
         n, (vocab, dim) = ids.numel(), matrix.shape
-        if vocab < 1:
-            raise ValueError("matrix has no rows")
+        if not 1 <= vocab < 2 ** 31 - 1 or n >= 2 ** 30 or dim > 65536:
+            raise ValueError("need 1 to 2^31 - 2 rows of matrix, fewer than 2^30 ids, at most 65536 columns")
         if out is None:
             out, ldo = torch.empty(n, dim, dtype=matrix.dtype, device=ids.device), dim
         else:

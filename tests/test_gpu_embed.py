@@ -130,3 +130,14 @@ def test_outputs_that_share_memory_are_refused():
         EmbedRows.forward(ids, m, out=m)
     with pytest.raises(ValueError, match="overlaps"):
         EmbedRows.backward(ids, m, 9, out=m)
+
+
+def test_more_columns_than_the_kernels_take_are_refused():
+    from bidmach_b200 import EmbedRows
+    ids = torch.zeros(3, dtype=torch.int32, device="cuda")
+    wide = torch.zeros(3, 65537, device="cuda")
+    with pytest.raises(ValueError, match="columns"):
+        EmbedRows.forward(ids, wide)
+    with pytest.raises(ValueError, match="columns"):
+        EmbedRows.backward(ids, wide, 5)
+    assert EmbedRows.forward(ids, wide[:, :65536].contiguous()).shape == (3, 65536)
