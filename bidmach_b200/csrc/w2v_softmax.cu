@@ -1595,7 +1595,12 @@ void column_tiles(int dim, int *nt, int *ntile, int *nlast) {
   *ntile = *nt > 1 ? kN : *nlast;
 }
 
-Layout plan(const Shape &x, bool grad) {
+bool direct(int type, const void *p, int64_t ld) {   // TMA can read the caller's matrix
+  return type != W2V_F32 && aligned(p, 16) && ld % 8 == 0;
+}
+
+// `direct_h`, `direct_w`: operands that TMA reads where they lie, so that no copy of them is made.
+Layout plan(const Shape &x, bool grad, bool direct_h, bool direct_w) {
   Layout l{};
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
@@ -1617,8 +1622,8 @@ Layout plan(const Shape &x, bool grad) {
   }
   l.width = (int)up(x.dim, 64);
   l.nparts = x.type == W2V_F32 ? 3 : 1;
-  l.hs = take(x.n * l.width * l.nparts * 2);
-  l.ws = take(x.vocab * l.width * l.nparts * 2);
+  l.hs = take(direct_h ? 0 : x.n * l.width * l.nparts * 2);
+  l.ws = take(direct_w ? 0 : x.vocab * l.width * l.nparts * 2);
   if (!grad) {
     l.parts = take(2 * ((x.vocab + kN - 1) / kN) * std::min(x.n, kLossRows) * sizeof(Part));
   } else {
@@ -1639,11 +1644,6 @@ Layout plan(const Shape &x, bool grad) {
   return l;
 }
 
-template <typename T>
-bool direct(const void *p, int64_t ld) {   // TMA can read the caller's matrix
-  return sizeof(T) == 2 && aligned(p, 16) && ld * sizeof(T) % 16 == 0;
-}
-
 // Operands for the products: the caller's own where TMA can read them, else staged ones.
 template <typename T>
 int stage(const Shape &x, const Layout &l, const void *h, int64_t ldh, const void *w, int64_t ldw, const float *gloss,
@@ -1660,8 +1660,8 @@ int stage(const Shape &x, const Layout &l, const void *h, int64_t ldh, const voi
                                    split ? sw : Source{nullptr, 0, 0}, x.dim, gloss, targets, x.labels, x.vocab, sc);
     if (err) return err;
   }
-  uint16_t *hs = direct<T>(h, ldh) ? nullptr : reinterpret_cast<uint16_t *>(ws + l.hs);
-  uint16_t *wst = direct<T>(w, ldw) ? nullptr : reinterpret_cast<uint16_t *>(ws + l.ws);
+  uint16_t *hs = direct(x.type, h, ldh) ? nullptr : reinterpret_cast<uint16_t *>(ws + l.hs);
+  uint16_t *wst = direct(x.type, w, ldw) ? nullptr : reinterpret_cast<uint16_t *>(ws + l.ws);
   const int64_t staged = (int64_t)l.width * l.nparts;
   if (hs || wst) {
     const int err = launch_chained(stage_kernel<T>, dim3(blocks, 1, 2), 256, 0, s, sh, sw, x.dim, hs, wst, l.width, staged, parts, sc);
@@ -1883,9 +1883,10 @@ int run_grad(const Shape &x, const Layout &l, const void *h, int64_t ldh, const 
 
 extern "C" int *w2v_softmax_fault(void) { return fault_flag(); }
 
-extern "C" int64_t w2v_softmax_workspace(int64_t n, int64_t vocab, int dim, int labels, int type, int grad) {
+extern "C" int64_t w2v_softmax_workspace(int64_t n, int64_t vocab, int dim, int labels, int type, int flags) {
   const Shape x{n, vocab, dim, labels, type};
-  return good_shape(x) ? plan(x, grad != 0).total : -1;
+  const bool h = flags & W2V_HIDDEN_IN_PLACE, w = flags & W2V_WEIGHT_IN_PLACE;
+  return good_shape(x) ? plan(x, flags & W2V_SOFTMAX_GRAD, type != W2V_F32 && h, type != W2V_F32 && w).total : -1;
 }
 
 extern "C" int w2v_softmax_loss(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, const int *targets,
@@ -1895,7 +1896,7 @@ extern "C" int w2v_softmax_loss(const void *hidden, int64_t ldh, const void *wei
   if (!good_shape(x) || ldh < dim || ldw < dim || !weight || !workspace || !aligned(workspace, 256)) return 1;
   if (n == 0) return 0;
   if (!hidden || !targets || !loss || !lse) return 1;
-  const Layout l = plan(x, false);
+  const Layout l = plan(x, false, direct(type, hidden, ldh), direct(type, weight, ldw));
   if (workspace_bytes < l.total) return 1;
   if (const int fault = take_fault()) return fault;
   char *ws = static_cast<char *>(workspace);
@@ -1914,7 +1915,7 @@ extern "C" int w2v_softmax_grad(const void *hidden, int64_t ldh, const void *wei
       !aligned(workspace, 256) || (ldg != 0 && ldg != 1))
     return 1;
   if (n > 0 && (!hidden || !targets || !lse || !gloss || !dhidden)) return 1;
-  const Layout l = plan(x, true);
+  const Layout l = plan(x, true, direct(type, hidden, ldh), direct(type, weight, ldw));
   if (workspace_bytes < l.total) return 1;
   if (const int fault = take_fault()) return fault;
   char *ws = static_cast<char *>(workspace);

@@ -8,6 +8,7 @@ from .adamw import TYPES, check, on_device, stream_of
 from .embed import check_apart, check_ids, check_matrix
 
 CUDA_ERROR_LAUNCH_TIMEOUT = 702
+GRAD, HIDDEN_IN_PLACE, WEIGHT_IN_PLACE = 1, 2, 4      # flags of w2v_softmax_workspace
 
 
 def _vector(x, name: str, n: int, device):
@@ -51,11 +52,16 @@ class Softmax:
         return ldh, ldw, n, weight.shape[0], dim, labels
 
     @staticmethod
-    def _workspace(n, vocab, dim, labels, kind, grad, device):
-        size = _lib.load().w2v_softmax_workspace(n, vocab, dim, labels, kind, int(grad))
+    def _workspace(hidden, ldh, weight, ldw, labels, grad):
+        flags = GRAD if grad else 0
+        if hidden.element_size() == 2:     # matrices that are read where they lie need no room for a copy
+            flags |= HIDDEN_IN_PLACE if hidden.data_ptr() % 16 == 0 and ldh % 8 == 0 else 0
+            flags |= WEIGHT_IN_PLACE if weight.data_ptr() % 16 == 0 and ldw % 8 == 0 else 0
+        (n, dim), vocab = hidden.shape, weight.shape[0]
+        size = _lib.load().w2v_softmax_workspace(n, vocab, dim, labels, TYPES[hidden.dtype], flags)
         if size < 0:
             raise ValueError("w2v_softmax_workspace refused the sizes")
-        return torch.empty(size, dtype=torch.uint8, device=device), size
+        return torch.empty(size, dtype=torch.uint8, device=hidden.device), size
 
     @staticmethod
     def check():
@@ -83,7 +89,7 @@ class Softmax:
             _vector(lse, "lse", n, dev)
             check_apart("lse", lse, hidden=hidden, weight=weight, targets=targets, loss=loss)
         with on_device(dev):
-            work, size = Softmax._workspace(n, vocab, dim, labels, kind, False, dev)
+            work, size = Softmax._workspace(hidden, ldh, weight, ldw, labels, False)
             check(_lib.load().w2v_softmax_loss(hidden.data_ptr(), ldh, weight.data_ptr(), ldw, targets.data_ptr(), n,
                                                vocab, dim, labels, kind, loss.data_ptr(), lse.data_ptr(),
                                                work.data_ptr(), size, stream_of(dev)), "w2v_softmax_loss")
@@ -121,7 +127,7 @@ class Softmax:
         if given[1]:
             check_apart("dweight", dweight, **inputs, dhidden=dhidden)
         with on_device(dev):
-            work, size = Softmax._workspace(n, vocab, dim, labels, kind, True, dev)
+            work, size = Softmax._workspace(hidden, ldh, weight, ldw, labels, True)
             check(_lib.load().w2v_softmax_grad(hidden.data_ptr(), ldh, weight.data_ptr(), ldw, targets.data_ptr(), n,
                                                vocab, dim, labels, kind, lse.data_ptr(), gloss.data_ptr(),
                                                0 if one else 1, dhidden.data_ptr(), lddh, dweight.data_ptr(), lddw,

@@ -464,7 +464,11 @@ int w2v_window_rows(const int *words, const int *lb, const int *ub, int n, int n
  * labels <= 1024.  fp32 operands are multiplied to 22 bits, counted from the largest number of each one's
  * row (rows down to 2^-60 of the largest one).  A row of hidden with an infinity or a NaN gives a NaN in its own lse (and in dweight),
  * a row of weight in all of them. */
-int64_t w2v_softmax_workspace(int64_t n, int64_t vocab, int dim, int labels, int type, int grad);   /* -1: refused */
+/* Size of the scratch memory, -1 for sizes that are refused.  flags: GRAD for w2v_softmax_grad, 0 for
+ * w2v_softmax_loss; a 16-bit matrix whose address is a multiple of 16 bytes and whose ld is one of 8 is read where it
+ * lies, and its flag leaves out the room for a copy. */
+enum { W2V_SOFTMAX_GRAD = 1, W2V_HIDDEN_IN_PLACE = 2, W2V_WEIGHT_IN_PLACE = 4 };
+int64_t w2v_softmax_workspace(int64_t n, int64_t vocab, int dim, int labels, int type, int flags);
 int w2v_softmax_loss(const void *hidden, int64_t ldh, const void *weight, int64_t ldw,
                      const int *targets, int64_t n, int64_t vocab, int dim, int labels, int type,
                      float *loss, float *lse, void *workspace, int64_t workspace_bytes, void *stream);

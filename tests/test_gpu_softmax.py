@@ -384,3 +384,18 @@ def test_the_next_call_says_that_a_kernel_gave_up():
         assert count() == before and flag[0] == 0
         call()
     assert torch.equal(Softmax.loss(hidden, weight, targets)[0], loss)
+
+
+@pytest.mark.parametrize("t", ["bf16", "f16"])
+def test_no_room_for_copies_that_are_not_made(t):
+    """A 200 MB matrix that TMA reads where it lies: the loss allocates its 13 MB of row parts."""
+    from bidmach_b200 import Softmax
+    hidden = torch.randn(1024, 512, device="cuda").to(TYPES[t])
+    weight = torch.zeros(200000, 512, dtype=TYPES[t], device="cuda")
+    targets = torch.zeros(1024, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    _, lse = Softmax.loss(hidden, weight, targets)
+    assert torch.cuda.max_memory_allocated() - before < 20 << 20
+    assert (lse - 12.206072645530174).abs().max() < 1e-5      # log 200000

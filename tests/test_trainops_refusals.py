@@ -161,3 +161,17 @@ def test_fullsoftmax_options_are_checked_when_the_model_is_made():
     o.momentBits = 4
     with pytest.raises(ValueError, match="momentBits"):
         m.init(16)
+
+
+@pytest.mark.parametrize("n,vocab,dim", [(5, 300, 40), (300, 1000, 64), (9000, 50000, 301)])
+@pytest.mark.parametrize("grad", [0, 1])
+def test_softmax_workspace_without_copies(n, vocab, dim, grad):
+    """A 16-bit matrix that is read where it lies takes no room; fp32 ones are always split."""
+    size = _lib.load().w2v_softmax_workspace
+    width = (dim + 63) // 64 * 64
+    for kind in (1, 2):
+        full = size(n, vocab, dim, 1, kind, grad)
+        for flag, rows in ((2, n), (4, vocab)):
+            copy = (rows * width * 2 + 1023) // 1024 * 1024
+            assert full - size(n, vocab, dim, 1, kind, grad | flag) == copy - 1024
+    assert size(n, vocab, dim, 1, 0, grad | 6) == size(n, vocab, dim, 1, 0, grad)
