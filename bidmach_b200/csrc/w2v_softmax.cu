@@ -31,8 +31,12 @@
 // For few rows the bound is reading W once: a kernel with eight rows in shared memory, W straight from
 // memory in its own type, plain fp32 arithmetic.  fp32 goes that way up to 16 rows, in two passes: the
 // tensor cores would need W in two parts, three more passes over it (100000 x 256, loss / gradients: 8 rows
-// 30 / 78 us, 16 rows 60 / 156, against 107 / 223 for 9 or more).  16-bit types need no such parts, so
-// four rows are the border (4 rows 24 / 97 us, 8 rows 30 / 110, against 27 / 86).
+// 30 / 78 us, 16 rows 60 / 156, against 107 / 223 for 9 or more).  16-bit types go that way up to four
+// rows.  The loss does so where W would have to be copied (100000 x 300, 4 rows: 44 us against 66) or has at most
+// 256 columns, a step of the kernel's (128: 27 against 26, 256: 24 against 28, 384: 54 against 31, 1024: 138
+// against 82).  The gradients always do: here d stays in fp32 and is not rounded to 16 bits, for a
+// tenth more time, a quarter at most (100000 x 256, 4 rows: 98 us against 88, x 768 231 against 187; x 300, where
+// W would be copied, 163 against 180).
 #include <cuda.h>
 #include <math.h>
 
@@ -52,7 +56,8 @@ namespace {
 using namespace w2v;
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kFewRows = 8;   // of a pass
+constexpr int kFewRows = 8;   // of a pass, fp32
+constexpr int kFewRows16 = 4;
 constexpr int kMaxDim = 4096;
 
 // A row's sum of exponentials as 2^m * s, with exponents in units of log2 e.
@@ -1577,13 +1582,17 @@ int few_dh_blocks(int64_t vocab) {
   return (int)std::min<int64_t>((vocab + 31) / 32, (int64_t)device_sm_count());
 }
 int few_rows_of(int64_t n) { return n <= 1 ? 1 : n <= 2 ? 2 : n <= 4 ? 4 : 8; }
-bool few_rows(const Shape &x) { return x.n <= (x.type == W2V_F32 ? 2 * kFewRows : 4); }
+bool few_rows(const Shape &x, bool grad, bool direct_w) {
+  if (x.type == W2V_F32) return x.n <= 2 * kFewRows;
+  return x.n <= kFewRows16 && (grad || !direct_w || x.dim <= 256);
+}
 
 struct Layout {
   int64_t scalars, hs, ws, parts, probs, pieces, acc_h, acc_w, total;
   int width, nparts;         // staged operands
   int64_t rows, words;       // of a piece of d
   int nt, ntile, nlast;
+  bool few;
 };
 
 // Column tiles of a gradient: as wide as they can be, the rest in a last one.  A block of K of any width up
@@ -1609,7 +1618,8 @@ Layout plan(const Shape &x, bool grad, bool direct_h, bool direct_w) {
     return here;
   };
   l.scalars = take(sizeof(Scalars));
-  if (few_rows(x)) {
+  l.few = few_rows(x, grad, direct_w);
+  if (l.few) {
     const int rb = few_rows_of(x.n);
     if (!grad) {
       l.parts = take((int64_t)few_blocks(x.vocab) * rb * sizeof(Part));
@@ -1712,7 +1722,7 @@ int run_loss(const Shape &x, const Layout &l, const void *h, int64_t ldh, const 
                           rows, static_cast<const T *>(h) + r0 * ldh, ldh, static_cast<const T *>(w), ldw, x.vocab, x.dim,
                           wide, targets + r0 * x.labels, x.labels, loss + r0, lse + r0);
   };
-  if (few_rows(x)) {
+  if (l.few) {
     int err = 0;
     for (int64_t r0 = 0; r0 < x.n && !err; r0 += kFewRows) {
       const int rows = (int)std::min<int64_t>(kFewRows, x.n - r0);
@@ -1722,7 +1732,8 @@ int run_loss(const Shape &x, const Layout &l, const void *h, int64_t ldh, const 
         case 1: err = few_loss<T, 1>(x, l, hr, ldh, rows, w, ldw, ws, &count, s); break;
         case 2: err = few_loss<T, 2>(x, l, hr, ldh, rows, w, ldw, ws, &count, s); break;
         case 4: err = few_loss<T, 4>(x, l, hr, ldh, rows, w, ldw, ws, &count, s); break;
-        default: err = few_loss<T, 8>(x, l, hr, ldh, rows, w, ldw, ws, &count, s);
+        default:
+          if constexpr (sizeof(T) == 4) err = few_loss<T, 8>(x, l, hr, ldh, rows, w, ldw, ws, &count, s);
       }
       if (!err) err = join_rows(count, rows, r0, rows);
     }
@@ -1777,7 +1788,7 @@ int run_grad(const Shape &x, const Layout &l, const void *h, int64_t ldh, const 
              const float *lse, const float *gloss, int64_t ldg, void *dh, int64_t lddh, void *dw, int64_t lddw, char *ws,
              cudaStream_t s) {
   if (x.n == 0) return (int)cudaMemset2DAsync(dw, lddw * sizeof(T), 0, x.dim * sizeof(T), x.vocab, s);
-  if (few_rows(x)) {
+  if (l.few) {
     int err = 0;
     for (int64_t r0 = 0; r0 < x.n && !err; r0 += kFewRows) {
       const int rows = (int)std::min<int64_t>(kFewRows, x.n - r0);
@@ -1789,7 +1800,8 @@ int run_grad(const Shape &x, const Layout &l, const void *h, int64_t ldh, const 
         case 1: err = go(std::integral_constant<int, 1>()); break;
         case 2: err = go(std::integral_constant<int, 2>()); break;
         case 4: err = go(std::integral_constant<int, 4>()); break;
-        default: err = go(std::integral_constant<int, 8>());
+        default:
+          if constexpr (sizeof(T) == 4) err = go(std::integral_constant<int, 8>());
       }
     }
     return err;
@@ -1886,7 +1898,10 @@ extern "C" int *w2v_softmax_fault(void) { return fault_flag(); }
 extern "C" int64_t w2v_softmax_workspace(int64_t n, int64_t vocab, int dim, int labels, int type, int flags) {
   const Shape x{n, vocab, dim, labels, type};
   const bool h = flags & W2V_HIDDEN_IN_PLACE, w = flags & W2V_WEIGHT_IN_PLACE;
-  return good_shape(x) ? plan(x, flags & W2V_SOFTMAX_GRAD, type != W2V_F32 && h, type != W2V_F32 && w).total : -1;
+  const bool grad = flags & W2V_SOFTMAX_GRAD, half = type != W2V_F32;
+  if (!good_shape(x)) return -1;
+  // without its flag, W may be read in place all the same, and another path taken for it
+  return std::max(plan(x, grad, half && h, half && w).total, plan(x, grad, half && h, half).total);
 }
 
 extern "C" int w2v_softmax_loss(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, const int *targets,

@@ -399,3 +399,31 @@ def test_no_room_for_copies_that_are_not_made(t):
     _, lse = Softmax.loss(hidden, weight, targets)
     assert torch.cuda.max_memory_allocated() - before < 20 << 20
     assert (lse - 12.206072645530174).abs().max() < 1e-5      # log 200000
+
+
+@pytest.mark.parametrize("n", [1, 2, 3, 4, 5])
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("dim", [255, 256, 257, 264, 272])
+def test_both_sides_of_the_few_rows_border(n, dim, t):
+    """Few rows go one way or another by type, width and alignment; a workspace of the size that is asked for
+    without flags is enough for each."""
+    from bidmach_b200 import _lib
+    x = inputs(n, 900, dim, 2, t)
+    hold(run(*x), *x, t)
+    h, w, y, g = (v.cuda() for v in x)
+    lib, kind = _lib.load(), list(TYPES).index(t)
+    loss, lse = torch.empty(n, device="cuda"), torch.empty(n, device="cuda")
+    dh, dw = torch.empty_like(h), torch.empty_like(w)
+    ok = (h.data_ptr(), dim, w.data_ptr(), dim, y.data_ptr(), n, 900, dim, 2, kind)
+    for grad in (0, 1):
+        size = lib.w2v_softmax_workspace(n, 900, dim, 2, kind, grad)
+        work = torch.empty(size, dtype=torch.uint8, device="cuda")
+        stream = torch.cuda.current_stream().cuda_stream
+        if grad:
+            err = lib.w2v_softmax_grad(*ok, lse.data_ptr(), g.data_ptr(), 1, dh.data_ptr(), dim, dw.data_ptr(), dim,
+                                       work.data_ptr(), size, stream)
+        else:
+            err = lib.w2v_softmax_loss(*ok, loss.data_ptr(), lse.data_ptr(), work.data_ptr(), size, stream)
+        assert err == 0
+        torch.cuda.synchronize()
+    hold((loss, lse, dh, dw), *x, t)
