@@ -476,7 +476,9 @@ int w2v_softmax_loss(const void *hidden, int64_t ldh, const void *weight, int64_
  * that w2v_softmax_loss gave: with k_i targets in row i
  *   d[i][v] = gloss_i (k_i exp(l[i][v] - lse[i]) - targets of row i that are v)
  *   dhidden = d weight,  dweight = d^T hidden
- * both written whole, of `type`.  Equal calls give equal bits. */
+ * both written whole, of `type`.  Equal calls give equal bits.  With 16-bit operands and more than four rows d
+ * is rounded to their type; in fp16, with ldg 1, in steps of 2^-38 of the largest |gloss_i k_i| of the call, so a row
+ * whose factor is below 1e-6 of that keeps little of its probabilities in dhidden. */
 int w2v_softmax_grad(const void *hidden, int64_t ldh, const void *weight, int64_t ldw,
                      const int *targets, int64_t n, int64_t vocab, int dim, int labels, int type,
                      const float *lse, const float *gloss, int64_t ldg, void *dhidden, int64_t lddh,
