@@ -261,6 +261,8 @@ class AdamW:
             if mout is not None or vout is not None:
                 raise ValueError("32-bit moments are not copied: mout and vout are for 8 bits")
             return self.m, self.v
+        if list(map(torch.Tensor.data_ptr, self.params)) != self._at:
+            self._moved()
         n = len(self._sizes)
         if mout is None:
             mout = [torch.empty(k, dtype=torch.float32, device=self.device) for k in self._sizes]

@@ -469,3 +469,13 @@ def test_moments_into_shared_memory_are_refused():
     for _ in range(2):
         assert all(torch.equal(a, b) for g, w in zip(got, want) for a, b in zip(g, w))
         got = opt.moments([x, y], [z[:600], z[600:856]])
+
+
+def test_moments_over_a_parameter_that_moved_are_refused():
+    from bidmach_b200 import AdamW
+    p, out = torch.zeros(256, device="cuda"), torch.zeros(256, device="cuda")
+    opt = AdamW([p], AdamW.Opts(bits=8, rounding="random"))
+    opt.moments([out], [torch.zeros(256, device="cuda")])
+    p.data = out
+    with pytest.raises(ValueError, match="shares memory"):
+        opt.moments([out], [torch.zeros(256, device="cuda")])
