@@ -427,3 +427,28 @@ def test_both_sides_of_the_few_rows_border(n, dim, t):
         assert err == 0
         torch.cuda.synchronize()
     hold((loss, lse, dh, dw), *x, t)
+
+
+def test_the_first_call_of_a_process_is_captured():
+    """What a process sets up once is allowed in a capture too."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    code = """
+import torch
+from bidmach_b200 import Softmax
+h, w = torch.randn(40, 64, device="cuda"), torch.randn(300, 64, device="cuda")
+y, one = torch.zeros(40, dtype=torch.int32, device="cuda"), torch.ones((), device="cuda")
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    loss, lse = Softmax.loss(h, w, y)
+    dh, dw = Softmax.grad(h, w, y, lse, one)
+graph.replay()
+torch.cuda.synchronize()
+again = Softmax.loss(h, w, y)
+assert torch.equal(loss, again[0]) and all(torch.equal(a, b) for a, b in zip((dh, dw), Softmax.grad(h, w, y, lse, one)))
+print("captured")
+"""
+    done = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "captured" in done.stdout, done.stderr[-2000:]
