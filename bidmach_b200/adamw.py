@@ -57,7 +57,8 @@ class Opts:
     are right in the mean (random bits from ``seed``, the step and the element: equal runs give equal
     bits).  ``"nearest"`` is for a few steps, or for comparing with one: the codes of sqrt(v) are 3 to 6 %
     apart and a step with ``beta2`` 0.999 lowers it by 0.05 %, so a moment rounded to nearest never falls and
-    hardly rises.  None is ``"nearest"`` with a warning."""
+    hardly rises.  None is ``"nearest"`` with a warning.  Either way 8 bits span 16 octaves: beside the largest of its
+    256 elements, an ``m`` below 2^-16 is held as zero and a sqrt(v) as the smallest code."""
     lrate: float = 1e-3
     beta1: float = 0.9
     beta2: float = 0.999

@@ -136,6 +136,8 @@ __device__ __forceinline__ void tmem_load16(uint32_t addr, float (&x)[16]) {
 }
 __device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
+// 2^-22 relative, zero below 2^-126: no more than the logit's own rounding makes of its exponential (a logit of 16
+// is rounded by 2^-20), and one instruction where a tile has 65536 of them.
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -1,8 +1,9 @@
 // The rows of a minibatch for the softmax over the whole vocabulary: for each position whose word is
 // somebody's context, the word, and the centre words that have it in their window.  These are the pairs
-// of the positive update (Word2Vec.scala:283-302, 309-330), grouped by context: the logits of a
-// context word are then computed once for all of its up to 2 * nskip centres.  Positions without a
-// pair are left out (subsampling drops about half of a text), in the order of the text.
+// of the positive update (Word2Vec.scala:283-302, 309-330), grouped by the context's position: its
+// logits are then computed once for all of its up to 2 * nskip centres (a word that stands at several positions has a
+// row for each).  Positions without a pair are left out (subsampling drops about half of a text), in the
+// order of the text.
 //
 // Three passes over 12 bytes a position: count rows in blocks of 256, add the counts up, write.
 #include "../../include/bidmach_b200.h"
