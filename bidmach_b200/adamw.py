@@ -136,11 +136,9 @@ class AdamW:
     def _fill(self):
         """The table of addresses.  Aliases of the parameters are kept beside it, so that the memory it names
         stays theirs until it is filled again."""
-        self._apart([*self.params, *self.m, *self.v, *(self.mscale or ()), *(self.vscale or ())],
-                    "a tensor of the state overlaps another or a parameter")
+        spans = self._apart([*self.params, *self.m, *self.v, *(self.mscale or ()), *(self.vscale or ())],
+                            "a tensor of the state overlaps another or a parameter")
         self._held = [p.detach() for p in self.params]
-        mine = [*self.params, *self.m, *self.v, *(self.mscale or ()), *(self.vscale or ())]
-        spans = sorted((x.data_ptr(), x.data_ptr() + x.numel() * x.element_size()) for x in mine if x.numel())
         self._begins, self._ends = [a for a, _ in spans], [b for _, b in spans]
         self._seen = set()      # addresses that have passed `_foreign`
         self._at = list(map(torch.Tensor.data_ptr, self.params))
@@ -203,9 +201,11 @@ class AdamW:
 
     @staticmethod
     def _apart(tensors, what):
-        spans = sorted((x.data_ptr(), x.data_ptr() + x.numel() * x.element_size()) for x in tensors if x.numel())
+        """Refuses tensors that share memory; returns the begin and end of each, in order."""
+        spans = sorted((at, at + n * x.element_size()) for x in tensors if (n := x.numel()) for at in (x.data_ptr(),))
         if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
             raise ValueError(what)
+        return spans
 
     def _like(self, tensors, sizes, what):
         """Refuses tensors that are not contiguous ones of this device and these sizes (in few passes:

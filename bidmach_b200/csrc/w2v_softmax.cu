@@ -17,7 +17,7 @@
 //   grad_kernel              dH and dW from that piece, added up in fp32 over the pieces (row blocks).
 // The products are bound by the issue of the matrix instructions and, over long times, by the power cap:
 // 8192 x 131072 x 1024 logits in bf16 take 1.39 ms in a single run (1.58 PFLOP/s, 0.93 of the measured burst
-// rate) and 1.47 in a row (1.40 GHz); d and both gradients of the same sizes 5.5 ms (1.2 PFLOP/s).
+// rate) and 1.5 in a row (1.40 GHz); d and both gradients of the same sizes 5.5 to 5.7 ms (1.2 PFLOP/s).
 // fp32 operands are split into two fp16 numbers (after a common power-of-two scale), x = hi + lo, and
 // hi hi + hi lo + lo hi computed: 22 bits of each operand.  Products of fp16 or bf16 operands are exact in
 // the fp32 accumulators.  d is rounded once to the operands' type (fp32: to hi + lo with lo scaled by
