@@ -124,3 +124,24 @@ def test_operands_at_the_ends_of_the_range(big, small):
     e = (32 * U + 2.0 ** -20) * (x[0].double().abs() @ x[1].double().abs().T).amax(1) + 2.0 ** -20 * (1 + f["lse"].abs())
     assert torch.all((got[1].cpu().double() - f["lse"]).abs() <= e)
     assert torch.isfinite(got[2]).all() and torch.isfinite(got[3]).all()
+
+
+@pytest.mark.parametrize("size", [2.0 ** 10, 2.0 ** 13.5])
+@pytest.mark.parametrize("n,vocab,dim", SIZES)
+def test_a_large_row_that_one_scale_still_serves(n, vocab, dim, size):
+    """Just below the border to three parts.  dw is held to 22 bits of its rows' largest numbers: an element far
+    below its row's largest has fewer bits of its own."""
+    hidden, weight, targets, gloss = inputs(n, vocab, dim, 2, "f32")
+    hidden[7] *= size
+    targets[7] = -1
+    rows = torch.ones(n, dtype=torch.bool)
+    rows[7] = False
+    got = run(hidden, weight, targets, gloss)
+    hold_some(got, hidden, weight, targets, gloss, rows)
+    f = formula(hidden, weight, targets, gloss)
+    h = hidden.double().abs()[rows].amax(1, keepdim=True).expand(-1, dim)
+    size = f["d"][rows].abs().T @ h
+    e = (dim * U + 2.0 ** -20) * (hidden.double().abs()[rows] @ weight.double().abs().T).amax(1) + 2.0 ** -20 * (1 + f["lse"][rows].abs())
+    off = (2 * e + 2.0 ** -20)[:, None] * f["prob"][rows].abs()
+    bound = 1.001 * off.T @ h + (2 * U * (n + 64) + 2.0 ** -20 + 2.0 ** -22) * size + 2 * U * f["dw"].abs() + 2.0 ** -126
+    assert torch.all((got[3].double().cpu() - f["dw"]).abs() <= bound)
